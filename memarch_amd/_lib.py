@@ -1,4 +1,4 @@
-"""ctypes binding of libmce.so (declarations in include/mce.h).
+"""ctypes binding of libmce.so (declarations in include/mce.h) and libmce_attn.so (include/mce_attn.h).
 
 torch is imported before the library is loaded: torch ships its own libamdhip64.so with the same SONAME as
 /opt/rocm's, so loading torch first makes libmce.so bind to the one HIP runtime that owns torch's streams
@@ -11,8 +11,10 @@ import torch  # noqa: F401  (must precede the CDLL load, see module docstring)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmce.so")
+ATTN_LIB_PATH = os.path.join(HERE, "libmce_attn.so")
 
 _P = ctypes.c_void_p
+_F = ctypes.c_float
 _I = ctypes.c_int64
 _S = ctypes.c_size_t
 _INT = ctypes.c_int
@@ -67,7 +69,18 @@ SIGNATURES = {
     "mce_swiglu_last_hip_error": (_INT, []),
 }
 
+# the attention library, in the order of include/mce_attn.h
+_TENSOR = [_P, _I, _I, _I]   # pointer and element strides (batch, token, head)
+ATTN_SIGNATURES = {
+    "mce_attn_error_string": (ctypes.c_char_p, [_INT]),
+    "mce_attn_last_hip_error": (_INT, []),
+    "mce_attn_fwd": (_INT, 3 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P]),
+    "mce_attn_bwd_ws_bytes": (_S, 7 * [_I]),
+    "mce_attn_bwd": (_INT, 4 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P, _P, _P, _P, _S, _P]),
+}
+
 _lib = None
+_attn_lib = None
 _call_hook = None  # optional callable(name, phase) run around every C-ABI call, phase "begin" / "end"
 
 
@@ -75,23 +88,39 @@ class MceError(RuntimeError):
     pass
 
 
+def _load(path, signatures):
+    if not os.path.exists(path):
+        raise MceError(f"{path} is missing; build it with `python -m memarch_amd.build`")
+    lib = ctypes.CDLL(path)
+    for name, (res, args) in signatures.items():
+        fn = getattr(lib, name)
+        fn.restype = res
+        fn.argtypes = args
+    return lib
+
+
 def load():
     """Load libmce.so once. Raises if the library has not been built: there is no fallback path."""
     global _lib
     if _lib is None:
-        if not os.path.exists(LIB_PATH):
-            raise MceError(f"{LIB_PATH} is missing; build it with `python -m memarch_amd.build`")
-        lib = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
-            fn = getattr(lib, name)
-            fn.restype = res
-            fn.argtypes = args
-        _lib = lib
+        _lib = _load(LIB_PATH, SIGNATURES)
     return _lib
+
+
+def load_attn():
+    """Load libmce_attn.so once. Raises if the library has not been built: there is no fallback path."""
+    global _attn_lib
+    if _attn_lib is None:
+        _attn_lib = _load(ATTN_LIB_PATH, ATTN_SIGNATURES)
+    return _attn_lib
 
 
 def check(rc, what):
     if rc != 0:
+        if what in ATTN_SIGNATURES:
+            lib = load_attn()
+            msg = lib.mce_attn_error_string(rc).decode()
+            raise MceError(f"{what} failed: {msg} (code {rc}, hipError {lib.mce_attn_last_hip_error()})")
         lib = load()
         msg = lib.mce_error_string(rc).decode()
         hip = lib.mce_last_hip_error()
@@ -110,6 +139,7 @@ def call(name, *args):
     hook = _call_hook
     if hook is not None:
         hook(name, "begin")
-    check(getattr(load(), name)(*args), name)
+    lib = load_attn() if name in ATTN_SIGNATURES else load()
+    check(getattr(lib, name)(*args), name)
     if hook is not None:
         hook(name, "end")

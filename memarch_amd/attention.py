@@ -1,0 +1,167 @@
+"""Causal attention over a sliding window with first tokens that stay visible, on MI355X (libmce_attn.so).
+
+`window_attention(q, k, v, window, sinks, lengths)` stands where memarch's blocks call scaled_dot_product_attention or
+their block-window helpers (lm.py:448-554, full2.py:154-181): one kernel forward, two backward, no scores in memory.
+Position i of a sequence sees position j <= i when i - j < window or j < sinks. Products take bf16 or fp16 operands and
+sum in fp32; softmax statistics are fp32 (include/mce_attn.h). All device work runs on torch's current stream; a tensor
+that is not on a GPU raises, and there is no other code path.
+"""
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .fused_ops import _ptr, _stream
+
+# element-type codes of include/mce_attn.h
+_DTYPES = {torch.bfloat16: 1, torch.float16: 2}
+MAX_HEAD_DIM = 128
+_MAX_STRIDE = 1 << 21   # elements between two tokens (the library's limit)
+
+
+def _check_same(ref, *named):
+    """All tensors on ref's GPU."""
+    for name, t in named:
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
+    if not ref.is_cuda:
+        raise ValueError("memarch_amd.attention runs on the GPU only; got a tensor on " + str(ref.device))
+
+
+class _On:
+    """Makes the tensors' GPU current around a launch if it is not (a launch goes to the current device)."""
+
+    def __init__(self, dev):
+        self.dev = dev
+        self.prev = -1
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if cur != self.dev.index:
+            self.prev = cur
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.prev >= 0:
+            torch.cuda.set_device(self.prev)
+
+
+def _strided(t):
+    """(tensor, (pointer, batch, token, head strides)) of a [B, T, H, D] operand: the tensor itself when the library
+    can read it where it lies (contiguous last dimension, 16-byte alignment, tokens at least D apart), else a
+    contiguous copy."""
+    t = t.detach()
+    b, n, h, d = t.shape
+    sb, st, sh, sd = t.stride()
+    sb, st, sh = sb if b > 1 else 0, st if n > 1 else d, sh if h > 1 else 0
+    if sd != 1 or (sb | st | sh) & 7 or not d <= st <= _MAX_STRIDE or t.data_ptr() & 15:
+        t = t.contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone()
+        sb, st, sh = n * h * d, h * d, d
+    return t, (t.data_ptr(), sb, st, sh)
+
+
+def _lengths(lengths, b, most):
+    """[B] int32 device lengths (None: all of them whole); values outside 0 .. most count as the nearest of the two."""
+    if lengths is None:
+        return None
+    if lengths.dim() != 1 or lengths.shape[0] != b or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"lengths must be [B={b}] int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
+    if lengths.dtype is torch.int64:
+        lengths = lengths.clamp(0, most).int()
+    return lengths.contiguous()
+
+
+def _mask_args(window, sinks):
+    window = 0 if window is None else int(window)
+    if window < 0 or (window == 0 and sinks):
+        raise ValueError("window must be at least 1 (None: every earlier position is seen, without sinks)")
+    if sinks < 0:
+        raise ValueError(f"sinks={sinks} must not be negative")
+    return window, int(sinks)
+
+
+def _scale(scale, d):
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"scale={scale} must be positive and finite")
+    return scale
+
+
+def _check_heads(q, k, v, what):
+    if k.shape != v.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
+    if q.shape[-1] != k.shape[-1] or q.shape[-1] % 8 or not 8 <= q.shape[-1] <= MAX_HEAD_DIM:
+        raise ValueError(f"the head dimension must be a multiple of 8 up to {MAX_HEAD_DIM}, alike for all, got "
+                         f"{q.shape[-1]} and {k.shape[-1]}")
+    if k.shape[-2] < 1 or q.shape[-2] < 1 or q.shape[-2] % k.shape[-2]:
+        raise ValueError(f"{q.shape[-2]} query heads cannot share {k.shape[-2]} key/value heads")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{what} must all be bfloat16 or all float16, got {q.dtype}, {k.dtype} and {v.dtype}")
+
+
+def _forward(q, k, v, lengths, window, sinks, scale, need_lse):
+    B, T, Hq, D = q.shape
+    (q, qs), (k, ks), (v, vs) = _strided(q), _strided(k), _strided(v)
+    out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device) if need_lse else None
+    with _On(q.device):
+        _lib.call("mce_attn_fwd", *qs, *ks, *vs, _ptr(lengths), B, T, Hq, k.shape[2], D, window, sinks, scale,
+                  _DTYPES[q.dtype], out.data_ptr(), _ptr(lse), _stream(q.device))
+    return q, k, v, out, lse
+
+
+class _WindowAttention(torch.autograd.Function):
+    """forward(ctx, q, k, v, lengths, window, sinks, scale) -> out; backward -> dq, dk, dv."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, window, sinks, scale):
+        q, k, v, out, lse = _forward(q, k, v, lengths, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        ctx.mask = (window, sinks, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go):
+        q, k, v, out, lse, lengths = ctx.saved_tensors
+        window, sinks, scale = ctx.mask
+        B, T, Hq, D = q.shape
+        Hkv = k.shape[2]
+        (q, qs), (k, ks), (v, vs), (go, gs) = _strided(q), _strided(k), _strided(v), _strided(go)
+        dq = torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device)
+        dk = torch.empty(B, T, Hkv, D, dtype=q.dtype, device=q.device)
+        dv = torch.empty_like(dk)
+        n = _lib.load_attn().mce_attn_bwd_ws_bytes(B, T, Hq, Hkv, D, window, sinks)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        with _On(q.device):
+            _lib.call("mce_attn_bwd", *qs, *ks, *vs, *gs, _ptr(lengths), B, T, Hq, Hkv, D, window, sinks, scale,
+                      _DTYPES[q.dtype], out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                      ws.data_ptr(), n, _stream(q.device))
+        return dq, dk, dv, None, None, None, None
+
+
+@torch.compiler.disable
+def window_attention(q, k, v, window=None, sinks=0, lengths=None, scale=None):
+    """Causal attention of q [B, T, Hq, D] over k, v [B, T, Hkv, D] (bf16 or fp16, Hq a multiple of Hkv, D a multiple of
+    8 up to 128, any strides) -> [B, T, Hq, D]. Position i sees j <= i with i - j < window or j < sinks (window None:
+    every j <= i). lengths [B] marks a padded batch: positions at or past a sequence's length see nothing and are seen
+    by none, their output and gradients are 0 and what lies in their rows is not read. scale defaults to D^-0.5.
+    Under torch.autocast fp32 tensors are cast to its type, as for scaled_dot_product_attention. Differentiable once
+    in q, k and v."""
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        q, k, v = (t.to(dt) if t.dtype is torch.float32 else t for t in (q, k, v))
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or q.shape[:2] != k.shape[:2]:
+        raise ValueError(f"q {tuple(q.shape)} must be [B, T, Hq, D], k {tuple(k.shape)} and v {tuple(v.shape)} "
+                         "[B, T, Hkv, D]")
+    _check_heads(q, k, v, "q, k and v")
+    window, sinks = _mask_args(window, sinks)
+    scale = _scale(scale, q.shape[3])
+    lengths = _lengths(lengths, q.shape[0], q.shape[1])
+    _check_same(q, ("k", k), ("v", v), ("lengths", lengths))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
+    return _forward(q, k, v, lengths, window, sinks, scale, False)[3]

@@ -1,0 +1,512 @@
+// attn.hip — causal attention over a sliding window with first tokens that stay visible, forward and backward, for
+// MI355X (gfx950). The C ABI is in include/mce_attn.h; tiles and fragments are in attn_tile.h.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/mce_attn.h"
+#include "attn_tile.h"
+
+namespace {
+
+using namespace attn;
+
+constexpr int NW = 4;               // waves per workgroup
+constexpr int THREADS = 64 * NW;
+constexpr int BQ = 32 * NW;         // query rows per workgroup of k_attn_fwd and k_attn_dq (32 per wave)
+constexpr int BK = 64;              // keys per tile there
+constexpr int BKV = 32 * NW;        // keys per workgroup of k_attn_dkv (32 per wave)
+constexpr int BR = 32;              // query rows per tile there
+
+struct Strided {
+  const uint16_t* p;
+  int64_t sb, st, sh;  // elements between batches, tokens, heads
+};
+
+struct Args {
+  Strided q, k, v, go;
+  const uint16_t* out;       // contiguous [B, T, Hq, D]
+  uint16_t *o, *dq, *dk, *dv;
+  float* lse;                // [B, Hq, T]
+  float* delta;              // [B, Hq, T]
+  const int32_t* lengths;
+  int B, T, Hq, Hkv, grp, D;
+  int window, sinks;         // window = INT32_MAX: none
+  float scale;
+};
+
+__device__ __forceinline__ int seq_len(const Args& a, int b) {
+  if (a.lengths == nullptr) return a.T;
+  const int n = a.lengths[b];
+  return n < 0 ? 0 : (n > a.T ? a.T : n);
+}
+
+// The key tiles that rows q0 .. q1 (inclusive) see: those of the first `sinks` positions (n_sink tiles from 0) and then
+// those from tile `lo` to tile `hi`.
+struct KeyTiles {
+  int n_sink, lo, n;
+  __device__ __forceinline__ KeyTiles(const Args& a, int q0, int q1) {
+    const int first = q0 - a.window + 1;   // first key of the window of row q0
+    lo = first <= 0 ? 0 : first / BK;
+    n_sink = (a.sinks + BK - 1) / BK;
+    n_sink = n_sink < lo ? n_sink : lo;
+    n = n_sink + q1 / BK - lo + 1;
+  }
+  __device__ __forceinline__ int key0(int it) const { return (it < n_sink ? it : lo + it - n_sink) * BK; }
+};
+
+// Masks a 32 x 32 block of scores held as [keys][rows]: accumulator element e of lane l is key
+// k0 + 8*(e/4) + 4*(l/32) + e%4 and row `row` (of lane l%32).
+__device__ __forceinline__ void mask_keys(f32x16& s, int row, int k0h, int window, int sinks, float fill) {
+  const int rel = row - k0h;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int c = 8 * (e / 4) + e % 4;
+    const bool see = (uint32_t)(rel - c) < (uint32_t)window || (k0h + c < sinks && rel - c >= 0);
+    s[e] = see ? s[e] : fill;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- forward
+template <typename T, int DP>
+__global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
+  constexpr int IMG = BK * DP * 2;                     // bytes of a tile
+  __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];   // K and V, two tiles each
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int nq = (a.T + BQ - 1) / BQ;
+  const int qb = nq - 1 - blockIdx.x % nq;             // the rows with the most keys first
+  const int bh = blockIdx.x / nq, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / a.grp;
+  const int len = seq_len(a, b);
+  const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
+  uint16_t* const op = a.o + ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
+  float* const lp = a.lse == nullptr ? nullptr : a.lse + (int64_t)bh * a.T + row;
+  f32x16 acc[DP / 32] = {};
+  float m = -INFINITY, l = 0.f;
+  const float c = a.scale * LOG2E;
+  if (q0 < len) {
+    const int q1 = (q0 + BQ < len ? q0 + BQ : len) - 1;
+    const KeyTiles kt(a, q0, q1);
+    FragAddr<DP> ad;
+    ad.init(lane);
+    TileLoad<DP, BK, NW> tk, tv;
+    tk.init((int)a.k.st * 2, a.D, wave, lane);
+    tv.init((int)a.v.st * 2, a.D, wave, lane);
+    const uint16_t* const kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+    const uint16_t* const vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+    auto issue = [&](int it, int buf) {
+      const int k0 = kt.key0(it);
+      tk.issue(tile_rsrc<BK>(kp, a.k.st, k0, len, a.D), lds, buf * 2 * IMG, wave);
+      tv.issue(tile_rsrc<BK>(vp, a.v.st, k0, len, a.D), lds, buf * 2 * IMG + IMG, wave);
+    };
+    issue(0, 0);
+    // the wave's query rows as fragments: row l%32, columns 16 ks + 8 h + 0..7
+    u32x4 qf[DP / 16];
+    const i32x4 qr = tile_rsrc<32>(a.q.p + b * a.q.sb + hq * a.q.sh, a.q.st, r0, len, a.D);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int col = 16 * ks + 8 * h;
+      qf[ks] = load16(qr, col < a.D ? (lane & 31) * (int)a.q.st * 2 + col * 2 : OOB);
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+    for (int it = 0; it < kt.n; ++it) {
+      const int img = (it & 1) * 2 * IMG;
+      if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
+      const int k0 = kt.key0(it);
+      const bool none = k0 > r0 + 31;                  // every key of the tile lies behind the wave's rows
+      if (!none) {
+        f32x16 s[2] = {};
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int ks = 0; ks < DP / 16; ++ks) s[kb] = mfma<T>(frag_rows<DP>(lds, ad, img, kb, ks), qf[ks], s[kb]);
+        const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
+        if (!all) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) mask_keys(s[kb], row, k0 + 32 * kb + 4 * h, a.window, a.sinks, -INFINITY);
+        }
+        float mx = m;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
+        mx = max_halves(mx);
+        const float mu = mx == -INFINITY ? 0.f : mx;   // a row that has seen nothing yet
+        const float al = __builtin_amdgcn_exp2f((m - mu) * c);
+        m = mx;
+        l *= al;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= al;
+        const float mc = mu * c;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e], c, -mc));
+            l += s[kb][e];
+          }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const u32x4 pf = frag_acc<T>(s[kk >> 1], kk & 1);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = mfma<T>(frag_tr<DP>(lds, ad, img + IMG, dt, kk), pf, acc[dt]);
+        }
+      }
+      wait_vmcnt<0>();
+      __syncthreads();
+    }
+  }
+  l = sum_halves(l);
+  const bool in = row < a.T, see = row < len;
+  const float inv = see ? 1.f / l : 0.f;
+  store_acc<T, DP>(acc, inv, op, a.D, in, h);
+  if (lp != nullptr && in && h == 0) *lp = see ? m + __builtin_amdgcn_logf(l) / c : INFINITY;
+}
+
+// --------------------------------------------------------------------------------------------------------------- dq
+template <typename T, int DP>
+__global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
+  constexpr int IMG = BK * DP * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int nq = (a.T + BQ - 1) / BQ;
+  const int qb = nq - 1 - blockIdx.x % nq;
+  const int bh = blockIdx.x / nq, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / a.grp;
+  const int len = seq_len(a, b);
+  const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
+  const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
+  f32x16 acc[DP / 32] = {};
+  float delta = 0.f;
+  const float c = a.scale * LOG2E;
+  if (q0 < len) {
+    const int q1 = (q0 + BQ < len ? q0 + BQ : len) - 1;
+    const KeyTiles kt(a, q0, q1);
+    FragAddr<DP> ad;
+    ad.init(lane);
+    TileLoad<DP, BK, NW> tk, tv;
+    tk.init((int)a.k.st * 2, a.D, wave, lane);
+    tv.init((int)a.v.st * 2, a.D, wave, lane);
+    const uint16_t* const kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+    const uint16_t* const vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+    auto issue = [&](int it, int buf) {
+      const int k0 = kt.key0(it);
+      tk.issue(tile_rsrc<BK>(kp, a.k.st, k0, len, a.D), lds, buf * 2 * IMG, wave);
+      tv.issue(tile_rsrc<BK>(vp, a.v.st, k0, len, a.D), lds, buf * 2 * IMG + IMG, wave);
+    };
+    issue(0, 0);
+    u32x4 qf[DP / 16], gf[DP / 16];
+    const i32x4 qr = tile_rsrc<32>(a.q.p + b * a.q.sb + hq * a.q.sh, a.q.st, r0, len, a.D);
+    const i32x4 gr = tile_rsrc<32>(a.go.p + b * a.go.sb + hq * a.go.sh, a.go.st, r0, len, a.D);
+    const i32x4 orr = tile_rsrc<32>(a.out + (int64_t)b * a.T * a.Hq * a.D + (int64_t)hq * a.D, (int64_t)a.Hq * a.D, r0,
+                                    len, a.D);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int col = 16 * ks + 8 * h, r = lane & 31;
+      qf[ks] = load16(qr, col < a.D ? r * (int)a.q.st * 2 + col * 2 : OOB);
+      gf[ks] = load16(gr, col < a.D ? r * (int)a.go.st * 2 + col * 2 : OOB);
+      const u32x4 of = load16(orr, col < a.D ? r * a.Hq * a.D * 2 + col * 2 : OOB);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        delta = __builtin_fmaf(lo_f32<T>(gf[ks][e]), lo_f32<T>(of[e]), delta);
+        delta = __builtin_fmaf(hi_f32<T>(gf[ks][e]), hi_f32<T>(of[e]), delta);
+      }
+    }
+    delta = sum_halves(delta);
+    const float nl = row < len ? -a.lse[(int64_t)bh * a.T + row] : -INFINITY;
+    wait_vmcnt<0>();
+    __syncthreads();
+    for (int it = 0; it < kt.n; ++it) {
+      const int img = (it & 1) * 2 * IMG;
+      if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
+      const int k0 = kt.key0(it);
+      if (k0 <= r0 + 31) {
+        const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          f32x16 s, ds;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = nl;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ds[e] = -delta;
+#pragma unroll
+          for (int ks = 0; ks < DP / 16; ++ks) s = mfma<T>(frag_rows<DP>(lds, ad, img, kb, ks), qf[ks], s);
+#pragma unroll
+          for (int ks = 0; ks < DP / 16; ++ks) ds = mfma<T>(frag_rows<DP>(lds, ad, img + IMG, kb, ks), gf[ks], ds);
+          if (!all) mask_keys(s, row, k0 + 32 * kb + 4 * h, a.window, a.sinks, -INFINITY);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ds[e] *= __builtin_amdgcn_exp2f(s[e] * c);
+#pragma unroll
+          for (int sl = 0; sl < 2; ++sl) {
+            const u32x4 df = frag_acc<T>(ds, sl);
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+              acc[dt] = mfma<T>(frag_tr<DP>(lds, ad, img, dt, 2 * kb + sl), df, acc[dt]);
+          }
+        }
+      }
+      wait_vmcnt<0>();
+      __syncthreads();
+    }
+  }
+  const bool in = row < a.T;
+  store_acc<T, DP>(acc, a.scale, a.dq + ofs, a.D, in, h);
+  if (in && h == 0) a.delta[(int64_t)bh * a.T + row] = row < len ? delta : 0.f;
+}
+
+// ---------------------------------------------------------------------------------------------------------- dk, dv
+template <typename T, int DP>
+__global__ __launch_bounds__(THREADS, 1) void k_attn_dkv(Args a) {
+  constexpr int IMG = BR * DP * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];   // Q and go, two tiles each
+  __shared__ float stats[2][2][BR];                              // -lse and -delta of the tile's rows
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int nk = (a.T + BKV - 1) / BKV;
+  const int kblk = blockIdx.x % nk;                    // the keys with the most rows first
+  const int bh = blockIdx.x / nk, b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int len = seq_len(a, b);
+  const int kb0 = kblk * BKV, j0 = kb0 + wave * 32, key = j0 + (lane & 31);
+  f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+  const float c = a.scale * LOG2E;
+  if (kb0 < len) {
+    // rows kb0 .. q_end - 1 may see a key of the block
+    int64_t q_end64 = kb0 < a.sinks ? len : (int64_t)kb0 + BKV - 1 + a.window;
+    const int q_end = q_end64 < len ? (int)q_end64 : len;
+    const int t0 = kb0 / BR, nt = (q_end + BR - 1) / BR - t0, total = nt * a.grp;
+    FragAddr<DP> ad;
+    ad.init(lane);
+    TileLoad<DP, BR, NW> tq, tg;
+    tq.init((int)a.q.st * 2, a.D, wave, lane);
+    tg.init((int)a.go.st * 2, a.D, wave, lane);
+    float st0 = 0.f;
+    auto issue = [&](int it, int buf) {
+      const int g = it / nt, i0 = (t0 + it - g * nt) * BR, hq = hk * a.grp + g;
+      tq.issue(tile_rsrc<BR>(a.q.p + b * a.q.sb + hq * a.q.sh, a.q.st, i0, len, a.D), lds, buf * 2 * IMG, wave);
+      tg.issue(tile_rsrc<BR>(a.go.p + b * a.go.sb + hq * a.go.sh, a.go.st, i0, len, a.D), lds, buf * 2 * IMG + IMG, wave);
+      if (threadIdx.x < 2 * BR) {
+        const int r = i0 + (threadIdx.x & (BR - 1));
+        const int64_t o = ((int64_t)b * a.Hq + hq) * a.T + r;
+        st0 = threadIdx.x < BR ? (r < len ? -a.lse[o] : -INFINITY) : (r < len ? -a.delta[o] : 0.f);
+      }
+    };
+    auto put = [&](int buf) {
+      if (threadIdx.x < 2 * BR) stats[buf][threadIdx.x / BR][threadIdx.x & (BR - 1)] = st0;
+    };
+    issue(0, 0);
+    u32x4 kf[DP / 16], vf[DP / 16];
+    const i32x4 kr = tile_rsrc<32>(a.k.p + b * a.k.sb + hk * a.k.sh, a.k.st, j0, len, a.D);
+    const i32x4 vr = tile_rsrc<32>(a.v.p + b * a.v.sb + hk * a.v.sh, a.v.st, j0, len, a.D);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int col = 16 * ks + 8 * h, r = lane & 31;
+      kf[ks] = load16(kr, col < a.D ? r * (int)a.k.st * 2 + col * 2 : OOB);
+      vf[ks] = load16(vr, col < a.D ? r * (int)a.v.st * 2 + col * 2 : OOB);
+    }
+    put(0);
+    wait_vmcnt<0>();
+    __syncthreads();
+    for (int it = 0; it < total; ++it) {
+      const int buf = it & 1, img = buf * 2 * IMG;
+      if (it + 1 < total) issue(it + 1, buf ^ 1);
+      const int i0 = (t0 + it % nt) * BR;
+      const bool some = i0 + BR - 1 >= j0 && (i0 - (j0 + 31) < a.window || j0 < a.sinks);
+      if (some) {
+        f32x16 s, ds;
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(&stats[buf][0][8 * e4 + 4 * h]);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(&stats[buf][1][8 * e4 + 4 * h]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[4 * e4 + e] = x[e];
+            ds[4 * e4 + e] = y[e];
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) s = mfma<T>(frag_rows<DP>(lds, ad, img, 0, ks), kf[ks], s);
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) ds = mfma<T>(frag_rows<DP>(lds, ad, img + IMG, 0, ks), vf[ks], ds);
+        const bool all = j0 + 31 <= i0 && i0 + BR - 1 - j0 < a.window;
+        if (!all) {
+          const int rel = i0 + 4 * h - key;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int d = rel + 8 * (e / 4) + e % 4;
+            s[e] = (uint32_t)d < (uint32_t)a.window || (key < a.sinks && d >= 0) ? s[e] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[e] = __builtin_amdgcn_exp2f(s[e] * c);
+          ds[e] *= s[e];
+        }
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl) {
+          const u32x4 pf = frag_acc<T>(s, sl), df = frag_acc<T>(ds, sl);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt) dv[dt] = mfma<T>(frag_tr<DP>(lds, ad, img + IMG, dt, sl), pf, dv[dt]);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt) dk[dt] = mfma<T>(frag_tr<DP>(lds, ad, img, dt, sl), df, dk[dt]);
+        }
+      }
+      put(buf ^ 1);
+      wait_vmcnt<0>();
+      __syncthreads();
+    }
+  }
+  const int64_t ofs = (((int64_t)b * a.T + key) * a.Hkv + hk) * a.D;
+  const bool in = key < a.T;
+  store_acc<T, DP>(dk, a.scale, a.dk + ofs, a.D, in, h);
+  store_acc<T, DP>(dv, 1.f, a.dv + ofs, a.D, in, h);
+}
+
+// -------------------------------------------------------------------------------------------------------- host side
+thread_local int g_hip_error = 0;   // the calling thread's last failed launch
+
+int finish() {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) {
+    g_hip_error = (int)e;
+    return MCE_ATTN_ELAUNCH;
+  }
+  return MCE_ATTN_OK;
+}
+
+// Token strides up to 2^21 elements keep every offset inside a tile of at most 128 rows in 31 bits.
+constexpr int64_t MAX_ST = int64_t(1) << 21;
+
+int check_strided(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t D) {
+  if (p == nullptr || sb < 0 || sh < 0 || st < D || st > MAX_ST) return MCE_ATTN_EINVAL;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) || (sb | st | sh) % 8) return MCE_ATTN_EALIGN;
+  return MCE_ATTN_OK;
+}
+
+int check_sizes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
+  if (B < 0 || T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || D > 128 || D % 8 || window < 0 || sinks < 0)
+    return MCE_ATTN_EINVAL;
+  if (T > (int64_t(1) << 30) || Hq * D > MAX_ST) return MCE_ATTN_EINVAL;
+  // one workgroup per 128 rows of every head
+  if (T > 0 && (B > (int64_t(1) << 31) / Hq || B * Hq * ((T + 127) / 128) >= (int64_t(1) << 31)))
+    return MCE_ATTN_EINVAL;
+  return MCE_ATTN_OK;
+}
+
+Args make_args(Strided q, Strided k, Strided v, const int32_t* lengths, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+               int64_t D, int64_t window, int64_t sinks, float scale) {
+  Args a = {};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.lengths = lengths;
+  a.B = (int)B;
+  a.T = (int)T;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.grp = (int)(Hq / Hkv);
+  a.D = (int)D;
+  a.window = window == 0 || window > T ? INT32_MAX : (int)window;
+  a.sinks = a.window == INT32_MAX ? 0 : (int)(sinks > T ? T : sinks);
+  a.scale = scale;
+  return a;
+}
+
+template <typename T, int DP>
+int launch_fwd(const Args& a, hipStream_t st) {
+  const unsigned n = (unsigned)((int64_t)a.B * a.Hq * ((a.T + BQ - 1) / BQ));
+  hipLaunchKernelGGL((k_attn_fwd<T, DP>), dim3(n), dim3(THREADS), 0, st, a);
+  return finish();
+}
+
+template <typename T, int DP>
+int launch_bwd(const Args& a, hipStream_t st) {
+  const unsigned n = (unsigned)((int64_t)a.B * a.Hq * ((a.T + BQ - 1) / BQ));
+  hipLaunchKernelGGL((k_attn_dq<T, DP>), dim3(n), dim3(THREADS), 0, st, a);
+  const unsigned nk = (unsigned)((int64_t)a.B * a.Hkv * ((a.T + BKV - 1) / BKV));
+  hipLaunchKernelGGL((k_attn_dkv<T, DP>), dim3(nk), dim3(THREADS), 0, st, a);
+  return finish();
+}
+
+bool good_scale(float s) { return s > 0.f && s <= 3.0e38f; }
+
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" {
+
+const char* mce_attn_error_string(int code) {
+  switch (code) {
+    case MCE_ATTN_OK: return "ok";
+    case MCE_ATTN_EINVAL: return "invalid argument (size, stride, head count, scale, element type or null pointer)";
+    case MCE_ATTN_EALIGN: return "misaligned (pointers must be 16-byte aligned, strides multiples of 8 elements)";
+    case MCE_ATTN_EWORKSPACE: return "workspace missing, too small or not 256-byte aligned";
+    case MCE_ATTN_ELAUNCH: return "a HIP launch failed";
+    default: return "unknown error";
+  }
+}
+
+int mce_attn_last_hip_error(void) { return g_hip_error; }
+
+int mce_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
+                 int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const int32_t* lengths,
+                 int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks, float scale,
+                 int dtype, void* out, float* lse, void* stream) {
+  int rc = check_sizes(B, T, Hq, Hkv, D, window, sinks);
+  if (rc) return rc;
+  if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16)) return MCE_ATTN_EINVAL;
+  if (B == 0 || T == 0) return MCE_ATTN_OK;
+  if ((rc = check_strided(q, q_sb, q_st, q_sh, D)) || (rc = check_strided(k, k_sb, k_st, k_sh, D)) ||
+      (rc = check_strided(v, v_sb, v_st, v_sh, D)))
+    return rc;
+  if (out == nullptr) return MCE_ATTN_EINVAL;
+  if (reinterpret_cast<uintptr_t>(out) & 15) return MCE_ATTN_EALIGN;
+  Args a = make_args({static_cast<const uint16_t*>(q), q_sb, q_st, q_sh},
+                     {static_cast<const uint16_t*>(k), k_sb, k_st, k_sh},
+                     {static_cast<const uint16_t*>(v), v_sb, v_st, v_sh}, lengths, B, T, Hq, Hkv, D, window, sinks,
+                     scale);
+  a.o = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == MCE_ATTN_BF16) return D <= 64 ? launch_fwd<__bf16, 64>(a, st) : launch_fwd<__bf16, 128>(a, st);
+  return D <= 64 ? launch_fwd<_Float16, 64>(a, st) : launch_fwd<_Float16, 128>(a, st);
+}
+
+size_t mce_attn_bwd_ws_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                             int64_t sinks) {
+  if (check_sizes(B, T, Hq, Hkv, D, window, sinks)) return 0;
+  return (size_t)align256(B * Hq * T * 4);
+}
+
+int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
+                 int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const void* go, int64_t go_sb,
+                 int64_t go_st, int64_t go_sh, const int32_t* lengths, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                 int64_t D, int64_t window, int64_t sinks, float scale, int dtype, const void* out, const float* lse,
+                 void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_sizes(B, T, Hq, Hkv, D, window, sinks);
+  if (rc) return rc;
+  if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16)) return MCE_ATTN_EINVAL;
+  if (B == 0 || T == 0) return MCE_ATTN_OK;
+  if ((rc = check_strided(q, q_sb, q_st, q_sh, D)) || (rc = check_strided(k, k_sb, k_st, k_sh, D)) ||
+      (rc = check_strided(v, v_sb, v_st, v_sh, D)) || (rc = check_strided(go, go_sb, go_st, go_sh, D)))
+    return rc;
+  if (out == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr) return MCE_ATTN_EINVAL;
+  for (const void* p : {out, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return MCE_ATTN_EALIGN;
+  if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) ||
+      ws_bytes < mce_attn_bwd_ws_bytes(B, T, Hq, Hkv, D, window, sinks))
+    return MCE_ATTN_EWORKSPACE;
+  Args a = make_args({static_cast<const uint16_t*>(q), q_sb, q_st, q_sh},
+                     {static_cast<const uint16_t*>(k), k_sb, k_st, k_sh},
+                     {static_cast<const uint16_t*>(v), v_sb, v_st, v_sh}, lengths, B, T, Hq, Hkv, D, window, sinks,
+                     scale);
+  a.go = {static_cast<const uint16_t*>(go), go_sb, go_st, go_sh};
+  a.out = static_cast<const uint16_t*>(out);
+  a.lse = const_cast<float*>(lse);
+  a.delta = static_cast<float*>(ws);
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == MCE_ATTN_BF16) return D <= 64 ? launch_bwd<__bf16, 64>(a, st) : launch_bwd<__bf16, 128>(a, st);
+  return D <= 64 ? launch_bwd<_Float16, 64>(a, st) : launch_bwd<_Float16, 128>(a, st);
+}
+
+}  // extern "C"
