@@ -52,14 +52,17 @@ extern "C" {
 MCE_ATTN_API const char* mce_attn_error_string(int code);
 MCE_ATTN_API int mce_attn_last_hip_error(void);
 
-/* out, and for a backward lse (may be NULL): log of the softmax's denominator in units of q . k, +inf on empty rows. */
+/* out, and for a backward (both may be NULL) lse, the log of the softmax's denominator in units of q . k, +inf on empty
+ * rows, and res [B, T, Hq, D], what out's rounding left over: d_i = go_i . (out_i + res_i). Without res, d would carry
+ * out's rounding into every ds of its row, where nothing averages it: at T = 4 that alone put dq off by 4e-3 of its norm
+ * in bf16 (1.6e-3 is dq's own rounding). */
 MCE_ATTN_API int mce_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
                               int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
                               const int32_t* lengths, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
-                              int64_t window, int64_t sinks, float scale, int dtype, void* out, float* lse,
-                              void* stream);
+                              int64_t window, int64_t sinks, float scale, int dtype, void* out, void* res,
+                              float* lse, void* stream);
 
-/* dq, dk and dv from the forward's inputs, out and lse. The workspace holds d (fp32 [B, Hq, T]) and, where the sums of
+/* dq, dk and dv from the forward's inputs, out, res and lse. The workspace holds d (fp32 [B, Hq, T]) and, where the sums of
  * dk and dv are split over workgroups, their fp32 parts. */
 MCE_ATTN_API size_t mce_attn_bwd_ws_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                                           int64_t sinks);
@@ -67,8 +70,8 @@ MCE_ATTN_API int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t
                               int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
                               const void* go, int64_t go_sb, int64_t go_st, int64_t go_sh, const int32_t* lengths,
                               int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks,
-                              float scale, int dtype, const void* out, const float* lse, void* dq, void* dk, void* dv,
-                              void* ws, size_t ws_bytes, void* stream);
+                              float scale, int dtype, const void* out, const void* res, const float* lse, void* dq,
+                              void* dk, void* dv, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

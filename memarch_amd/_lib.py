@@ -74,9 +74,9 @@ _TENSOR = [_P, _I, _I, _I]   # pointer and element strides (batch, token, head)
 ATTN_SIGNATURES = {
     "mce_attn_error_string": (ctypes.c_char_p, [_INT]),
     "mce_attn_last_hip_error": (_INT, []),
-    "mce_attn_fwd": (_INT, 3 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P]),
+    "mce_attn_fwd": (_INT, 3 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P, _P]),
     "mce_attn_bwd_ws_bytes": (_S, 7 * [_I]),
-    "mce_attn_bwd": (_INT, 4 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "mce_attn_bwd": (_INT, 4 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
 }
 
 _lib = None

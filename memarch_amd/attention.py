@@ -102,15 +102,16 @@ def _check_heads(q, k, v, what):
         raise ValueError(f"{what} must all be bfloat16 or all float16, got {q.dtype}, {k.dtype} and {v.dtype}")
 
 
-def _forward(q, k, v, lengths, window, sinks, scale, need_lse):
+def _forward(q, k, v, lengths, window, sinks, scale, train):
     B, T, Hq, D = q.shape
     (q, qs), (k, ks), (v, vs) = _strided(q), _strided(k), _strided(v)
     out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device) if need_lse else None
+    res = torch.empty_like(out) if train else None
+    lse = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device) if train else None
     with _On(q.device):
         _lib.call("mce_attn_fwd", *qs, *ks, *vs, _ptr(lengths), B, T, Hq, k.shape[2], D, window, sinks, scale,
-                  _DTYPES[q.dtype], out.data_ptr(), _ptr(lse), _stream(q.device))
-    return q, k, v, out, lse
+                  _DTYPES[q.dtype], out.data_ptr(), _ptr(res), _ptr(lse), _stream(q.device))
+    return q, k, v, out, res, lse
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -118,15 +119,15 @@ class _WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, window, sinks, scale):
-        q, k, v, out, lse = _forward(q, k, v, lengths, window, sinks, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        q, k, v, out, res, lse = _forward(q, k, v, lengths, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, out, res, lse, lengths)
         ctx.mask = (window, sinks, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
+        q, k, v, out, res, lse, lengths = ctx.saved_tensors
         window, sinks, scale = ctx.mask
         B, T, Hq, D = q.shape
         Hkv = k.shape[2]
@@ -138,7 +139,7 @@ class _WindowAttention(torch.autograd.Function):
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         with _On(q.device):
             _lib.call("mce_attn_bwd", *qs, *ks, *vs, *gs, _ptr(lengths), B, T, Hq, Hkv, D, window, sinks, scale,
-                      _DTYPES[q.dtype], out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                      _DTYPES[q.dtype], out.data_ptr(), res.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                       ws.data_ptr(), n, _stream(q.device))
         return dq, dk, dv, None, None, None, None
 

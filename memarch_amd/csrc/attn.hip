@@ -24,8 +24,8 @@ struct Strided {
 
 struct Args {
   Strided q, k, v, go;
-  const uint16_t* out;       // contiguous [B, T, Hq, D]
-  uint16_t *o, *dq, *dk, *dv;
+  const uint16_t *out, *res; // contiguous [B, T, Hq, D], backward
+  uint16_t *o, *r, *dq, *dk, *dv;
   float* lse;                // [B, Hq, T]
   float* delta;              // [B, Hq, T]
   const int32_t* lengths;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
   const int bh = blockIdx.x / nq, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / a.grp;
   const int len = seq_len(a, b);
   const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
-  uint16_t* const op = a.o + ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
+  const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
   float* const lp = a.lse == nullptr ? nullptr : a.lse + (int64_t)bh * a.T + row;
   f32x16 acc[DP / 32] = {};
   float m = -INFINITY, l = 0.f;
@@ -158,7 +158,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
   l = sum_halves(l);
   const bool in = row < a.T, see = row < len;
   const float inv = see ? 1.f / l : 0.f;
-  store_acc<T, DP>(acc, inv, op, a.D, in, h);
+  store_acc<T, DP>(acc, inv, a.o + ofs, a.D, in, h);
+  if (a.r != nullptr) store_acc<T, DP, true>(acc, inv, a.r + ofs, a.D, in, h);
   if (lp != nullptr && in && h == 0) *lp = see ? m + __builtin_amdgcn_logf(l) / c : INFINITY;
 }
 
@@ -196,18 +197,19 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
     u32x4 qf[DP / 16], gf[DP / 16];
     const i32x4 qr = tile_rsrc<32>(a.q.p + b * a.q.sb + hq * a.q.sh, a.q.st, r0, len, a.D);
     const i32x4 gr = tile_rsrc<32>(a.go.p + b * a.go.sb + hq * a.go.sh, a.go.st, r0, len, a.D);
-    const i32x4 orr = tile_rsrc<32>(a.out + (int64_t)b * a.T * a.Hq * a.D + (int64_t)hq * a.D, (int64_t)a.Hq * a.D, r0,
-                                    len, a.D);
+    const int64_t head = (int64_t)b * a.T * a.Hq * a.D + (int64_t)hq * a.D, ldo = (int64_t)a.Hq * a.D;
+    const i32x4 orr = tile_rsrc<32>(a.out + head, ldo, r0, len, a.D), rr = tile_rsrc<32>(a.res + head, ldo, r0, len, a.D);
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
       const int col = 16 * ks + 8 * h, r = lane & 31;
       qf[ks] = load16(qr, col < a.D ? r * (int)a.q.st * 2 + col * 2 : OOB);
       gf[ks] = load16(gr, col < a.D ? r * (int)a.go.st * 2 + col * 2 : OOB);
-      const u32x4 of = load16(orr, col < a.D ? r * a.Hq * a.D * 2 + col * 2 : OOB);
+      const int oo = col < a.D ? r * (int)ldo * 2 + col * 2 : OOB;
+      const u32x4 of = load16(orr, oo), rf = load16(rr, oo);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        delta = __builtin_fmaf(lo_f32<T>(gf[ks][e]), lo_f32<T>(of[e]), delta);
-        delta = __builtin_fmaf(hi_f32<T>(gf[ks][e]), hi_f32<T>(of[e]), delta);
+        delta = __builtin_fmaf(lo_f32<T>(gf[ks][e]), lo_f32<T>(of[e]) + lo_f32<T>(rf[e]), delta);
+        delta = __builtin_fmaf(hi_f32<T>(gf[ks][e]), hi_f32<T>(of[e]) + hi_f32<T>(rf[e]), delta);
       }
     }
     delta = sum_halves(delta);
@@ -448,7 +450,7 @@ int mce_attn_last_hip_error(void) { return g_hip_error; }
 int mce_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
                  int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const int32_t* lengths,
                  int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks, float scale,
-                 int dtype, void* out, float* lse, void* stream) {
+                 int dtype, void* out, void* res, float* lse, void* stream) {
   int rc = check_sizes(B, T, Hq, Hkv, D, window, sinks);
   if (rc) return rc;
   if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16)) return MCE_ATTN_EINVAL;
@@ -457,12 +459,13 @@ int mce_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
       (rc = check_strided(v, v_sb, v_st, v_sh, D)))
     return rc;
   if (out == nullptr) return MCE_ATTN_EINVAL;
-  if (reinterpret_cast<uintptr_t>(out) & 15) return MCE_ATTN_EALIGN;
+  if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(res)) & 15) return MCE_ATTN_EALIGN;
   Args a = make_args({static_cast<const uint16_t*>(q), q_sb, q_st, q_sh},
                      {static_cast<const uint16_t*>(k), k_sb, k_st, k_sh},
                      {static_cast<const uint16_t*>(v), v_sb, v_st, v_sh}, lengths, B, T, Hq, Hkv, D, window, sinks,
                      scale);
   a.o = static_cast<uint16_t*>(out);
+  a.r = static_cast<uint16_t*>(res);
   a.lse = lse;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dtype == MCE_ATTN_BF16) return D <= 64 ? launch_fwd<__bf16, 64>(a, st) : launch_fwd<__bf16, 128>(a, st);
@@ -478,8 +481,8 @@ size_t mce_attn_bwd_ws_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int6
 int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
                  int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const void* go, int64_t go_sb,
                  int64_t go_st, int64_t go_sh, const int32_t* lengths, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
-                 int64_t D, int64_t window, int64_t sinks, float scale, int dtype, const void* out, const float* lse,
-                 void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream) {
+                 int64_t D, int64_t window, int64_t sinks, float scale, int dtype, const void* out, const void* res,
+                 const float* lse, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream) {
   int rc = check_sizes(B, T, Hq, Hkv, D, window, sinks);
   if (rc) return rc;
   if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16)) return MCE_ATTN_EINVAL;
@@ -487,8 +490,8 @@ int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
   if ((rc = check_strided(q, q_sb, q_st, q_sh, D)) || (rc = check_strided(k, k_sb, k_st, k_sh, D)) ||
       (rc = check_strided(v, v_sb, v_st, v_sh, D)) || (rc = check_strided(go, go_sb, go_st, go_sh, D)))
     return rc;
-  if (out == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr) return MCE_ATTN_EINVAL;
-  for (const void* p : {out, (const void*)dq, (const void*)dk, (const void*)dv})
+  if (out == nullptr || res == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr) return MCE_ATTN_EINVAL;
+  for (const void* p : {out, res, (const void*)dq, (const void*)dk, (const void*)dv})
     if (reinterpret_cast<uintptr_t>(p) & 15) return MCE_ATTN_EALIGN;
   if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) ||
       ws_bytes < mce_attn_bwd_ws_bytes(B, T, Hq, Hkv, D, window, sinks))
@@ -499,6 +502,7 @@ int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
                      scale);
   a.go = {static_cast<const uint16_t*>(go), go_sb, go_st, go_sh};
   a.out = static_cast<const uint16_t*>(out);
+  a.res = static_cast<const uint16_t*>(res);
   a.lse = const_cast<float*>(lse);
   a.delta = static_cast<float*>(ws);
   a.dq = static_cast<uint16_t*>(dq);

@@ -209,8 +209,9 @@ __device__ __forceinline__ float sum_halves(float x) {
 
 // Stores the accumulators acc[dt] (rows = columns 32 dt + ... of the result, accumulator column = its row l%32) scaled
 // by f: row `row` of p, DP/32 x 16 bytes x 2 per lane. The halves exchange 4 columns of every 16, so that each lane
-// stores 16 bytes. Only rows with ok and columns below d are written.
-template <typename T, int DP>
+// stores 16 bytes. Only rows with ok and columns below d are written. RES: the values stored are what the rounding of
+// the same call without RES leaves over, rounded in their turn.
+template <typename T, int DP, bool RES = false>
 __device__ __forceinline__ void store_acc(const f32x16 (&acc)[DP / 32], float f, uint16_t* p, int d, bool ok, int h) {
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
@@ -219,7 +220,10 @@ __device__ __forceinline__ void store_acc(const f32x16 (&acc)[DP / 32], float f,
       // lane half h holds columns 16 s + 4 h + {0..3} (lo) and 16 s + 8 + 4 h + {0..3} (hi)
       uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = pack2<T>(acc[dt][8 * s + 2 * e] * f, acc[dt][8 * s + 2 * e + 1] * f);
+      for (int e = 0; e < 4; ++e) {
+        const float x = acc[dt][8 * s + 2 * e] * f, y = acc[dt][8 * s + 2 * e + 1] * f;
+        w[e] = RES ? pack2<T>(x - (float)(T)x, y - (float)(T)y) : pack2<T>(x, y);
+      }
       // swap(w[2], w[0])'s halves: low lanes end with columns 16 s + 0..7, high lanes with 16 s + 8..15
       const auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
       const auto r1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
