@@ -1,4 +1,4 @@
-"""ctypes binding of libmce.so (declarations in include/mce.h) and libmce_attn.so (include/mce_attn.h).
+"""ctypes binding of libmce.so (declarations in include/mce.h) and libmce_attn.so (include/mce_attn.h, mce_rope.h).
 
 torch is imported before the library is loaded: torch ships its own libamdhip64.so with the same SONAME as
 /opt/rocm's, so loading torch first makes libmce.so bind to the one HIP runtime that owns torch's streams
@@ -69,7 +69,7 @@ SIGNATURES = {
     "mce_swiglu_last_hip_error": (_INT, []),
 }
 
-# the attention library, in the order of include/mce_attn.h
+# the attention library, in the order of include/mce_attn.h, include/mce_rope.h
 _TENSOR = [_P, _I, _I, _I]   # pointer and element strides (batch, token, head)
 ATTN_SIGNATURES = {
     "mce_attn_error_string": (ctypes.c_char_p, [_INT]),
@@ -77,6 +77,12 @@ ATTN_SIGNATURES = {
     "mce_attn_fwd": (_INT, 3 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P, _P]),
     "mce_attn_bwd_ws_bytes": (_S, 7 * [_I]),
     "mce_attn_bwd": (_INT, 4 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    # include/mce_rope.h
+    "mce_rope_fwd": (_INT, 2 * _TENSOR + [_P, _P, _I, _P, _INT, _I, _I, _P, _P] + 6 * [_I] +
+                     [_INT, _F, _INT, _INT, _P, _P, _P]),
+    "mce_rope_bwd_ws_bytes": (_S, 5 * [_I] + [_INT]),
+    "mce_rope_bwd": (_INT, 4 * _TENSOR + [_P, _P, _I, _P, _INT, _I, _I, _P, _P] + 6 * [_I] +
+                     [_INT, _F, _INT, _INT, _P, _P, _P, _P, _P, _S, _P]),
 }
 
 _lib = None
