@@ -40,7 +40,7 @@ extern "C" {
 #define MCE_ROPE_OK 0
 #define MCE_ROPE_EINVAL 1     /* size, stride, element type or null pointer */
 #define MCE_ROPE_EWORKSPACE 3 /* workspace missing, too small or not 256-byte aligned */
-#define MCE_ROPE_ELAUNCH 4    /* a HIP launch failed */
+#define MCE_ROPE_ELAUNCH 4    /* a HIP launch failed (mce_attn_last_hip_error; the codes' texts: mce_attn_error_string) */
 
 /* element types of q, k, their gradients and the outputs */
 #define MCE_ROPE_F32 0

@@ -1,4 +1,5 @@
-"""ctypes binding of libmce.so (declarations in include/mce.h) and libmce_attn.so (include/mce_attn.h, mce_rope.h).
+"""ctypes binding of libmce.so (declarations in include/mce.h) and libmce_attn.so (include/mce_attn.h, mce_paged.h,
+mce_rope.h).
 
 torch is imported before the library is loaded: torch ships its own libamdhip64.so with the same SONAME as
 /opt/rocm's, so loading torch first makes libmce.so bind to the one HIP runtime that owns torch's streams
@@ -69,7 +70,7 @@ SIGNATURES = {
     "mce_swiglu_last_hip_error": (_INT, []),
 }
 
-# the attention library, in the order of include/mce_attn.h, include/mce_rope.h
+# the attention library, in the order of include/mce_attn.h, include/mce_paged.h, include/mce_rope.h
 _TENSOR = [_P, _I, _I, _I]   # pointer and element strides (batch, token, head)
 ATTN_SIGNATURES = {
     "mce_attn_error_string": (ctypes.c_char_p, [_INT]),
@@ -77,6 +78,9 @@ ATTN_SIGNATURES = {
     "mce_attn_fwd": (_INT, 3 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P, _P]),
     "mce_attn_bwd_ws_bytes": (_S, 7 * [_I]),
     "mce_attn_bwd": (_INT, 4 * _TENSOR + [_P] + 7 * [_I] + [_F, _INT, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    # include/mce_paged.h
+    "mce_paged_ws_bytes": (_S, 8 * [_I]),
+    "mce_paged": (_INT, [_P, _I, _I] + 2 * _TENSOR + [_P, _I, _P] + 9 * [_I] + [_F, _INT, _P, _P, _S, _P]),
     # include/mce_rope.h
     "mce_rope_fwd": (_INT, 2 * _TENSOR + [_P, _P, _I, _P, _INT, _I, _I, _P, _P] + 6 * [_I] +
                      [_INT, _F, _INT, _INT, _P, _P, _P]),

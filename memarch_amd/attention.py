@@ -1,9 +1,11 @@
-"""Causal attention over a sliding window with first tokens that stay visible, on MI355X (libmce_attn.so).
+"""Causal attention over a sliding window with first tokens that stay visible, and its form for one new token per
+sequence over a paged cache, on MI355X (libmce_attn.so).
 
 `window_attention(q, k, v, window, sinks, lengths)` stands where memarch's blocks call scaled_dot_product_attention or
 their block-window helpers (lm.py:448-554, full2.py:154-181): one kernel forward, two backward, no scores in memory.
 Position i of a sequence sees position j <= i when i - j < window or j < sinks. Products take bf16 or fp16 operands and
-sum in fp32; softmax statistics are fp32 (include/mce_attn.h). All device work runs on torch's current stream; a tensor
+sum in fp32; softmax statistics are fp32 (include/mce_attn.h, include/mce_paged.h). `paged_attention` is the last row of
+the same attention for each sequence, its keys and values lying in the pages of a cache. All device work runs on torch's current stream; a tensor
 that is not on a GPU raises, and there is no other code path.
 """
 import math
@@ -166,3 +168,61 @@ def window_attention(q, k, v, window=None, sinks=0, lengths=None, scale=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
     return _forward(q, k, v, lengths, window, sinks, scale, False)[3]
+
+
+def _cache(t, name):
+    """Element strides (page, slot, head) of a cache, which is never copied: the library reads it where it lies."""
+    _, page, h, d = t.shape
+    sp, st, sh, sd = t.stride()
+    sh = sh if h > 1 else 0
+    if sd != 1 or (sp | st | sh) & 7 or not d <= st <= _MAX_STRIDE or t.data_ptr() & 15:
+        raise ValueError(f"{name} must have a contiguous last dimension, a 16-byte aligned base, strides that are "
+                         f"multiples of 8 and slots at least {d} elements apart, got strides {t.stride()}")
+    return t.data_ptr(), sp, st, sh
+
+
+@torch.compiler.disable
+@torch.no_grad()
+def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sinks=0, scale=None):
+    """Attention of one new token per sequence, q [B, Hq, D], over the pages of a cache, k_cache and v_cache [pages,
+    page, Hkv, D] (bf16 or fp16; page and D multiples of 8, D up to 128) -> [B, Hq, D]. Token j of sequence b lies in
+    page block_table[b, j // page] (int32 [B, max_pages]) at slot j % page; lengths [B] (int32 or int64) counts a
+    sequence's cached tokens with the new one, whose keys and values are in the cache already. The mask is that of
+    window_attention's last row. A sequence of length 0 gives 0; tokens in pages outside the cache (entries of -1, say)
+    and past max_pages are not seen. The caches are read where they lie, 16 bytes at a time. No gradient."""
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError(f"q {tuple(q.shape)} must be [B, Hq, D], k_cache {tuple(k_cache.shape)} and v_cache "
+                         f"{tuple(v_cache.shape)} [pages, page, Hkv, D]")
+    _check_heads(q, k_cache, v_cache, "q and the caches")
+    B, Hq, D = q.shape
+    pages, page, Hkv, _ = k_cache.shape
+    if page < 8 or page % 8 or page > 65536:
+        raise ValueError(f"pages of {page} tokens are not supported (a multiple of 8 up to 65536 is)")
+    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.dtype is not torch.int32:
+        raise ValueError(f"block_table must be int32 [B={B}, max_pages], got {tuple(block_table.shape)} "
+                         f"{block_table.dtype}")
+    window, sinks = _mask_args(window, sinks)
+    scale = _scale(scale, D)
+    if lengths is None:
+        raise ValueError("lengths must be given")
+    lengths = _lengths(lengths, B, 2**31 - 1)
+    _check_same(q, ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("lengths", lengths))
+    max_pages = block_table.shape[1]
+    if max_pages > 1 and block_table.stride(1) != 1 or B > 1 and block_table.stride(0) < max_pages:
+        block_table = block_table.contiguous()
+    sb, sh, sd = q.stride()
+    sb, sh = sb if B > 1 else 0, sh if Hq > 1 else D
+    if sd != 1 or (sb | sh) & 7 or not D <= sh <= _MAX_STRIDE or q.data_ptr() & 15:
+        q = q.contiguous()
+        if q.data_ptr() & 15:
+            q = q.clone()
+        sb, sh = Hq * D, D
+    kc, vc = _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache")
+    out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+    n = _lib.load_attn().mce_paged_ws_bytes(B, Hq, Hkv, D, page, max_pages, window, sinks)
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    with _On(q.device):
+        _lib.call("mce_paged", q.data_ptr(), sb, sh, *kc, *vc, block_table.data_ptr(),
+                  block_table.stride(0) if B > 1 else 0, lengths.data_ptr(), B, Hq, Hkv, D, pages, page, max_pages,
+                  window, sinks, scale, _DTYPES[q.dtype], out.data_ptr(), _ptr(ws), n, _stream(q.device))
+    return out

@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRCS = [os.path.join(HERE, "csrc", f) for f in ("mce.hip", "induct.hip", "swiglu.hip")]
 LIB = os.path.join(HERE, "libmce.so")
-ATTN_SRCS = [os.path.join(HERE, "csrc", f) for f in ("attn.hip", "rope.hip")]
+ATTN_SRCS = [os.path.join(HERE, "csrc", f) for f in ("attn.hip", "paged.hip", "rope.hip")]
 ATTN_LIB = os.path.join(HERE, "libmce_attn.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "../../include/mce_attn.h"
+#include "attn_host.h"
 #include "attn_tile.h"
 
 namespace {
@@ -361,26 +362,6 @@ __global__ __launch_bounds__(THREADS, 1) void k_attn_dkv(Args a) {
 }
 
 // -------------------------------------------------------------------------------------------------------- host side
-thread_local int g_hip_error = 0;   // the calling thread's last failed launch
-
-int finish() {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) {
-    g_hip_error = (int)e;
-    return MCE_ATTN_ELAUNCH;
-  }
-  return MCE_ATTN_OK;
-}
-
-// Token strides up to 2^21 elements keep every offset inside a tile of at most 128 rows in 31 bits.
-constexpr int64_t MAX_ST = int64_t(1) << 21;
-
-int check_strided(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t D) {
-  if (p == nullptr || sb < 0 || sh < 0 || st < D || st > MAX_ST) return MCE_ATTN_EINVAL;
-  if ((reinterpret_cast<uintptr_t>(p) & 15) || (sb | st | sh) % 8) return MCE_ATTN_EALIGN;
-  return MCE_ATTN_OK;
-}
-
 int check_sizes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
   if (B < 0 || T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || D > 128 || D % 8 || window < 0 || sinks < 0)
     return MCE_ATTN_EINVAL;
@@ -426,11 +407,9 @@ int launch_bwd(const Args& a, hipStream_t st) {
   return finish();
 }
 
-bool good_scale(float s) { return s > 0.f && s <= 3.0e38f; }
-
-int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
-
 }  // namespace
+
+thread_local int mce_attn_hip_error = 0;
 
 extern "C" {
 
@@ -445,7 +424,7 @@ const char* mce_attn_error_string(int code) {
   }
 }
 
-int mce_attn_last_hip_error(void) { return g_hip_error; }
+int mce_attn_last_hip_error(void) { return mce_attn_hip_error; }
 
 int mce_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
                  int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const int32_t* lengths,

@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "../../include/mce_rope.h"
+#include "attn_host.h"
 
 namespace {
 
@@ -410,7 +411,7 @@ bool whole_pieces(const void* p, int64_t sb, int64_t st, int64_t sh) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (sb | st | sh) % 8 == 0;
 }
 
-int finish() { return hipGetLastError() == hipSuccess ? MCE_ROPE_OK : MCE_ROPE_ELAUNCH; }
+using attn::finish;
 
 template <typename T, bool NORM, bool IL, bool BWD>
 void launch(Args& a, bool pieces, int64_t nq, int64_t nk, hipStream_t st) {
