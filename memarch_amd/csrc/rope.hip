@@ -554,7 +554,7 @@ int mce_rope_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
     const int e = run<true>(a, norm, interleaved, dtype, pieces, nq, nk, st);
     if (e) return e;
   }
-  if (norm) {
+  if (weights) {
     hipLaunchKernelGGL(k_rope_dw, dim3((unsigned)(2 * D)), dim3(64), 0, st, part, (int)nq, part + nq * D, (int)nk, dqw,
                        dkw, (int)D);
     return finish();
