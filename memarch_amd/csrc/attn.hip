@@ -18,6 +18,8 @@ constexpr int BK = 64;              // keys per tile there
 constexpr int BKV = 32 * NW;        // keys per workgroup of k_attn_dkv (32 per wave)
 constexpr int BR = 32;              // query rows per tile there
 
+constexpr float LAZY = 8.f;         // k_attn_fwd: growth of a maximum (log2) up to which its old value is kept
+
 struct Strided {
   const uint16_t* p;
   int64_t sb, st, sh;  // elements between batches, tokens, heads
@@ -56,14 +58,24 @@ struct KeyTiles {
 };
 
 // Masks a 32 x 32 block of scores held as [keys][rows]: accumulator element e of lane l is key
-// k0 + 8*(e/4) + 4*(l/32) + e%4 and row `row` (of lane l%32).
-__device__ __forceinline__ void mask_keys(f32x16& s, int row, int k0h, int window, int sinks, float fill) {
+// k0h + 8*(e/4) + e%4 (k0h = first key + 4*(l/32)) and row `row` (of lane l%32). Both forms are free of branches; the
+// one without first tokens in the block is a compare and a select per element.
+__device__ __forceinline__ void mask_keys(f32x16& s, int row, int k0h, int window, int sinks, bool with_sinks) {
   const int rel = row - k0h;
+  if (with_sinks) {
+    const int left = sinks - k0h;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int c = 8 * (e / 4) + e % 4;
-    const bool see = (uint32_t)(rel - c) < (uint32_t)window || (k0h + c < sinks && rel - c >= 0);
-    s[e] = see ? s[e] : fill;
+    for (int e = 0; e < 16; ++e) {
+      const int c = 8 * (e / 4) + e % 4;
+      const bool see = ((uint32_t)(rel - c) < (uint32_t)window) | ((c < left) & (rel >= c));
+      s[e] = see ? s[e] : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int c = 8 * (e / 4) + e % 4;
+      s[e] = (uint32_t)(rel - c) < (uint32_t)window ? s[e] : -INFINITY;
+    }
   }
 }
 
@@ -117,13 +129,14 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
       if (!none) {
         f32x16 s[2] = {};
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) s[kb] = mfma<T>(frag_rows<DP>(lds, ad, img, kb, ks), qf[ks], s[kb]);
+          for (int kb = 0; kb < 2; ++kb) s[kb] = mfma<T>(frag_rows<DP>(lds, ad, img, kb, ks), qf[ks], s[kb]);
         const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
         if (!all) {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) mask_keys(s[kb], row, k0 + 32 * kb + 4 * h, a.window, a.sinks, -INFINITY);
+          for (int kb = 0; kb < 2; ++kb)
+            mask_keys(s[kb], row, k0 + 32 * kb + 4 * h, a.window, a.sinks, k0 < a.sinks);
         }
         float mx = m;
 #pragma unroll
@@ -131,13 +144,16 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
         mx = max_halves(mx);
-        const float mu = mx == -INFINITY ? 0.f : mx;   // a row that has seen nothing yet
-        const float al = __builtin_amdgcn_exp2f((m - mu) * c);
-        m = mx;
-        l *= al;
+        // The sums are rescaled only when some row's maximum has grown by more than LAZY since the last time: until
+        // then its exponentials stay below 2^LAZY.
+        if (__builtin_amdgcn_ballot_w64((mx - m) * c > LAZY) != 0) {
+          const float al = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mx) * c);
+          m = mx;
+          l *= al;
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= al;
-        const float mc = mu * c;
+          for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= al;
+        }
+        const float mc = (m == -INFINITY ? 0.f : m) * c;   // a row that has seen nothing yet
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -234,7 +250,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
           for (int ks = 0; ks < DP / 16; ++ks) s = mfma<T>(frag_rows<DP>(lds, ad, img, kb, ks), qf[ks], s);
 #pragma unroll
           for (int ks = 0; ks < DP / 16; ++ks) ds = mfma<T>(frag_rows<DP>(lds, ad, img + IMG, kb, ks), gf[ks], ds);
-          if (!all) mask_keys(s, row, k0 + 32 * kb + 4 * h, a.window, a.sinks, -INFINITY);
+          if (!all) mask_keys(s, row, k0 + 32 * kb + 4 * h, a.window, a.sinks, k0 < a.sinks);
 #pragma unroll
           for (int e = 0; e < 16; ++e) ds[e] *= __builtin_amdgcn_exp2f(s[e] * c);
 #pragma unroll
@@ -333,7 +349,8 @@ __global__ __launch_bounds__(THREADS, 1) void k_attn_dkv(Args a) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int d = rel + 8 * (e / 4) + e % 4;
-            s[e] = (uint32_t)d < (uint32_t)a.window || (key < a.sinks && d >= 0) ? s[e] : -INFINITY;
+            const bool see = ((uint32_t)d < (uint32_t)a.window) | ((key < a.sinks) & (d >= 0));
+            s[e] = see ? s[e] : -INFINITY;
           }
         }
 #pragma unroll
