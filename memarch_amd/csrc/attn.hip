@@ -35,6 +35,9 @@ struct Args {
   int B, T, Hq, Hkv, grp, D;
   int window, sinks;         // window = INT32_MAX: none
   float scale;
+  // k_attn_dkv: the first n_sb key blocks (those with first tokens) are shared by S_s workgroups each, the others by S_r
+  int n_sb, S_s, S_r;
+  float *part_s, *part_r;    // their fp32 parts [B Hkv, block, S, 2, BKV, D] where S > 1
 };
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
@@ -237,6 +240,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       const int img = (it & 1) * 2 * IMG;
       if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
       const int k0 = kt.key0(it);
+      ad.refresh();
       if (k0 <= r0 + 31) {
         const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
 #pragma unroll
@@ -273,23 +277,31 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
 
 // ---------------------------------------------------------------------------------------------------------- dk, dv
 template <typename T, int DP>
-__global__ __launch_bounds__(THREADS, 1) void k_attn_dkv(Args a) {
+__global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   constexpr int IMG = BR * DP * 2;
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];   // Q and go, two tiles each
   __shared__ float stats[2][2][BR];                              // -lse and -delta of the tile's rows
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int nk = (a.T + BKV - 1) / BKV;
-  const int kblk = blockIdx.x % nk;                    // the keys with the most rows first
-  const int bh = blockIdx.x / nk, b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int nk = (a.T + BKV - 1) / BKV, nr = nk - a.n_sb;
+  // workgroups of the blocks with first tokens (the longest) first, then the others, those with the most rows first
+  const uint32_t heads = (uint32_t)a.B * a.Hkv, sink_wgs = heads * a.n_sb * a.S_s;
+  const bool sink = blockIdx.x < sink_wgs;
+  const uint32_t w = sink ? blockIdx.x : blockIdx.x - sink_wgs;
+  const int S = sink ? a.S_s : a.S_r, nb = sink ? a.n_sb : nr;
+  const int sp = w % S, blk = w / S % nb, bh = w / S / nb, b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int kblk = sink ? blk : a.n_sb + blk;
   const int len = seq_len(a, b);
   const int kb0 = kblk * BKV, j0 = kb0 + wave * 32, key = j0 + (lane & 31);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   const float c = a.scale * LOG2E;
+  int it0 = 0, it1 = 0;
   if (kb0 < len) {
     // rows kb0 .. q_end - 1 may see a key of the block
     int64_t q_end64 = kb0 < a.sinks ? len : (int64_t)kb0 + BKV - 1 + a.window;
     const int q_end = q_end64 < len ? (int)q_end64 : len;
     const int t0 = kb0 / BR, nt = (q_end + BR - 1) / BR - t0, total = nt * a.grp;
+    it0 = (int)((int64_t)total * sp / S);
+    it1 = (int)((int64_t)total * (sp + 1) / S);
     FragAddr<DP> ad;
     ad.init(lane);
     TileLoad<DP, BR, NW> tq, tg;
@@ -309,7 +321,7 @@ __global__ __launch_bounds__(THREADS, 1) void k_attn_dkv(Args a) {
     auto put = [&](int buf) {
       if (threadIdx.x < 2 * BR) stats[buf][threadIdx.x / BR][threadIdx.x & (BR - 1)] = st0;
     };
-    issue(0, 0);
+    if (it0 < it1) issue(it0, 0);
     u32x4 kf[DP / 16], vf[DP / 16];
     const i32x4 kr = tile_rsrc<32>(a.k.p + b * a.k.sb + hk * a.k.sh, a.k.st, j0, len, a.D);
     const i32x4 vr = tile_rsrc<32>(a.v.p + b * a.v.sb + hk * a.v.sh, a.v.st, j0, len, a.D);
@@ -322,10 +334,11 @@ __global__ __launch_bounds__(THREADS, 1) void k_attn_dkv(Args a) {
     put(0);
     wait_vmcnt<0>();
     __syncthreads();
-    for (int it = 0; it < total; ++it) {
-      const int buf = it & 1, img = buf * 2 * IMG;
-      if (it + 1 < total) issue(it + 1, buf ^ 1);
+    for (int it = it0; it < it1; ++it) {
+      const int buf = (it - it0) & 1, img = buf * 2 * IMG;
+      if (it + 1 < it1) issue(it + 1, buf ^ 1);
       const int i0 = (t0 + it % nt) * BR;
+      ad.refresh();
       const bool some = i0 + BR - 1 >= j0 && (i0 - (j0 + 31) < a.window || j0 < a.sinks);
       if (some) {
         f32x16 s, ds;
@@ -372,10 +385,43 @@ __global__ __launch_bounds__(THREADS, 1) void k_attn_dkv(Args a) {
       __syncthreads();
     }
   }
-  const int64_t ofs = (((int64_t)b * a.T + key) * a.Hkv + hk) * a.D;
   const bool in = key < a.T;
-  store_acc<T, DP>(dk, a.scale, a.dk + ofs, a.D, in, h);
-  store_acc<T, DP>(dv, 1.f, a.dv + ofs, a.D, in, h);
+  if (S == 1) {
+    const int64_t ofs = (((int64_t)b * a.T + key) * a.Hkv + hk) * a.D;
+    store_acc<T, DP>(dk, a.scale, a.dk + ofs, a.D, in, h);
+    store_acc<T, DP>(dv, 1.f, a.dv + ofs, a.D, in, h);
+  } else {
+    float* const p = (sink ? a.part_s : a.part_r) + ((((int64_t)bh * nb + blk) * S + sp) * 2 * BKV + key - kb0) * a.D;
+    store_f32<DP>(dk, p, a.D, in, h);
+    store_f32<DP>(dv, p + BKV * a.D, a.D, in, h);
+  }
+}
+
+// dk and dv of the blocks whose rows are shared by several workgroups: the sum of their parts in order, 4 columns of a
+// key per thread, `pieces` workgroups per block (few blocks with many parts each: the loads have to come from many
+// threads).
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dkv_join(Args a, int pieces) {
+  const int nk = (a.T + BKV - 1) / BKV, nr = nk - a.n_sb;
+  const uint32_t heads = (uint32_t)a.B * a.Hkv, sink_blocks = a.S_s > 1 ? heads * a.n_sb : 0;
+  const int i = blockIdx.x % pieces * 256 + threadIdx.x;
+  uint32_t w = blockIdx.x / pieces;
+  const bool sink = w < sink_blocks;
+  if (!sink) w -= sink_blocks;
+  const int S = sink ? a.S_s : a.S_r, nb = sink ? a.n_sb : nr;
+  const int blk = w % nb, bh = w / nb, b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int kb0 = (sink ? blk : a.n_sb + blk) * BKV, cols = a.D / 4;
+  const int which = i / (BKV * cols), r = i / cols % BKV, d = i % cols * 4, key = kb0 + r;
+  if (which > 1 || key >= a.T) return;
+  const float* const p = (sink ? a.part_s : a.part_r) + ((((int64_t)bh * nb + blk) * S * 2 + which) * BKV + r) * a.D + d;
+  f32x4 x = {};
+#pragma unroll 4
+  for (int sp = 0; sp < S; ++sp) x += *reinterpret_cast<const f32x4*>(p + (int64_t)sp * 2 * BKV * a.D);
+  if (which == 0) x *= a.scale;
+  u32x2 v;
+  v[0] = pack2<T>(x[0], x[1]);
+  v[1] = pack2<T>(x[2], x[3]);
+  *reinterpret_cast<u32x2*>((which ? a.dv : a.dk) + (((int64_t)b * a.T + key) * a.Hkv + hk) * a.D + d) = v;
 }
 
 // -------------------------------------------------------------------------------------------------------- host side
@@ -415,12 +461,63 @@ int launch_fwd(const Args& a, hipStream_t st) {
   return finish();
 }
 
+// How many workgroups share a key block's rows in k_attn_dkv. Lengths are not known to the host: T stands for all.
+struct Plan {
+  int n_sb, S_s, S_r;
+  int64_t part_s, part_r;   // floats of the parts
+};
+constexpr int64_t SLOTS = 512;    // workgroups of k_attn_dkv that run at once
+constexpr int64_t MIN_ITERS = 64; // row tiles below which a workgroup is not divided
+Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
+  Plan p = {0, 1, 1, 0, 0};
+  const int64_t grp = Hq / Hkv, nk = (T + BKV - 1) / BKV, nt = (T + BR - 1) / BR, heads = B * Hkv;
+  const bool causal = window == 0 || window >= T;
+  if (!causal && sinks > 0) {
+    p.n_sb = (int)((sinks + BKV - 1) / BKV);
+    if (p.n_sb > nk) p.n_sb = (int)nk;
+  }
+  const int64_t units = heads * (nk - p.n_sb);
+  // row tiles of the longest of the other blocks, and of all of them
+  int64_t longest = causal ? nt * grp : ((BKV - 1 + window + BR - 1) / BR + 1) * grp;
+  if (longest > nt * grp) longest = nt * grp;
+  const double work = (double)units * longest * (causal ? 0.5 : 1.0);
+  // S that ends first: rounds of equal workgroups, or (rows of different length, the longest first) the mean load and
+  // half of the last ones; a tenth of a round for the parts' traffic
+  double best = 1e300;
+  for (int S = 1; S <= 16 && (S == 1 || longest / S >= MIN_ITERS); ++S) {
+    const double each = (double)longest / S;
+    const double mean = work / SLOTS;
+    double cost = causal ? (mean > each ? mean : each) + 0.5 * each
+                         : (double)((units * S + SLOTS - 1) / SLOTS) * each;
+    if (S > 1) cost += 0.1 * mean + 8;
+    if (cost < best) {
+      best = cost;
+      p.S_r = S;
+    }
+  }
+  if (p.n_sb > 0) {
+    // a block with first tokens is seen by every later row: no workgroup longer than the others', or than a quarter of
+    // the whole
+    const double each = (double)longest / p.S_r, quarter = (work + (double)heads * p.n_sb * nt * grp) / SLOTS / 4;
+    const double most = each > quarter ? each : quarter;
+    const double s = (double)(nt * grp) / (most < MIN_ITERS ? MIN_ITERS : most);
+    p.S_s = s <= 1 ? 1 : (s > 256 ? 256 : (int)(s + 0.999));
+  }
+  p.part_s = p.S_s > 1 ? heads * p.n_sb * p.S_s * 2 * BKV * D : 0;
+  p.part_r = p.S_r > 1 ? heads * (nk - p.n_sb) * p.S_r * 2 * BKV * D : 0;
+  return p;
+}
+
 template <typename T, int DP>
 int launch_bwd(const Args& a, hipStream_t st) {
   const unsigned n = (unsigned)((int64_t)a.B * a.Hq * ((a.T + BQ - 1) / BQ));
   hipLaunchKernelGGL((k_attn_dq<T, DP>), dim3(n), dim3(THREADS), 0, st, a);
-  const unsigned nk = (unsigned)((int64_t)a.B * a.Hkv * ((a.T + BKV - 1) / BKV));
-  hipLaunchKernelGGL((k_attn_dkv<T, DP>), dim3(nk), dim3(THREADS), 0, st, a);
+  const int64_t heads = (int64_t)a.B * a.Hkv, nr = (a.T + BKV - 1) / BKV - a.n_sb;
+  hipLaunchKernelGGL((k_attn_dkv<T, DP>), dim3((unsigned)(heads * (a.n_sb * a.S_s + nr * a.S_r))), dim3(THREADS), 0, st,
+                     a);
+  const int64_t join = heads * ((a.S_s > 1 ? a.n_sb : 0) + (a.S_r > 1 ? nr : 0));
+  const int pieces = (2 * BKV * (a.D / 4) + 255) / 256;
+  if (join > 0) hipLaunchKernelGGL((k_attn_dkv_join<T>), dim3((unsigned)(join * pieces)), dim3(256), 0, st, a, pieces);
   return finish();
 }
 
@@ -471,7 +568,8 @@ int mce_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
 size_t mce_attn_bwd_ws_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                              int64_t sinks) {
   if (check_sizes(B, T, Hq, Hkv, D, window, sinks)) return 0;
-  return (size_t)align256(B * Hq * T * 4);
+  const Plan p = make_plan(B, T, Hq, Hkv, D, window, sinks);
+  return (size_t)(align256(B * Hq * T * 4) + align256(p.part_s * 4) + align256(p.part_r * 4));
 }
 
 int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
@@ -500,7 +598,13 @@ int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
   a.out = static_cast<const uint16_t*>(out);
   a.res = static_cast<const uint16_t*>(res);
   a.lse = const_cast<float*>(lse);
+  const Plan p = make_plan(B, T, Hq, Hkv, D, window, sinks);
+  a.n_sb = p.n_sb;
+  a.S_s = p.S_s;
+  a.S_r = p.S_r;
   a.delta = static_cast<float*>(ws);
+  a.part_s = a.delta + align256(B * Hq * T * 4) / 4;
+  a.part_r = a.part_s + align256(p.part_s * 4) / 4;
   a.dq = static_cast<uint16_t*>(dq);
   a.dk = static_cast<uint16_t*>(dk);
   a.dv = static_cast<uint16_t*>(dv);

@@ -141,40 +141,45 @@ __device__ __forceinline__ i32x4 tile_rsrc(const uint16_t* p, int64_t ld, int ro
   return make_rsrc(p + (int64_t)row0 * ld, left == 0 ? 0 : (int)((left - 1) * ld + d) * 2);
 }
 
-// Per-lane byte offsets of the fragments inside a tile.
+// Per-lane byte offsets of the fragments inside a tile. A column slice (16 columns, ks) or block (32 columns, dt) is some
+// bits of the chunk number, which the swizzle leaves where they are, so the offset of any is the first one's with those
+// bits flipped.
 template <int DP>
 struct FragAddr {
-  static constexpr int ROWB = DP * 2;
-  uint32_t row[DP / 16];     // rows fragment of column slice ks (16 columns), row block 0
-  uint32_t tr[DP / 32][2];   // tr fragment of column block dt (32 columns), halves 0 and 1, row slice 0
+  uint32_t row;     // rows fragment of column slice 0, row block 0
+  uint32_t tr[2];   // tr fragment of column block 0, row slice 0: rows 0..7 and 8..15
   __device__ __forceinline__ void init(int lane) {
     const int r = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) row[ks] = r * ROWB + (((2 * ks + h) ^ swz<DP>(r)) << 4);
+    row = r * DP * 2 + ((h ^ swz<DP>(r)) << 4);
     const int g = (lane >> 4) & 1, j = (lane >> 2) & 3, q = lane & 3;
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int rr = 8 * t + 4 * h + j;
-        tr[dt][t] = rr * ROWB + (((4 * dt + 2 * g + (q >> 1)) ^ swz<DP>(rr)) << 4) + 8 * (q & 1);
-      }
+    for (int t = 0; t < 2; ++t) {
+      const int rr = 8 * t + 4 * h + j;
+      tr[t] = rr * DP * 2 + (((2 * g + (q >> 1)) ^ swz<DP>(rr)) << 4) + 8 * (q & 1);
+    }
   }
+  // Forbids keeping the flipped offsets in registers past this point (a kernel short of registers calls it once per
+  // tile; the flips are then made again, one instruction each).
+  __device__ __forceinline__ void refresh() { asm volatile("" : "+v"(row), "+v"(tr[0]), "+v"(tr[1])); }
 };
 
 // rows fragment: rows rb*32 .. +31, columns 16 ks .. +15 (rb and img are compile-time or scalar: immediates)
 template <int DP>
 __device__ __forceinline__ u32x4 frag_rows(const char* lds, const FragAddr<DP>& ad, int img, int rb, int ks) {
-  return *reinterpret_cast<const u32x4*>(lds + ad.row[ks] + img + rb * 32 * DP * 2);
+  return *reinterpret_cast<const u32x4*>(lds + (ad.row ^ (ks << 5)) + img + rb * 32 * DP * 2);
 }
-// tr fragment: columns 32 dt .. +31, rows of slice kk (16 rows) in the accumulator's order
+// tr fragment: columns 32 dt .. +31, rows of slice kk (16 rows) in the accumulator's order. With DP = 128 the swizzle of
+// a row 8 further differs in the chunk's highest bit, as the column blocks dt and dt ^ 2 do: the second half needs no
+// offset of its own.
 template <int DP>
 __device__ __forceinline__ u32x4 frag_tr(const char* lds, const FragAddr<DP>& ad, int img, int dt, int kk) {
   const int off = img + kk * 16 * DP * 2;
+  const uint32_t first = ad.tr[0] ^ (dt << 6);
+  const uint32_t second = DP == 128 ? (ad.tr[0] ^ ((dt ^ 2) << 6)) + 8 * DP * 2 : ad.tr[1] ^ (dt << 6);
   const u32x2 a = __builtin_bit_cast(
-      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(const_cast<char*>(lds) + ad.tr[dt][0] + off)));
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(const_cast<char*>(lds) + first + off)));
   const u32x2 b = __builtin_bit_cast(
-      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(const_cast<char*>(lds) + ad.tr[dt][1] + off)));
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(const_cast<char*>(lds) + second + off)));
   u32x4 r;
   r[0] = a[0];
   r[1] = a[1];
@@ -234,6 +239,21 @@ __device__ __forceinline__ void store_acc(const f32x16 (&acc)[DP / 32], float f,
       v[2] = r0[1];
       v[3] = r1[1];
       if (ok && col < d) *reinterpret_cast<u32x4*>(p + col) = v;
+    }
+}
+
+// The same as fp32, unscaled: 16 bytes per lane and group of 4 columns.
+template <int DP>
+__device__ __forceinline__ void store_f32(const f32x16 (&acc)[DP / 32], float* p, int d, bool ok, int h) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const int col = 32 * dt + 8 * e4 + 4 * h;
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = acc[dt][4 * e4 + e];
+      if (ok && col < d) *reinterpret_cast<f32x4*>(p + col) = x;
     }
 }
 
