@@ -60,6 +60,38 @@ struct KeyTiles {
   __device__ __forceinline__ int key0(int it) const { return (it < n_sink ? it : lo + it - n_sink) * BK; }
 };
 
+// Which sequence, heads and block of rows (or keys) a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an
+// L2 of its own: where the key/value heads (or the query heads) of the batch are a multiple of 8, each XCD takes whole
+// ones. Blocks of one length (a window) run head by head, the query heads of a group side by side on the same keys;
+// without a window the longest blocks of all the XCD's heads run first, so that none is left over at the end.
+struct Place {
+  int b, hk, g, blk;   // sequence, key/value head, query head of its group, block (0: the longest without a window)
+  // n: blocks per head; sub: query heads of a group that are workgroups of their own (grp, or 1)
+  __device__ __forceinline__ Place(const Args& a, uint32_t bid, uint32_t n, uint32_t sub) {
+    const uint32_t kv = (uint32_t)a.B * a.Hkv;
+    const bool whole = kv % 8 == 0, heads = !whole && kv * sub % 8 == 0;
+    const uint32_t units = heads ? kv * sub : kv, in = heads ? 1 : sub;   // units per XCD set, workgroups inside a unit
+    const uint32_t x = whole || heads ? 8 : 1, xcd = bid % x, slot = bid / x, ux = units / x;
+    uint32_t u, i;
+    if (a.window == INT32_MAX) {
+      blk = slot / (ux * in);
+      const uint32_t r = slot - blk * (ux * in);
+      u = r / in;
+      i = r - u * in;
+    } else {
+      u = slot / (n * in);
+      const uint32_t r = slot - u * (n * in);
+      blk = r / in;
+      i = r - blk * in;
+    }
+    u = u * x + xcd;
+    const uint32_t k = heads ? u / sub : u;
+    g = heads ? u - k * sub : i;
+    b = k / a.Hkv;
+    hk = k - b * a.Hkv;
+  }
+};
+
 // Masks a 32 x 32 block of scores held as [keys][rows]: accumulator element e of lane l is key
 // k0h + 8*(e/4) + e%4 (k0h = first key + 4*(l/32)) and row `row` (of lane l%32). Both forms are free of branches; the
 // one without first tokens in the block is a compare and a select per element.
@@ -89,8 +121,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];   // K and V, two tiles each
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int nq = (a.T + BQ - 1) / BQ;
-  const int qb = nq - 1 - blockIdx.x % nq;             // the rows with the most keys first
-  const int bh = blockIdx.x / nq, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / a.grp;
+  const Place pl(a, blockIdx.x, nq, a.grp);
+  const int qb = nq - 1 - pl.blk, b = pl.b, hk = pl.hk, hq = hk * a.grp + pl.g, bh = b * a.Hq + hq;
   const int len = seq_len(a, b);
   const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
   const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
@@ -190,8 +222,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int nq = (a.T + BQ - 1) / BQ;
-  const int qb = nq - 1 - blockIdx.x % nq;
-  const int bh = blockIdx.x / nq, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / a.grp;
+  const Place pl(a, blockIdx.x, nq, a.grp);
+  const int qb = nq - 1 - pl.blk, b = pl.b, hk = pl.hk, hq = hk * a.grp + pl.g, bh = b * a.Hq + hq;
   const int len = seq_len(a, b);
   const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
   const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
@@ -288,7 +320,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   const bool sink = blockIdx.x < sink_wgs;
   const uint32_t w = sink ? blockIdx.x : blockIdx.x - sink_wgs;
   const int S = sink ? a.S_s : a.S_r, nb = sink ? a.n_sb : nr;
-  const int sp = w % S, blk = w / S % nb, bh = w / S / nb, b = bh / a.Hkv, hk = bh % a.Hkv;
+  const Place pl(a, w, nb * S, 1);
+  const int sp = pl.blk % S, blk = pl.blk / S, b = pl.b, hk = pl.hk, bh = b * a.Hkv + hk;
   const int kblk = sink ? blk : a.n_sb + blk;
   const int len = seq_len(a, b);
   const int kb0 = kblk * BKV, j0 = kb0 + wave * 32, key = j0 + (lane & 31);
