@@ -17,6 +17,7 @@ constexpr int BQ = 32 * NW;         // query rows per workgroup of k_attn_fwd an
 constexpr int BK = 64;              // keys per tile there
 constexpr int BKV = 32 * NW;        // keys per workgroup of k_attn_dkv (32 per wave)
 constexpr int BR = 32;              // query rows per tile there
+constexpr int NS = 4;               // tiles of k_attn_dkv's ring
 
 constexpr float LAZY = 8.f;         // k_attn_fwd: growth of a maximum (log2) up to which its old value is kept
 
@@ -30,7 +31,7 @@ struct Args {
   const uint16_t *out, *res; // contiguous [B, T, Hq, D], backward
   uint16_t *o, *r, *dq, *dk, *dv;
   float* lse;                // [B, Hq, T]
-  float* delta;              // [B, Hq, T]
+  float* stat;               // [B, Hq, 2, T]: -lse and -delta, what the backward's scores and products start from
   const int32_t* lengths;
   int B, T, Hq, Hkv, grp, D;
   int window, sinks;         // window = INT32_MAX: none
@@ -160,13 +161,25 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
       const int img = (it & 1) * 2 * IMG;
       if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
       const int k0 = kt.key0(it);
-      const bool none = k0 > r0 + 31;                  // every key of the tile lies behind the wave's rows
-      if (!none) {
+      // whether the wave's rows see a key of the tile
+      if (k0 <= r0 + 31 && (r0 - (k0 + BK - 1) < a.window || k0 < a.sinks)) {
         f32x16 s[2] = {};
+        // the key fragments are read three column slices (6 products) ahead
+        u32x4 kf[4][2];
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks)
+        for (int ks = 0; ks < 3; ++ks)
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) s[kb] = mfma<T>(frag_rows<DP>(lds, ad, img, kb, ks), qf[ks], s[kb]);
+          for (int kb = 0; kb < 2; ++kb) kf[ks][kb] = frag_rows<DP>(lds, ad, img, kb, ks);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            if (ks + 3 < DP / 16) kf[(ks + 3) & 3][kb] = frag_rows<DP>(lds, ad, img, kb, ks + 3);
+            s[kb] = mfma<T>(kf[ks & 3][kb], qf[ks], s[kb]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
         const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
         if (!all) {
 #pragma unroll
@@ -228,7 +241,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
   const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
   const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
   f32x16 acc[DP / 32] = {};
-  float delta = 0.f;
+  float delta = 0.f, nl = -INFINITY;
   const float c = a.scale * LOG2E;
   if (q0 < len) {
     const int q1 = (q0 + BQ < len ? q0 + BQ : len) - 1;
@@ -265,7 +278,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       }
     }
     delta = sum_halves(delta);
-    const float nl = row < len ? -a.lse[(int64_t)bh * a.T + row] : -INFINITY;
+    if (row < len) nl = -a.lse[(int64_t)bh * a.T + row];
     wait_vmcnt<0>();
     __syncthreads();
     for (int it = 0; it < kt.n; ++it) {
@@ -273,7 +286,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
       const int k0 = kt.key0(it);
       ad.refresh();
-      if (k0 <= r0 + 31) {
+      if (k0 <= r0 + 31 && (r0 - (k0 + BK - 1) < a.window || k0 < a.sinks)) {
         const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -304,15 +317,19 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
   }
   const bool in = row < a.T;
   store_acc<T, DP>(acc, a.scale, a.dq + ofs, a.D, in, h);
-  if (in && h == 0) a.delta[(int64_t)bh * a.T + row] = row < len ? delta : 0.f;
+  if (in && h == 0) {
+    float* const p = a.stat + (int64_t)bh * 2 * a.T + row;
+    p[0] = nl;
+    p[a.T] = row < len ? -delta : 0.f;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------- dk, dv
 template <typename T, int DP>
 __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   constexpr int IMG = BR * DP * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];   // Q and go, two tiles each
-  __shared__ float stats[2][2][BR];                              // -lse and -delta of the tile's rows
+  __shared__ __attribute__((aligned(1024))) char lds[NS * 2 * IMG];   // Q and go of the ring's tiles
+  __shared__ __attribute__((aligned(256))) float stats[NS][2][BR];    // -lse and -delta of their rows
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int nk = (a.T + BKV - 1) / BKV, nr = nk - a.n_sb;
   // workgroups of the blocks with first tokens (the longest) first, then the others, those with the most rows first
@@ -340,21 +357,21 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
     TileLoad<DP, BR, NW> tq, tg;
     tq.init((int)a.q.st * 2, a.D, wave, lane);
     tg.init((int)a.go.st * 2, a.D, wave, lane);
-    float st0 = 0.f;
-    auto issue = [&](int it, int buf) {
-      const int g = it / nt, i0 = (t0 + it - g * nt) * BR, hq = hk * a.grp + g;
+    // -lse and -delta: lanes 0..31 and 32..63 of one 4-byte load (every wave issues it, with the same values, so that all
+    // have the same number of loads under way). Rows past the text read zeros: their Q and go are zeros too.
+    const int soff = (lane & 31) * 4 + (lane >> 5) * a.T * 4;
+    constexpr int LOADS = decltype(tq)::N + decltype(tg)::N + 1;
+    auto issue = [&](int it) {
+      const int g = it / nt, i0 = (t0 + it - g * nt) * BR, hq = hk * a.grp + g, buf = (it - it0) & (NS - 1);
       tq.issue(tile_rsrc<BR>(a.q.p + b * a.q.sb + hq * a.q.sh, a.q.st, i0, len, a.D), lds, buf * 2 * IMG, wave);
       tg.issue(tile_rsrc<BR>(a.go.p + b * a.go.sb + hq * a.go.sh, a.go.st, i0, len, a.D), lds, buf * 2 * IMG + IMG, wave);
-      if (threadIdx.x < 2 * BR) {
-        const int r = i0 + (threadIdx.x & (BR - 1));
-        const int64_t o = ((int64_t)b * a.Hq + hq) * a.T + r;
-        st0 = threadIdx.x < BR ? (r < len ? -a.lse[o] : -INFINITY) : (r < len ? -a.delta[o] : 0.f);
-      }
+      const int rows = a.T - i0 < BR ? a.T - i0 : BR;
+      dma4(make_rsrc(a.stat + ((int64_t)b * a.Hq + hq) * 2 * a.T + i0, (a.T + rows) * 4),
+           reinterpret_cast<const char*>(&stats[0][0][0]), buf * 2 * BR * 4, (lane & 31) < rows ? soff : OOB);
     };
-    auto put = [&](int buf) {
-      if (threadIdx.x < 2 * BR) stats[buf][threadIdx.x / BR][threadIdx.x & (BR - 1)] = st0;
-    };
-    if (it0 < it1) issue(it0, 0);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i)
+      if (it0 + i < it1) issue(it0 + i);
     u32x4 kf[DP / 16], vf[DP / 16];
     const i32x4 kr = tile_rsrc<32>(a.k.p + b * a.k.sb + hk * a.k.sh, a.k.st, j0, len, a.D);
     const i32x4 vr = tile_rsrc<32>(a.v.p + b * a.v.sb + hk * a.v.sh, a.v.st, j0, len, a.D);
@@ -364,12 +381,15 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
       kf[ks] = load16(kr, col < a.D ? r * (int)a.k.st * 2 + col * 2 : OOB);
       vf[ks] = load16(vr, col < a.D ? r * (int)a.v.st * 2 + col * 2 : OOB);
     }
-    put(0);
-    wait_vmcnt<0>();
-    __syncthreads();
     for (int it = it0; it < it1; ++it) {
-      const int buf = (it - it0) & 1, img = buf * 2 * IMG;
-      if (it + 1 < it1) issue(it + 1, buf ^ 1);
+      const int buf = (it - it0) & (NS - 1), img = buf * 2 * IMG;
+      // this wave's loads of tile `it` have arrived when only those of the later ones are under way; behind the barrier
+      // all waves' have, and all are done with the tile whose place the next load takes
+      if (it + 2 < it1) wait_vmcnt<2 * LOADS>();
+      else if (it + 1 < it1) wait_vmcnt<LOADS>();
+      else wait_vmcnt<0>();
+      __syncthreads();
+      if (it + NS - 1 < it1) issue(it + NS - 1);
       const int i0 = (t0 + it % nt) * BR;
       ad.refresh();
       const bool some = i0 + BR - 1 >= j0 && (i0 - (j0 + 31) < a.window || j0 < a.sinks);
@@ -413,9 +433,6 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
           for (int dt = 0; dt < DP / 32; ++dt) dk[dt] = mfma<T>(frag_tr<DP>(lds, ad, img, dt, sl), df, dk[dt]);
         }
       }
-      put(buf ^ 1);
-      wait_vmcnt<0>();
-      __syncthreads();
     }
   }
   const bool in = key < a.T;
@@ -461,7 +478,7 @@ __global__ __launch_bounds__(256) void k_attn_dkv_join(Args a, int pieces) {
 int check_sizes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
   if (B < 0 || T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || D > 128 || D % 8 || window < 0 || sinks < 0)
     return MCE_ATTN_EINVAL;
-  if (T > (int64_t(1) << 30) || Hq * D > MAX_ST) return MCE_ATTN_EINVAL;
+  if (T > (int64_t(1) << 27) || Hq * D > MAX_ST) return MCE_ATTN_EINVAL;
   // one workgroup per 128 rows of every head
   if (T > 0 && (B > (int64_t(1) << 31) / Hq || B * Hq * ((T + 127) / 128) >= (int64_t(1) << 31)))
     return MCE_ATTN_EINVAL;
@@ -602,7 +619,7 @@ size_t mce_attn_bwd_ws_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int6
                              int64_t sinks) {
   if (check_sizes(B, T, Hq, Hkv, D, window, sinks)) return 0;
   const Plan p = make_plan(B, T, Hq, Hkv, D, window, sinks);
-  return (size_t)(align256(B * Hq * T * 4) + align256(p.part_s * 4) + align256(p.part_r * 4));
+  return (size_t)(align256(B * Hq * T * 8) + align256(p.part_s * 4) + align256(p.part_r * 4));
 }
 
 int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
@@ -635,8 +652,8 @@ int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
   a.n_sb = p.n_sb;
   a.S_s = p.S_s;
   a.S_r = p.S_r;
-  a.delta = static_cast<float*>(ws);
-  a.part_s = a.delta + align256(B * Hq * T * 4) / 4;
+  a.stat = static_cast<float*>(ws);
+  a.part_s = a.stat + align256(B * Hq * T * 8) / 4;
   a.part_r = a.part_s + align256(p.part_s * 4) / 4;
   a.dq = static_cast<uint16_t*>(dq);
   a.dk = static_cast<uint16_t*>(dk);

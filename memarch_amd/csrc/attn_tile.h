@@ -99,6 +99,15 @@ __device__ __forceinline__ void dma16(const i32x4& rsrc, const char* lds, int ds
                : "memory");
 }
 
+// The same with 4 bytes per lane, at lds + dst + 4 * lane.
+__device__ __forceinline__ void dma4(const i32x4& rsrc, const char* lds, int dst, int voff) {
+  const uint32_t a = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(LDS_AS const char*)lds + (uint32_t)dst);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(a), "v"(voff), "s"(rsrc)
+               : "memory");
+}
+
 // The swizzle: 8 consecutive rows at one chunk fall on the 8 different 16-byte bank groups of 128 bytes and 16 on the
 // 16 of 256 bytes (ds_read_b128), and the 4 rows x 32 bytes (16 lanes) or x 64 bytes (32 lanes) of a transposing read
 // likewise, so both kinds of reads are free of bank conflicts whichever width the LDS serves at once.
