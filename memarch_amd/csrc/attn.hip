@@ -229,23 +229,39 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
 }
 
 // --------------------------------------------------------------------------------------------------------------- dq
+// Keeps the compiler from moving anything past it.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+// The lane's number, worked out anew wherever it is asked for (registers are scarce in the loops).
+__device__ __forceinline__ int lane_now() {
+  int l = threadIdx.x & 63;
+  asm volatile("" : "+v"(l));
+  return l;
+}
+// the s-th four of eight packed pairs, as a fragment
+__device__ __forceinline__ u32x4 four(const uint32_t (&w)[8], int s) {
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = w[4 * s + e];
+  return r;
+}
+
 template <typename T, int DP>
 __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
   constexpr int IMG = BK * DP * 2;
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nq = (a.T + BQ - 1) / BQ;
   const Place pl(a, blockIdx.x, nq, a.grp);
   const int qb = nq - 1 - pl.blk, b = pl.b, hk = pl.hk, hq = hk * a.grp + pl.g, bh = b * a.Hq + hq;
   const int len = seq_len(a, b);
-  const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
-  const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
+  const int q0 = qb * BQ, r0 = q0 + wave * 32;
   f32x16 acc[DP / 32] = {};
   float delta = 0.f, nl = -INFINITY;
   const float c = a.scale * LOG2E;
   if (q0 < len) {
     const int q1 = (q0 + BQ < len ? q0 + BQ : len) - 1;
     const KeyTiles kt(a, q0, q1);
+    const int lane = lane_now();
     FragAddr<DP> ad;
     ad.init(lane);
     TileLoad<DP, BK, NW> tk, tv;
@@ -266,7 +282,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
     const i32x4 orr = tile_rsrc<32>(a.out + head, ldo, r0, len, a.D), rr = tile_rsrc<32>(a.res + head, ldo, r0, len, a.D);
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
-      const int col = 16 * ks + 8 * h, r = lane & 31;
+      const int col = 16 * ks + 8 * (lane >> 5), r = lane & 31;
       qf[ks] = load16(qr, col < a.D ? r * (int)a.q.st * 2 + col * 2 : OOB);
       gf[ks] = load16(gr, col < a.D ? r * (int)a.go.st * 2 + col * 2 : OOB);
       const int oo = col < a.D ? r * (int)ldo * 2 + col * 2 : OOB;
@@ -278,6 +294,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       }
     }
     delta = sum_halves(delta);
+    const int row = r0 + (lane & 31);
     if (row < len) nl = -a.lse[(int64_t)bh * a.T + row];
     wait_vmcnt<0>();
     __syncthreads();
@@ -287,34 +304,78 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       const int k0 = kt.key0(it);
       ad.refresh();
       if (k0 <= r0 + 31 && (r0 - (k0 + BK - 1) < a.window || k0 < a.sinks)) {
+        // The products of a tile in one sequence, for its two halves of 32 keys: scores (KS each), go v (KS each), dq
+        // (2 DT each). The fragment of each is read PD - 1 products ahead, and the vector work stands between products
+        // that do not wait for it: the exponentials of one half among the next products, ds likewise.
+        constexpr int KS = DP / 16, DT = DP / 32, N = 4 * KS + 4 * DT, PD = 4;
         const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
+        auto read = [&](int i) {
+          if (i < 4 * KS) return frag_rows<DP>(lds, ad, img + i / (2 * KS) * IMG, i / KS & 1, i % KS);
+          i -= 4 * KS;
+          return frag_tr<DP>(lds, ad, img, i % DT, i / DT);
+        };
+        u32x4 f[PD];
+#pragma unroll
+        for (int i = 0; i < PD - 1; ++i) f[i] = read(i);
+        f32x16 s[2], ds[2];
+        uint32_t dw[2][8];
+        int at = 0;                                      // the next product; a constant once unrolled
+        auto product = [&](const u32x4& x, const f32x16& acc0) {
+          if (at + PD - 1 < N) f[(at + PD - 1) % PD] = read(at + PD - 1);
+          const f32x16 r = mfma<T>(f[at % PD], x, acc0);
+          ++at;
+          return r;
+        };
+        auto probs = [&](int kb, int i) {                // the i-th of KS pieces
+#pragma unroll
+          for (int e = i * (16 / KS); e < (i + 1) * (16 / KS); ++e) s[kb][e] = __builtin_amdgcn_exp2f(s[kb][e] * c);
+        };
+        auto grads = [&](int kb, int i, int n) {         // the i-th of n pieces
+#pragma unroll
+          for (int e = i * 8 / n; e < (i + 1) * 8 / n; ++e)
+            dw[kb][e] = pack2<T>(s[kb][2 * e] * ds[kb][2 * e], s[kb][2 * e + 1] * ds[kb][2 * e + 1]);
+        };
+        fence();
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          f32x16 s, ds;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[e] = nl;
+          for (int e = 0; e < 16; ++e) s[kb][e] = nl;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) ds[e] = -delta;
-#pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) s = mfma<T>(frag_rows<DP>(lds, ad, img, kb, ks), qf[ks], s);
-#pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) ds = mfma<T>(frag_rows<DP>(lds, ad, img + IMG, kb, ks), gf[ks], ds);
-          if (!all) mask_keys(s, row, k0 + 32 * kb + 4 * h, a.window, a.sinks, k0 < a.sinks);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) ds[e] *= __builtin_amdgcn_exp2f(s[e] * c);
-#pragma unroll
-          for (int sl = 0; sl < 2; ++sl) {
-            const u32x4 df = frag_acc<T>(ds, sl);
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt)
-              acc[dt] = mfma<T>(frag_tr<DP>(lds, ad, img, dt, 2 * kb + sl), df, acc[dt]);
+          for (int i = 0; i < KS; ++i) {
+            s[kb] = product(qf[i], s[kb]);
+            if (kb == 1) probs(0, i);
+            fence();
           }
+          if (!all) {
+            const int ln = lane_now();
+            mask_keys(s[kb], r0 + (ln & 31), k0 + 32 * kb + 4 * (ln >> 5), a.window, a.sinks, k0 < a.sinks);
+          }
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ds[kb][e] = -delta;
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            ds[kb] = product(gf[i], ds[kb]);
+            if (kb == 0) probs(1, i);
+            else if (i > 0) grads(0, i - 1, KS - 1);
+            fence();
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * DT; ++i) {
+          acc[i % DT] = product(four(dw[i / DT / 2], i / DT & 1), acc[i % DT]);
+          if (i > 0 && i < 2 * DT) grads(1, i - 1, 2 * DT - 1);
+          fence();
         }
       }
       wait_vmcnt<0>();
       __syncthreads();
     }
   }
+  const int ln = lane_now(), h = ln >> 5, row = r0 + (ln & 31);
+  const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
   const bool in = row < a.T;
   store_acc<T, DP>(acc, a.scale, a.dq + ofs, a.D, in, h);
   if (in && h == 0) {
@@ -330,7 +391,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   constexpr int IMG = BR * DP * 2;
   __shared__ __attribute__((aligned(1024))) char lds[NS * 2 * IMG];   // Q and go of the ring's tiles
   __shared__ __attribute__((aligned(256))) float stats[NS][2][BR];    // -lse and -delta of their rows
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nk = (a.T + BKV - 1) / BKV, nr = nk - a.n_sb;
   // workgroups of the blocks with first tokens (the longest) first, then the others, those with the most rows first
   const uint32_t heads = (uint32_t)a.B * a.Hkv, sink_wgs = heads * a.n_sb * a.S_s;
@@ -341,7 +402,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   const int sp = pl.blk % S, blk = pl.blk / S, b = pl.b, hk = pl.hk, bh = b * a.Hkv + hk;
   const int kblk = sink ? blk : a.n_sb + blk;
   const int len = seq_len(a, b);
-  const int kb0 = kblk * BKV, j0 = kb0 + wave * 32, key = j0 + (lane & 31);
+  const int kb0 = kblk * BKV, j0 = kb0 + wave * 32;
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   const float c = a.scale * LOG2E;
   int it0 = 0, it1 = 0;
@@ -352,6 +413,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
     const int t0 = kb0 / BR, nt = (q_end + BR - 1) / BR - t0, total = nt * a.grp;
     it0 = (int)((int64_t)total * sp / S);
     it1 = (int)((int64_t)total * (sp + 1) / S);
+    const int lane = lane_now();
     FragAddr<DP> ad;
     ad.init(lane);
     TileLoad<DP, BR, NW> tq, tg;
@@ -359,15 +421,16 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
     tg.init((int)a.go.st * 2, a.D, wave, lane);
     // -lse and -delta: lanes 0..31 and 32..63 of one 4-byte load (every wave issues it, with the same values, so that all
     // have the same number of loads under way). Rows past the text read zeros: their Q and go are zeros too.
-    const int soff = (lane & 31) * 4 + (lane >> 5) * a.T * 4;
     constexpr int LOADS = decltype(tq)::N + decltype(tg)::N + 1;
     auto issue = [&](int it) {
       const int g = it / nt, i0 = (t0 + it - g * nt) * BR, hq = hk * a.grp + g, buf = (it - it0) & (NS - 1);
       tq.issue(tile_rsrc<BR>(a.q.p + b * a.q.sb + hq * a.q.sh, a.q.st, i0, len, a.D), lds, buf * 2 * IMG, wave);
       tg.issue(tile_rsrc<BR>(a.go.p + b * a.go.sb + hq * a.go.sh, a.go.st, i0, len, a.D), lds, buf * 2 * IMG + IMG, wave);
       const int rows = a.T - i0 < BR ? a.T - i0 : BR;
+      const int ln = lane_now();
       dma4(make_rsrc(a.stat + ((int64_t)b * a.Hq + hq) * 2 * a.T + i0, (a.T + rows) * 4),
-           reinterpret_cast<const char*>(&stats[0][0][0]), buf * 2 * BR * 4, (lane & 31) < rows ? soff : OOB);
+           reinterpret_cast<const char*>(&stats[0][0][0]), buf * 2 * BR * 4,
+           (ln & 31) < rows ? ((ln & 31) + (ln >> 5) * a.T) * 4 : OOB);
     };
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i)
@@ -377,7 +440,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
     const i32x4 vr = tile_rsrc<32>(a.v.p + b * a.v.sb + hk * a.v.sh, a.v.st, j0, len, a.D);
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
-      const int col = 16 * ks + 8 * h, r = lane & 31;
+      const int col = 16 * ks + 8 * (lane >> 5), r = lane & 31;
       kf[ks] = load16(kr, col < a.D ? r * (int)a.k.st * 2 + col * 2 : OOB);
       vf[ks] = load16(vr, col < a.D ? r * (int)a.v.st * 2 + col * 2 : OOB);
     }
@@ -394,24 +457,44 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
       ad.refresh();
       const bool some = i0 + BR - 1 >= j0 && (i0 - (j0 + 31) < a.window || j0 < a.sinks);
       if (some) {
+        // The products of a tile in one sequence: the scores (KS), go v (KS), dv (2 DT), dk (2 DT). The fragment of each
+        // is read PD - 1 products ahead, and the vector work stands between the products that do not wait for it:
+        // exponentials among go v, ds among dv. fence() keeps both where they are.
+        constexpr int KS = DP / 16, DT = DP / 32, N = 2 * KS + 4 * DT, PD = 3;
+        auto read = [&](int i) {
+          if (i < KS) return frag_rows<DP>(lds, ad, img, 0, i);
+          if (i < 2 * KS) return frag_rows<DP>(lds, ad, img + IMG, 0, i - KS);
+          i -= 2 * KS;
+          if (i < 2 * DT) return frag_tr<DP>(lds, ad, img + IMG, i % DT, i / DT);
+          i -= 2 * DT;
+          return frag_tr<DP>(lds, ad, img, i % DT, i / DT);
+        };
+        u32x4 f[PD];
+#pragma unroll
+        for (int i = 0; i < PD - 1; ++i) f[i] = read(i);
+        const int h = lane_now() >> 5;
         f32x16 s, ds;
 #pragma unroll
         for (int e4 = 0; e4 < 4; ++e4) {
           const f32x4 x = *reinterpret_cast<const f32x4*>(&stats[buf][0][8 * e4 + 4 * h]);
-          const f32x4 y = *reinterpret_cast<const f32x4*>(&stats[buf][1][8 * e4 + 4 * h]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[4 * e4 + e] = x[e];
-            ds[4 * e4 + e] = y[e];
-          }
+          for (int e = 0; e < 4; ++e) s[4 * e4 + e] = x[e];
+        }
+        fence();
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          f[(i + PD - 1) % PD] = read(i + PD - 1);
+          s = mfma<T>(f[i % PD], kf[i], s);
+          fence();
         }
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) s = mfma<T>(frag_rows<DP>(lds, ad, img, 0, ks), kf[ks], s);
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(&stats[buf][1][8 * e4 + 4 * h]);
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) ds = mfma<T>(frag_rows<DP>(lds, ad, img + IMG, 0, ks), vf[ks], ds);
-        const bool all = j0 + 31 <= i0 && i0 + BR - 1 - j0 < a.window;
-        if (!all) {
-          const int rel = i0 + 4 * h - key;
+          for (int e = 0; e < 4; ++e) ds[4 * e4 + e] = y[e];
+        }
+        if (!(j0 + 31 <= i0 && i0 + BR - 1 - j0 < a.window)) {
+          const int key = j0 + (lane_now() & 31), rel = i0 + 4 * h - key;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int d = rel + 8 * (e / 4) + e % 4;
@@ -419,22 +502,41 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
             s[e] = see ? s[e] : -INFINITY;
           }
         }
+        uint32_t dw[8];
+        fence();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[e] = __builtin_amdgcn_exp2f(s[e] * c);
-          ds[e] *= s[e];
+        for (int i = 0; i < KS; ++i) {
+          f[(KS + i + PD - 1) % PD] = read(KS + i + PD - 1);
+          ds = mfma<T>(f[(KS + i) % PD], vf[i], ds);
+#pragma unroll
+          for (int e = i * (8 / KS); e < (i + 1) * (8 / KS); ++e) {
+            s[2 * e] = __builtin_amdgcn_exp2f(s[2 * e] * c);
+            s[2 * e + 1] = __builtin_amdgcn_exp2f(s[2 * e + 1] * c);
+          }
+          fence();
+        }
+        u32x4 pf;
+#pragma unroll
+        for (int i = 0; i < 2 * DT; ++i) {
+          f[(2 * KS + i + PD - 1) % PD] = read(2 * KS + i + PD - 1);
+          if (i % DT == 0) pf = frag_acc<T>(s, i / DT);
+          dv[i % DT] = mfma<T>(f[(2 * KS + i) % PD], pf, dv[i % DT]);
+#pragma unroll
+          for (int e = (i - 1) * 8 / (2 * DT - 1); e < i * 8 / (2 * DT - 1); ++e)
+            dw[e] = pack2<T>(s[2 * e] * ds[2 * e], s[2 * e + 1] * ds[2 * e + 1]);
+          fence();
         }
 #pragma unroll
-        for (int sl = 0; sl < 2; ++sl) {
-          const u32x4 pf = frag_acc<T>(s, sl), df = frag_acc<T>(ds, sl);
-#pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt) dv[dt] = mfma<T>(frag_tr<DP>(lds, ad, img + IMG, dt, sl), pf, dv[dt]);
-#pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt) dk[dt] = mfma<T>(frag_tr<DP>(lds, ad, img, dt, sl), df, dk[dt]);
+        for (int i = 0; i < 2 * DT; ++i) {
+          constexpr int AT = 2 * KS + 2 * DT;
+          if (AT + i + PD - 1 < N) f[(AT + i + PD - 1) % PD] = read(AT + i + PD - 1);
+          dk[i % DT] = mfma<T>(f[(AT + i) % PD], four(dw, i / DT), dk[i % DT]);
+          fence();
         }
       }
     }
   }
+  const int ln = lane_now(), h = ln >> 5, key = j0 + (ln & 31);
   const bool in = key < a.T;
   if (S == 1) {
     const int64_t ofs = (((int64_t)b * a.T + key) * a.Hkv + hk) * a.D;

@@ -118,27 +118,32 @@ __device__ __forceinline__ int swz(int r) {
   else return (r1 << 2) | ((r0 ^ r3) << 1) | r2;
 }
 
-// Loads of a tile of ROWS rows by NW waves: instruction i moves 1 KiB of the image; wave w issues i = w, w + NW, ...
+// Loads of a tile of ROWS rows by NW waves: instruction i moves 1 KiB of the image; wave w issues i = w, w + NW, ... A
+// wave's instructions are a multiple of 16 rows apart, so they have one swizzle, and one offset per lane serves them all
+// (a lane without a column stays past every resource's records).
 template <int DP, int ROWS, int NW>
 struct TileLoad {
   static constexpr int ROWB = DP * 2;
   static constexpr int BYTES = ROWS * ROWB;
   static constexpr int RPI = 1024 / ROWB;            // rows per instruction
   static constexpr int N = BYTES / 1024 / NW;        // instructions per wave
-  static_assert(BYTES % (1024 * NW) == 0, "whole instructions per wave");
-  int voff[N];
+  static_assert(BYTES % (1024 * NW) == 0 && NW * RPI % 16 == 0, "whole instructions per wave, 16 rows apart");
+  int voff, step;
   // ldb: bytes between rows; d: columns that exist (a multiple of 8): the others read zeros
   __device__ __forceinline__ void init(int ldb, int d, int wave, int lane) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int row = (j * NW + wave) * RPI + lane / (DP / 8);
-      const int c = (lane % (DP / 8)) ^ swz<DP>(row);
-      voff[j] = c * 8 < d ? row * ldb + c * 16 : OOB;
-    }
+    const int row = wave * RPI + lane / (DP / 8);
+    const int c = (lane % (DP / 8)) ^ swz<DP>(row);
+    voff = c * 8 < d ? row * ldb + c * 16 : OOB;
+    step = NW * RPI * ldb;
   }
   __device__ __forceinline__ void issue(const i32x4& rsrc, const char* lds, int img, int wave) const {
+    int v = voff;
+    asm volatile("" : "+v"(v));                      // the sums below are made again each time: registers are scarce
 #pragma unroll
-    for (int j = 0; j < N; ++j) dma16(rsrc, lds, img + (j * NW + wave) * 1024, voff[j]);
+    for (int j = 0; j < N; ++j) {
+      dma16(rsrc, lds, img + (j * NW + wave) * 1024, v);
+      v += step;
+    }
   }
 };
 
