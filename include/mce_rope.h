@@ -17,8 +17,8 @@
  *
  * Buffers: q [B, T, Hq, D] and k [B, T, Hkv, D] with element strides (batch, token, head) and a contiguous last
  * dimension, gradients g like them; cos and sin [P, R/2] contiguous; outputs contiguous. Any alignment and any even
- * R <= D <= 256: rows of whole 16-byte pieces (all pointers 16-byte aligned, strides and D multiples of 8, R of 16)
- * move as such, others element by element. Every call is asynchronous on `stream`, allocates nothing, and returns 0 or
+ * R <= D <= 256: heads made of whole 16-byte pieces (of n = 8 elements, 4 in fp32: all pointers 16-byte aligned, strides
+ * and D multiples of n, and R/2, or with interleaved pairs R) move as such, others element by element. Every call is asynchronous on `stream`, allocates nothing, and returns 0 or
  * an MCE_ROPE_E* code; arguments are checked before anything is launched.
  */
 #ifndef MCE_ROPE_H

@@ -2,11 +2,10 @@
 // The C ABI and the formulas are in include/mce_rope.h.
 //
 // Both passes are HBM streams (2 element accesses per element forward, 3 backward), so the layout serves the loads: a
-// head vector belongs to a group of G lanes (a power of two), each lane moving two 16-byte pieces of it (two pairs of
-// them in fp32). In the half layout the two pieces are the two halves of 8 rotation pairs, interleaved they lie side by
-// side; either way a lane rotates what it loaded with 8 consecutive table entries, and the norm's sum is the only value
-// that crosses lanes. A group takes UNR heads of one token at once: their loads are issued together and share the
-// token's table entries.
+// head vector belongs to a group of G lanes (a power of two), each lane moving two 16-byte pieces of it, neighbouring
+// lanes neighbouring pieces. In the half layout a lane's two pieces are the two sides of its rotation pairs, interleaved
+// pairs lie inside a piece; either way the norm's sum is the only value that crosses lanes. A group takes UNR heads of one
+// token at once: their loads are issued together, kept as loaded until each is used, and share the token's table entries.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -16,15 +15,16 @@
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int UNR_F = 2, UNR_B = 1;   // heads per group at once, forward and backward
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// 8 consecutive elements as fp32
+// A 16-byte piece: N elements of T
 template <typename T>
 struct Piece {
-  __device__ static __forceinline__ void load(const T* p, float (&v)[8]) {
-    const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  static constexpr int N = 8;
+  __device__ static __forceinline__ void unpack(const u32x4& a, float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t w = a[e];
@@ -32,43 +32,53 @@ struct Piece {
       v[2 * e + 1] = (float)__builtin_bit_cast(T, (uint16_t)(w >> 16));
     }
   }
-  __device__ static __forceinline__ void store(T* p, const float (&v)[8]) {
+  __device__ static __forceinline__ u32x4 pack(const float (&v)[8]) {
     u32x4 a;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       a[e] = (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * e]) |
              ((uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * e + 1]) << 16);
-    __builtin_nontemporal_store(a, reinterpret_cast<u32x4*>(p));
+    return a;
   }
 };
 template <>
 struct Piece<float> {
-  __device__ static __forceinline__ void load(const float* p, float (&v)[8]) {
-    const f32x4 a = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)),
-                b = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p + 4));
+  static constexpr int N = 4;
+  __device__ static __forceinline__ void unpack(const u32x4& a, float (&v)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      v[e] = a[e];
-      v[4 + e] = b[e];
+      const uint32_t w = a[e];
+      v[e] = __builtin_bit_cast(float, w);
     }
   }
-  __device__ static __forceinline__ void store(float* p, const float (&v)[8]) {
-    f32x4 a, b;
+  __device__ static __forceinline__ u32x4 pack(const float (&v)[4]) {
+    u32x4 a;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a[e] = v[e];
-      b[e] = v[4 + e];
-    }
-    __builtin_nontemporal_store(a, reinterpret_cast<f32x4*>(p));
-    __builtin_nontemporal_store(b, reinterpret_cast<f32x4*>(p + 4));
+    for (int e = 0; e < 4; ++e) a[e] = __builtin_bit_cast(uint32_t, v[e]);
+    return a;
   }
 };
-__device__ __forceinline__ void load_f32(const float* p, float (&v)[8]) {   // table entries and weights: kept in caches
-  const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+template <typename T>
+__device__ __forceinline__ u32x4 load_piece(const T* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T* p, const u32x4& a) {
+  __builtin_nontemporal_store(a, reinterpret_cast<u32x4*>(p));
+}
+// N fp32 table entries or weights (multiples of 2, 8-byte aligned at least): kept in the caches
+template <int N>
+__device__ __forceinline__ void load_f32(const float* p, float* v) {
+  if constexpr (N % 4 == 0) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e] = a[e];
-    v[4 + e] = b[e];
+    for (int i = 0; i < N / 4; ++i) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * i + e] = a[e];
+    }
+  } else {
+    v[0] = p[0];
+    v[1] = p[1];
   }
 }
 
@@ -109,41 +119,46 @@ __device__ __forceinline__ float group_sum(float x, int G) {
   return x;
 }
 
-// A lane's two pieces and its table entries: lane p of the group.
+// A lane's two pieces of a head vector of D elements, N to a piece: their first elements, whether they exist and whether
+// they are rotated.
+template <int N, bool IL>
 struct Lane {
-  int c0, c1;      // element offsets of the pieces
-  bool on0, on1;   // whether they exist
-  bool turns;      // whether they are rotated, by table entries 8p .. 8p+7
-  __device__ __forceinline__ Lane(const Args& a, int p, bool il) {
-    const int half = a.R / 2;
-    turns = 8 * p < half;
-    if (turns) {
-      c0 = il ? 16 * p : 8 * p;
-      c1 = il ? c0 + 8 : c0 + half;
-    } else {
-      c0 = a.R + 16 * (p - half / 8);
-      c1 = c0 + 8;
+  int c0, c1;
+  bool on0, on1, turn0, turn1;
+  __device__ __forceinline__ Lane(const Args& a, int p) {
+    if constexpr (IL) {   // piece p and the one half the pieces further
+      c0 = N * p;
+      c1 = c0 + N * ((a.D / N + 1) / 2);
+      on0 = p < (a.D / N + 1) / 2;
+      on1 = on0 && c1 < a.D;
+      turn0 = on0 && c0 < a.R;
+      turn1 = on1 && c1 < a.R;
+    } else {              // the two sides of N pairs; behind the rotated part as above
+      const int half = a.R / 2, rest = (a.D - a.R) / N, q = p - half / N;
+      turn0 = turn1 = q < 0;
+      c0 = turn0 ? N * p : a.R + N * q;
+      c1 = turn0 ? c0 + half : c0 + N * ((rest + 1) / 2);
+      on0 = turn0 || q < (rest + 1) / 2;
+      on1 = turn0 || (on0 && c1 < a.D);
     }
-    on0 = c0 < a.D;
-    on1 = c1 < a.D;
   }
 };
 
-// the rotation by (c, s); the inverse one with the sine's sign turned
-template <bool IL>
-__device__ __forceinline__ void rotate(float (&u)[8], float (&v)[8], const float (&c)[8], const float (&s)[8]) {
+// the rotation by the lane's table entries (c, s): N pairs across its pieces, or N/2 inside each
+template <int N, bool IL>
+__device__ __forceinline__ void rotate(float (&u)[N], float (&v)[N], const float (&c)[N], const float (&s)[N]) {
   if constexpr (IL) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < N / 2; ++e) {
       const float a = u[2 * e], b = u[2 * e + 1], x = v[2 * e], y = v[2 * e + 1];
       u[2 * e] = a * c[e] - b * s[e];
       u[2 * e + 1] = b * c[e] + a * s[e];
-      v[2 * e] = x * c[4 + e] - y * s[4 + e];
-      v[2 * e + 1] = y * c[4 + e] + x * s[4 + e];
+      v[2 * e] = x * c[N / 2 + e] - y * s[N / 2 + e];
+      v[2 * e + 1] = y * c[N / 2 + e] + x * s[N / 2 + e];
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < N; ++e) {
       const float a = u[e], b = v[e];
       u[e] = a * c[e] - b * s[e];
       v[e] = b * c[e] + a * s[e];
@@ -153,21 +168,23 @@ __device__ __forceinline__ void rotate(float (&u)[8], float (&v)[8], const float
 
 // A workgroup's share of one side: groups of a.G lanes over units of UNR heads of one token.
 template <typename T, bool NORM, bool IL, bool BWD, int UNR>
-__global__ __launch_bounds__(THREADS) void k_rope(Args a) {
+__global__ __launch_bounds__(THREADS, 4) void k_rope(Args a) {
+  using P = Piece<T>;
+  constexpr int N = P::N;
   const bool kside = blockIdx.x >= a.blocks_q;
-  const Side& sd = a.side[kside];
+  const Side sd = kside ? a.side[1] : a.side[0];
   const uint32_t block = kside ? blockIdx.x - a.blocks_q : blockIdx.x;
   const uint32_t blocks = kside ? gridDim.x - a.blocks_q : a.blocks_q;
   const int G = a.G, p = threadIdx.x & (G - 1);
   const uint32_t groups = THREADS / G, group = threadIdx.x / G;
   const uint32_t hu = (sd.H + UNR - 1) / UNR, units = a.tokens * hu;
-  const Lane ln(a, p, IL);
-  float w0[8] = {}, w1[8] = {}, dw0[8] = {}, dw1[8] = {};
+  const Lane<N, IL> ln(a, p);
+  float w0[N], w1[N], dw0[N] = {}, dw1[N] = {};
   if constexpr (NORM) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w0[e] = w1[e] = 1.f;
-    if (ln.on0 && sd.w != nullptr) load_f32(sd.w + ln.c0, w0);
-    if (ln.on1 && sd.w != nullptr) load_f32(sd.w + ln.c1, w1);
+    for (int e = 0; e < N; ++e) w0[e] = w1[e] = 1.f;
+    if (ln.on0 && sd.w != nullptr) load_f32<N>(sd.w + ln.c0, w0);
+    if (ln.on1 && sd.w != nullptr) load_f32<N>(sd.w + ln.c1, w1);
   }
   const float inv_d = 1.f / a.D;
   for (uint32_t unit = block * groups + group; unit < units; unit += blocks * groups) {
@@ -175,92 +192,112 @@ __global__ __launch_bounds__(THREADS) void k_rope(Args a) {
     const T* const xp = static_cast<const T*>(sd.x) + b * sd.xb + t * sd.xt;
     const T* const gp = BWD ? static_cast<const T*>(sd.g) + b * sd.gb + t * sd.gt : nullptr;
     T* const yp = static_cast<T*>(sd.y) + (int64_t)tok * sd.H * a.D;
-    float x0[UNR][8], x1[UNR][8], g0[UNR][8], g1[UNR][8];
+    u32x4 xr0[UNR], xr1[UNR], gr0[UNR], gr1[UNR];
 #pragma unroll
     for (int j = 0; j < UNR; ++j) {
       const bool on = h0 + j < (uint32_t)sd.H;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x0[j][e] = x1[j][e] = g0[j][e] = g1[j][e] = 0.f;
+      xr0[j] = xr1[j] = gr0[j] = gr1[j] = u32x4{};
       if constexpr (!BWD || NORM) {
-        if (on && ln.on0) Piece<T>::load(xp + (h0 + j) * sd.xh + ln.c0, x0[j]);
-        if (on && ln.on1) Piece<T>::load(xp + (h0 + j) * sd.xh + ln.c1, x1[j]);
+        if (on && ln.on0) xr0[j] = load_piece(xp + (h0 + j) * sd.xh + ln.c0);
+        if (on && ln.on1) xr1[j] = load_piece(xp + (h0 + j) * sd.xh + ln.c1);
       }
       if constexpr (BWD) {
-        if (on && ln.on0) Piece<T>::load(gp + (h0 + j) * sd.gh + ln.c0, g0[j]);
-        if (on && ln.on1) Piece<T>::load(gp + (h0 + j) * sd.gh + ln.c1, g1[j]);
+        if (on && ln.on0) gr0[j] = load_piece(gp + (h0 + j) * sd.gh + ln.c0);
+        if (on && ln.on1) gr1[j] = load_piece(gp + (h0 + j) * sd.gh + ln.c1);
       }
     }
+    // table entries; where nothing turns the identity
     const int64_t row = table_row(a, b, t);
-    float c[8] = {}, s[8] = {};
-    if (ln.turns && row >= 0) {
-      load_f32(a.cos + row * (a.R / 2) + 8 * p, c);
-      load_f32(a.sin + row * (a.R / 2) + 8 * p, s);
-    }
-    if constexpr (BWD) {
+    float c[N], s[N];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = -s[e];
+    for (int e = 0; e < N; ++e) {
+      c[e] = 1.f;
+      s[e] = 0.f;
     }
-    const float bad = row >= 0 ? 0.f : __builtin_nanf("");
+    if (row >= 0) {
+      const int64_t o = row * (a.R / 2);
+      if constexpr (IL) {
+        if (ln.turn0) {
+          load_f32<N / 2>(a.cos + o + ln.c0 / 2, c);
+          load_f32<N / 2>(a.sin + o + ln.c0 / 2, s);
+        }
+        if (ln.turn1) {
+          load_f32<N / 2>(a.cos + o + ln.c1 / 2, c + N / 2);
+          load_f32<N / 2>(a.sin + o + ln.c1 / 2, s + N / 2);
+        }
+      } else if (ln.turn0) {
+        load_f32<N>(a.cos + o + ln.c0, c);
+        load_f32<N>(a.sin + o + ln.c0, s);
+      }
+    }
+    if constexpr (BWD) {   // the inverse rotation
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] = -s[e];
+    }
 #pragma unroll
     for (int j = 0; j < UNR; ++j) {
+      float x0[N], x1[N], u[N], v[N];
       float r = 1.f;
+      if constexpr (!BWD || NORM) {
+        P::unpack(xr0[j], x0);
+        P::unpack(xr1[j], x1);
+      }
       if constexpr (NORM) {
         float q = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q += x0[j][e] * x0[j][e] + x1[j][e] * x1[j][e];
+        for (int e = 0; e < N; ++e) q += x0[e] * x0[e] + x1[e] * x1[e];
         r = 1.f / sqrtf(group_sum(q, G) * inv_d + a.eps);
-      }
-      float(&u)[8] = BWD ? g0[j] : x0[j];
-      float(&v)[8] = BWD ? g1[j] : x1[j];
-      if constexpr (NORM && !BWD) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          u[e] = u[e] * r * w0[e];
-          v[e] = v[e] * r * w1[e];
+        for (int e = 0; e < N; ++e) {
+          x0[e] *= r;
+          x1[e] *= r;
         }
       }
-      if (ln.turns) rotate<IL>(u, v, c, s);
-      if constexpr (NORM && BWD) {   // u, v: dn
+      if constexpr (BWD) {
+        P::unpack(gr0[j], u);
+        P::unpack(gr1[j], v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          u[e] = NORM ? x0[e] * w0[e] : x0[e];
+          v[e] = NORM ? x1[e] * w1[e] : x1[e];
+        }
+      }
+      // (a lane in which only one or none of its pieces turns has the identity in the other's place; half layout: both)
+      if (ln.turn0) rotate<N, IL>(u, v, c, s);
+      if constexpr (NORM && BWD) {   // u, v: dn; heads past the last have zeros
         float dot = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float a0 = x0[j][e] * r, a1 = x1[j][e] * r;
-          if (h0 + j < (uint32_t)sd.H) {
-            dw0[e] += u[e] * a0;
-            dw1[e] += v[e] * a1;
-          }
-          x0[j][e] = a0;
-          x1[j][e] = a1;
+        for (int e = 0; e < N; ++e) {
+          dw0[e] += u[e] * x0[e];
+          dw1[e] += v[e] * x1[e];
           u[e] *= w0[e];
           v[e] *= w1[e];
-          dot += u[e] * a0 + v[e] * a1;
+          dot += u[e] * x0[e] + v[e] * x1[e];
         }
         dot = group_sum(dot, G) * inv_d;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          u[e] = r * (u[e] - x0[j][e] * dot);
-          v[e] = r * (v[e] - x1[j][e] * dot);
+        for (int e = 0; e < N; ++e) {
+          u[e] = r * (u[e] - x0[e] * dot);
+          v[e] = r * (v[e] - x1[e] * dot);
         }
       }
+      if (row < 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        u[e] += bad;
-        v[e] += bad;
+        for (int e = 0; e < N; ++e) u[e] = v[e] = __builtin_nanf("");
+        if constexpr (NORM && BWD) dw0[0] = __builtin_nanf("");   // one NaN is enough to show
       }
       if (h0 + j < (uint32_t)sd.H) {
-        if (ln.on0) Piece<T>::store(yp + (int64_t)(h0 + j) * a.D + ln.c0, u);
-        if (ln.on1) Piece<T>::store(yp + (int64_t)(h0 + j) * a.D + ln.c1, v);
+        if (ln.on0) store_piece(yp + (int64_t)(h0 + j) * a.D + ln.c0, P::pack(u));
+        if (ln.on1) store_piece(yp + (int64_t)(h0 + j) * a.D + ln.c1, P::pack(v));
       }
-    }
-    if constexpr (NORM && BWD) {
-      if (row < 0) dw0[0] += bad;   // one NaN is enough to show
     }
   }
   if constexpr (NORM && BWD) {
     __shared__ float red[THREADS / 64][256];
     // lanes of one wave with the same place in their groups, then the waves
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < N; ++e)
       for (int o = 32; o >= G; o >>= 1) {
         dw0[e] += __shfl_xor(dw0[e], o);
         dw1[e] += __shfl_xor(dw1[e], o);
@@ -268,7 +305,7 @@ __global__ __launch_bounds__(THREADS) void k_rope(Args a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (lane < G) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < N; ++e) {
         if (ln.on0) red[wave][ln.c0 + e] = dw0[e];
         if (ln.on1) red[wave][ln.c1 + e] = dw1[e];
       }
@@ -289,7 +326,7 @@ template <typename T, bool NORM, bool IL, bool BWD>
 __global__ __launch_bounds__(THREADS) void k_rope_any(Args a) {
   constexpr int E = 4;   // elements per lane: D <= 256
   const bool kside = blockIdx.x >= a.blocks_q;
-  const Side& sd = a.side[kside];
+  const Side sd = kside ? a.side[1] : a.side[0];
   const uint32_t block = kside ? blockIdx.x - a.blocks_q : blockIdx.x;
   const uint32_t blocks = kside ? gridDim.x - a.blocks_q : a.blocks_q;
   const int lane = threadIdx.x & 63;
@@ -366,28 +403,29 @@ __global__ __launch_bounds__(THREADS) void k_rope_any(Args a) {
   }
 }
 
-// dw[c] = sum of the parts of column c, 64 rows apart per lane in a fixed order: one wave per column of a side.
+// dw[c] = sum of the parts of column c, in fp64, 64 rows apart per lane in a fixed order: one wave per column of a side.
 __global__ __launch_bounds__(64) void k_rope_dw(const float* part_q, int nq, const float* part_k, int nk, float* dqw,
                                                 float* dkw, int D) {
   const bool kside = (int)blockIdx.x >= D;
   const int c = kside ? blockIdx.x - D : blockIdx.x, n = kside ? nk : nq;
   const float* const p = kside ? part_k : part_q;
-  float v = 0.f;
+  double v = 0.;
   for (int i = threadIdx.x; i < n; i += 64) v += p[(int64_t)i * D + c];
-  v = group_sum(v, 64);
-  if (threadIdx.x == 0) (kside ? dkw : dqw)[c] = v;
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if (threadIdx.x == 0) (kside ? dkw : dqw)[c] = (float)v;
 }
 
 // -------------------------------------------------------------------------------------------------------- host side
 
-int64_t lanes_of(int64_t D, int64_t R) { return R / 16 + (D - R + 15) / 16; }
-int group_of(int64_t lanes) {
+// Lanes per head vector: two pieces of n elements each.
+int group_of(int64_t D, int64_t R, int64_t n, bool interleaved) {
+  const int64_t lanes = interleaved ? (D / n + 1) / 2 : R / 2 / n + ((D - R) / n + 1) / 2;
   int g = 1;
   while (g < lanes) g *= 2;
   return g;
 }
 
-// Workgroups of the backward's two sides: in proportion to their heads, at most MAX_BLOCKS together.
+// Workgroups of the backward's two sides: in proportion to their heads, at most MAX_BLOCKS (4 per CU) together.
 constexpr int64_t MAX_BLOCKS = 1024;
 void bwd_blocks(int64_t tokens, int64_t Hq, int64_t Hkv, int64_t& nq, int64_t& nk) {
   const int64_t per = 16;   // head vectors below which another workgroup does not pay
@@ -407,33 +445,41 @@ bool bad_sizes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D) {
          B * T * (Hq > Hkv ? Hq : Hkv) >= (int64_t(1) << 31);
 }
 
-bool whole_pieces(const void* p, int64_t sb, int64_t st, int64_t sh) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (sb | st | sh) % 8 == 0;
+bool whole_pieces(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t n) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (sb | st | sh) % n == 0;
+}
+
+// Whether head vectors and tables can be moved in pieces of n elements: rotation pairs across whole pieces (half layout)
+// or inside them, table entries in fours (or twos: fp32, interleaved).
+bool whole_layout(int64_t D, int64_t R, int64_t n, bool interleaved, const void* cos, const void* sin, const void* qw,
+                  const void* kw) {
+  return D % n == 0 && (interleaved ? R : R / 2) % n == 0 && (R / 2) % (interleaved ? n / 2 : n) == 0 &&
+         whole_pieces(cos, 0, 0, 0, n) && whole_pieces(sin, 0, 0, 0, n) && whole_pieces(qw, 0, 0, 0, n) &&
+         whole_pieces(kw, 0, 0, 0, n);
 }
 
 using attn::finish;
 
 template <typename T, bool NORM, bool IL, bool BWD>
 void launch(Args& a, bool pieces, int64_t nq, int64_t nk, hipStream_t st) {
-  if (BWD) {
+  if constexpr (BWD) {
     a.blocks_q = (uint32_t)nq;
     if (pieces)
-      hipLaunchKernelGGL((k_rope<T, NORM, IL, BWD, 2>), dim3((unsigned)(nq + nk)), dim3(THREADS), 0, st, a);
+      hipLaunchKernelGGL((k_rope<T, NORM, IL, BWD, UNR_B>), dim3((unsigned)(nq + nk)), dim3(THREADS), 0, st, a);
     else
       hipLaunchKernelGGL((k_rope_any<T, NORM, IL, BWD>), dim3((unsigned)(nq + nk)), dim3(THREADS), 0, st, a);
-    return;
-  }
-  if (!pieces) {
+  } else if (!pieces) {
     auto blocks = [&](int H) { return (uint32_t)(((int64_t)a.tokens * H + THREADS / 64 - 1) / (THREADS / 64)); };
     a.blocks_q = blocks(a.side[0].H);
     hipLaunchKernelGGL((k_rope_any<T, NORM, IL, BWD>), dim3(a.blocks_q + blocks(a.side[1].H)), dim3(THREADS), 0, st, a);
-    return;
+  } else {
+    auto blocks = [&](int H) {
+      return (uint32_t)(((int64_t)a.tokens * ((H + UNR_F - 1) / UNR_F) * a.G + THREADS - 1) / THREADS);
+    };
+    a.blocks_q = blocks(a.side[0].H);
+    hipLaunchKernelGGL((k_rope<T, NORM, IL, BWD, UNR_F>), dim3(a.blocks_q + blocks(a.side[1].H)), dim3(THREADS), 0, st,
+                       a);
   }
-  auto blocks = [&](int H, int unr) {
-    return (uint32_t)(((int64_t)a.tokens * ((H + unr - 1) / unr) * a.G + THREADS - 1) / THREADS);
-  };
-  a.blocks_q = blocks(a.side[0].H, 4);
-  hipLaunchKernelGGL((k_rope<T, NORM, IL, BWD, 4>), dim3(a.blocks_q + blocks(a.side[1].H, 4)), dim3(THREADS), 0, st, a);
 }
 
 template <bool BWD>
@@ -494,11 +540,11 @@ int mce_rope_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
   a.D = (int)D;
   a.R = (int)R;
   a.eps = eps;
-  const bool pieces = D % 8 == 0 && R % 16 == 0 && whole_pieces(q, q_sb, q_st, q_sh) &&
-                      whole_pieces(k, k_sb, k_st, k_sh) && whole_pieces(q_out, 0, 0, 0) &&
-                      whole_pieces(k_out, 0, 0, 0) && whole_pieces(cos, 0, 0, 0) && whole_pieces(sin, 0, 0, 0) &&
-                      whole_pieces(qw, 0, 0, 0) && whole_pieces(kw, 0, 0, 0);
-  a.G = group_of(lanes_of(D, R));
+  const int64_t n = dtype == MCE_ROPE_F32 ? 4 : 8;
+  const bool pieces = whole_layout(D, R, n, interleaved, cos, sin, qw, kw) && whole_pieces(q, q_sb, q_st, q_sh, n) &&
+                      whole_pieces(k, k_sb, k_st, k_sh, n) && whole_pieces(q_out, 0, 0, 0, n) &&
+                      whole_pieces(k_out, 0, 0, 0, n);
+  a.G = group_of(D, R, n, interleaved);
   return run<false>(a, norm, interleaved, dtype, pieces, 0, 0, reinterpret_cast<hipStream_t>(stream));
 }
 
@@ -545,12 +591,12 @@ int mce_rope_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
     a.D = (int)D;
     a.R = (int)R;
     a.eps = eps;
-    const bool pieces = D % 8 == 0 && R % 16 == 0 && whole_pieces(q, q_sb, q_st, q_sh) &&
-                        whole_pieces(k, k_sb, k_st, k_sh) && whole_pieces(gq, gq_sb, gq_st, gq_sh) &&
-                        whole_pieces(gk, gk_sb, gk_st, gk_sh) && whole_pieces(dq, 0, 0, 0) &&
-                        whole_pieces(dk, 0, 0, 0) && whole_pieces(cos, 0, 0, 0) && whole_pieces(sin, 0, 0, 0) &&
-                        whole_pieces(qw, 0, 0, 0) && whole_pieces(kw, 0, 0, 0);
-    a.G = group_of(lanes_of(D, R));
+    const int64_t n = dtype == MCE_ROPE_F32 ? 4 : 8;
+    const bool pieces = whole_layout(D, R, n, interleaved, cos, sin, qw, kw) && whole_pieces(q, q_sb, q_st, q_sh, n) &&
+                        whole_pieces(k, k_sb, k_st, k_sh, n) && whole_pieces(gq, gq_sb, gq_st, gq_sh, n) &&
+                        whole_pieces(gk, gk_sb, gk_st, gk_sh, n) && whole_pieces(dq, 0, 0, 0, n) &&
+                        whole_pieces(dk, 0, 0, 0, n);
+    a.G = group_of(D, R, n, interleaved);
     const int e = run<true>(a, norm, interleaved, dtype, pieces, nq, nk, st);
     if (e) return e;
   }
