@@ -23,6 +23,7 @@ constexpr int THREADS = 64 * NW;
 constexpr int BK = 32;             // keys per tile of a wave
 constexpr int HC = 32;             // query heads per workgroup: the columns of the products
 constexpr int MIN_TILES = 2 * NW;  // tiles below which a sequence is not split further
+constexpr int TARGET = 1024;       // workgroups that fill the GPU, some of them with shorter sequences
 
 struct Args {
   const uint16_t *q, *k, *v;
@@ -237,40 +238,53 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 2 : 1) void k_paged(Args a) {
   }
 }
 
-// out = the parts of one query head joined: one wave per head, 2 columns per lane.
+// out = the parts of one query head joined: one wave per head, 2 columns per lane. The parts' states are read by all
+// lanes at once and their factors shared through LDS, so that the sums' loads depend on nothing.
 template <typename T>
 __global__ __launch_bounds__(64) void k_paged_join(Args a) {
+  __shared__ float f[TARGET];
   const int64_t row = blockIdx.x;
   const Seen sn(a, (int)(row / a.Hq));
-  const int run = sn.run(a.S), n = (sn.tiles + run - 1) / run, d = threadIdx.x * 2;
+  const int run = sn.run(a.S), n = (sn.tiles + run - 1) / run, lane = threadIdx.x, d = lane * 2;
   const float c = a.scale * LOG2E;
   const float* const ml = a.ml + row * a.S * 2;
   float mm = -INFINITY;
-  for (int s = 0; s < n; ++s) mm = fmaxf(mm, ml[2 * s]);
+  for (int s = lane; s < n; s += 64) mm = fmaxf(mm, ml[2 * s]);
+  for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
   const float mu = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, x = 0.f, y = 0.f;
+  float ll = 0.f;
+  for (int s = lane; s < n; s += 64) {
+    f[s] = __builtin_amdgcn_exp2f((ml[2 * s] - mu) * c);
+    ll = __builtin_fmaf(ml[2 * s + 1], f[s], ll);
+  }
+  for (int o = 32; o > 0; o >>= 1) ll += __shfl_xor(ll, o);
+  __syncthreads();
   if (d < a.D) {
     const float* const p = a.part + row * a.S * a.D + d;
+    float x = 0.f, y = 0.f;
+#pragma unroll 8
     for (int s = 0; s < n; ++s) {
-      const float f = __builtin_amdgcn_exp2f((ml[2 * s] - mu) * c);
-      ll = __builtin_fmaf(ml[2 * s + 1], f, ll);
-      x = __builtin_fmaf(p[(int64_t)s * a.D], f, x);
-      y = __builtin_fmaf(p[(int64_t)s * a.D + 1], f, y);
+      const float2 v = *reinterpret_cast<const float2*>(p + (int64_t)s * a.D);
+      x = __builtin_fmaf(v.x, f[s], x);
+      y = __builtin_fmaf(v.y, f[s], y);
     }
-    const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+    const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);   // nothing seen: 0; NaN stays
     *reinterpret_cast<uint32_t*>(a.out + row * a.D + d) = pack2<T>(x * inv, y * inv);
   }
 }
 
 // -------------------------------------------------------------------------------------------------------- host side
 
-// Workgroups per key/value head of a sequence: as many as fill the GPU, at most one per MIN_TILES tiles of the longest
-// sequence that the table can hold.
-constexpr int64_t TARGET = 1024;
+// Workgroups per key/value head of a sequence. From 512 heads on one each: they fill the GPU, and the second launch and the
+// parts cost more than even rounds gain (96 sequences of 8 heads of 64, window 1024: 42.8 us against 46.7 with two each).
+// With fewer, TARGET in all (256 heads of 128, up to 8192 keys: 170, 160 and 165 us with 2, 4 and 8 each; 32 heads, up to
+// 131072 keys: 304, 295 and 313 us with 16, 32 and 64), at most one per MIN_TILES tiles of the longest sequence that the
+// table can hold.
 int64_t splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t page, int64_t max_pages, int64_t window, int64_t sinks) {
   int64_t n = page * max_pages;
   if (window > 0 && window + sinks < n) n = window + sinks;
   const int64_t tiles = (n + BK - 1) / BK + 2, units = B * Hkv * ((Hq / Hkv + HC - 1) / HC);
+  if (units >= TARGET / 2) return 1;
   int64_t s = (TARGET + units - 1) / units;
   const int64_t most = (tiles + MIN_TILES - 1) / MIN_TILES;
   s = s < most ? s : most;
