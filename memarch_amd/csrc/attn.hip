@@ -237,6 +237,11 @@ __device__ __forceinline__ int lane_now() {
   asm volatile("" : "+v"(l));
   return l;
 }
+// x, copied at this place (of 16 copies of one value the compiler would keep a set for the whole loop)
+__device__ __forceinline__ float now(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 // the s-th four of eight packed pairs, as a fragment
 __device__ __forceinline__ u32x4 four(const uint32_t (&w)[8], int s) {
   u32x4 r;
@@ -256,7 +261,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
   const int len = seq_len(a, b);
   const int q0 = qb * BQ, r0 = q0 + wave * 32;
   f32x16 acc[DP / 32] = {};
-  float delta = 0.f, nl = -INFINITY;
+  float delta = 0.f, nl = -INFINITY, sum = 0.f;
   const float c = a.scale * LOG2E;
   if (q0 < len) {
     const int q1 = (q0 + BQ < len ? q0 + BQ : len) - 1;
@@ -304,84 +309,93 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       const int k0 = kt.key0(it);
       ad.refresh();
       if (k0 <= r0 + 31 && (r0 - (k0 + BK - 1) < a.window || k0 < a.sinks)) {
-        // The products of a tile in one sequence, for its two halves of 32 keys: scores (KS each), go v (KS each), dq
-        // (2 DT each). The fragment of each is read PD - 1 products ahead, and the vector work stands between products
-        // that do not wait for it: the exponentials of one half among the next products, ds likewise.
-        constexpr int KS = DP / 16, DT = DP / 32, N = 4 * KS + 4 * DT, PD = 4;
+        // The products of a tile in one sequence, half (32 keys) after half: scores (KS), go v (KS), dq (2 DT fragments,
+        // two products each). The fragment of each is read PD - 1 steps ahead, and the exponentials stand between the
+        // products of go v. ds goes into dq as what it rounds to and what that leaves over: with one rounding alone dq
+        // was off by 2.5e-3 of its norm in bf16 (1.7e-3 is the rounding of dq itself), with the rest 1.9e-3.
+        constexpr int KS = DP / 16, DT = DP / 32, H = 2 * KS + 2 * DT, PD = 3;
         const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
         auto read = [&](int i) {
-          if (i < 4 * KS) return frag_rows<DP>(lds, ad, img + i / (2 * KS) * IMG, i / KS & 1, i % KS);
-          i -= 4 * KS;
-          return frag_tr<DP>(lds, ad, img, i % DT, i / DT);
+          const int kb = i / H;
+          i %= H;
+          if (i < 2 * KS) return frag_rows<DP>(lds, ad, img + i / KS * IMG, kb, i % KS);
+          i -= 2 * KS;
+          return frag_tr<DP>(lds, ad, img, i % DT, 2 * kb + i / DT);
         };
         u32x4 f[PD];
 #pragma unroll
         for (int i = 0; i < PD - 1; ++i) f[i] = read(i);
-        f32x16 s[2], ds[2];
-        uint32_t dw[2][8];
-        int at = 0;                                      // the next product; a constant once unrolled
-        auto product = [&](const u32x4& x, const f32x16& acc0) {
-          if (at + PD - 1 < N) f[(at + PD - 1) % PD] = read(at + PD - 1);
-          const f32x16 r = mfma<T>(f[at % PD], x, acc0);
-          ++at;
-          return r;
-        };
-        auto probs = [&](int kb, int i) {                // the i-th of KS pieces
-#pragma unroll
-          for (int e = i * (16 / KS); e < (i + 1) * (16 / KS); ++e) s[kb][e] = __builtin_amdgcn_exp2f(s[kb][e] * c);
-        };
-        auto grads = [&](int kb, int i, int n) {         // the i-th of n pieces
-#pragma unroll
-          for (int e = i * 8 / n; e < (i + 1) * 8 / n; ++e)
-            dw[kb][e] = pack2<T>(s[kb][2 * e] * ds[kb][2 * e], s[kb][2 * e + 1] * ds[kb][2 * e + 1]);
-        };
         fence();
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
+          auto step = [&](int i) -> const u32x4& {         // the half's i-th fragment; reads the one PD - 1 further
+            const int at = kb * H + i;
+            if (at + PD - 1 < 2 * H) f[(at + PD - 1) % PD] = read(at + PD - 1);
+            return f[at % PD];
+          };
+          f32x16 s, ds;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[kb][e] = nl;
+          for (int e = 0; e < 16; ++e) s[e] = now(nl);
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
-            s[kb] = product(qf[i], s[kb]);
-            if (kb == 1) probs(0, i);
+            s = mfma<T>(step(i), qf[i], s);
             fence();
           }
           if (!all) {
             const int ln = lane_now();
-            mask_keys(s[kb], r0 + (ln & 31), k0 + 32 * kb + 4 * (ln >> 5), a.window, a.sinks, k0 < a.sinks);
+            mask_keys(s, r0 + (ln & 31), k0 + 32 * kb + 4 * (ln >> 5), a.window, a.sinks, k0 < a.sinks);
           }
-        }
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) ds[kb][e] = -delta;
+          for (int e = 0; e < 16; ++e) ds[e] = now(-delta);
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
-            ds[kb] = product(gf[i], ds[kb]);
-            if (kb == 0) probs(1, i);
-            else if (i > 0) grads(0, i - 1, KS - 1);
+            ds = mfma<T>(step(KS + i), gf[i], ds);
+#pragma unroll
+            for (int e = i * (16 / KS); e < (i + 1) * (16 / KS); ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * c);
             fence();
           }
-        }
+          // ds of 16 keys as fragments
+          u32x4 hi[2], lo[2];
+          auto split = [&](int sl, int i) {
+            const int e = 8 * sl + 2 * i;
+            const float x = s[e] * ds[e], y = s[e + 1] * ds[e + 1];
+            sum += x + y;
+            const uint32_t w = pack2<T>(x, y);
+            hi[sl][i] = w;
+            lo[sl][i] = pack2<T>(x - lo_f32<T>(w), y - hi_f32<T>(w));
+          };
 #pragma unroll
-        for (int i = 0; i < 4 * DT; ++i) {
-          acc[i % DT] = product(four(dw[i / DT / 2], i / DT & 1), acc[i % DT]);
-          if (i > 0 && i < 2 * DT) grads(1, i - 1, 2 * DT - 1);
-          fence();
+          for (int i = 0; i < 4; ++i) split(0, i);
+#pragma unroll
+          for (int i = 0; i < 2 * DT; ++i) {
+            const int sl = i / DT, dt = i % DT;
+            const u32x4& x = step(2 * KS + i);
+            acc[dt] = mfma<T>(x, hi[sl], acc[dt]);
+            acc[dt] = mfma<T>(x, lo[sl], acc[dt]);
+            if (sl == 0) {
+#pragma unroll
+              for (int e = dt * 4 / DT; e < (dt + 1) * 4 / DT; ++e) split(1, e);
+            }
+            fence();
+          }
         }
       }
       wait_vmcnt<0>();
       __syncthreads();
     }
   }
+  sum = sum_halves(sum);
   const int ln = lane_now(), h = ln >> 5, row = r0 + (ln & 31);
   const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
   const bool in = row < a.T;
   store_acc<T, DP>(acc, a.scale, a.dq + ofs, a.D, in, h);
   if (in && h == 0) {
+    // The output's probabilities were rounded, so delta is off by some of its rounding, and the sum of the row's ds, which
+    // should be 0, by as much: what k_attn_dkv gets is put right by it (dk of 8 heads of 96, T = 1000: off by 1.42 times
+    // its own rounding instead of 1.51).
     float* const p = a.stat + (int64_t)bh * 2 * a.T + row;
     p[0] = nl;
-    p[a.T] = row < len ? -delta : 0.f;
+    p[a.T] = row < len ? -(delta + sum) : 0.f;
   }
 }
 
