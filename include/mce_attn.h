@@ -9,13 +9,15 @@
  *   j <= i  and  (window = 0  or  i - j < window  or  j < sinks)  and  i < lengths[b]
  *   s_ij = scale q_i . k_j;  p_i = softmax of s_ij over the j that i sees;  out_i = sum_j p_ij v_j
  * (window = 0: every earlier position; lengths NULL: T). A row that sees nothing (i >= lengths[b]) has out = 0, and the
- * gradients of such positions are 0. What lies in masked places is not used beyond a finite factor 0: rows at or past
- * lengths[b] are never read.
+ * gradients of such positions are 0; rows at or past lengths[b] are never read. Inside a sequence, masked pairs get a
+ * weight of exactly 0: finite values there do not matter, a NaN or an infinity may reach rows of the same or the next
+ * 128-row block that do not see it.
  *   d_i = go_i . out_i;  ds_ij = p_ij (go_i . v_j - d_i)
  *   dq_i = scale sum_j ds_ij k_j;  dk_j = scale sum_i ds_ij q_i;  dv_j = sum_i p_ij go_i  (dk, dv summed over the heads
  *   that share them)
  * Products take 16-bit operands and sum in fp32; softmax statistics are fp32; p and ds are rounded to the element type
- * as operands of the second products, results are rounded once.
+ * as operands of the second products (half of dq's products take what the rounding of ds leaves over as well), results
+ * are rounded once. In fp16, p (go v - d) has to stay in range, as the results have to.
  *
  * Buffers: q [B, T, Hq, D], k and v [B, T, Hkv, D], go like q: element strides (batch, token, head) are given, the last
  * dimension is contiguous; 16-byte aligned, strides multiples of 8, the token stride at least D. D is a multiple of 8 up to 128. out, dq
@@ -62,8 +64,8 @@ MCE_ATTN_API int mce_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t
                               int64_t window, int64_t sinks, float scale, int dtype, void* out, void* res,
                               float* lse, void* stream);
 
-/* dq, dk and dv from the forward's inputs, out, res and lse. The workspace holds d (fp32 [B, Hq, T]) and, where the sums of
- * dk and dv are split over workgroups, their fp32 parts. */
+/* dq, dk and dv from the forward's inputs, out, res and lse. The workspace holds -lse and -d (fp32 [B, Hq, 2, T]) and,
+ * where the sums of dk and dv are shared by several workgroups, their fp32 parts. */
 MCE_ATTN_API size_t mce_attn_bwd_ws_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                                           int64_t sinks);
 MCE_ATTN_API int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,

@@ -19,6 +19,7 @@ from .fused_ops import _ptr, _stream
 # element-type codes of include/mce_attn.h
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}
 MAX_HEAD_DIM = 128
+_MAX_INT = 2 ** 31 - 1   # more than any position
 _MAX_STRIDE = 1 << 21   # elements between two tokens (the library's limit)
 
 
@@ -82,13 +83,13 @@ def _mask_args(window, sinks):
         raise ValueError("window must be at least 1 (None: every earlier position is seen, without sinks)")
     if sinks < 0:
         raise ValueError(f"sinks={sinks} must not be negative")
-    return window, int(sinks)
+    return min(window, _MAX_INT), min(int(sinks), _MAX_INT)
 
 
 def _scale(scale, d):
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"scale={scale} must be positive and finite")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"scale={scale} must be positive and between 1e-30 and 1e30")
     return scale
 
 
@@ -151,7 +152,8 @@ def window_attention(q, k, v, window=None, sinks=0, lengths=None, scale=None):
     """Causal attention of q [B, T, Hq, D] over k, v [B, T, Hkv, D] (bf16 or fp16, Hq a multiple of Hkv, D a multiple of
     8 up to 128, any strides) -> [B, T, Hq, D]. Position i sees j <= i with i - j < window or j < sinks (window None:
     every j <= i). lengths [B] marks a padded batch: positions at or past a sequence's length see nothing and are seen
-    by none, their output and gradients are 0 and what lies in their rows is not read. scale defaults to D^-0.5.
+    by none, their output and gradients are 0 and what lies in their rows is not read (inside a length, a NaN or an
+    infinity may reach rows near it that do not see it, as 0 * NaN does in a dense form). scale defaults to D^-0.5.
     Under torch.autocast fp32 tensors are cast to its type, as for scaled_dot_product_attention. Differentiable once
     in q, k and v."""
     if torch.is_autocast_enabled("cuda"):
@@ -205,7 +207,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sink
     scale = _scale(scale, D)
     if lengths is None:
         raise ValueError("lengths must be given")
-    lengths = _lengths(lengths, B, 2**31 - 1)
+    lengths = _lengths(lengths, B, _MAX_INT)
     _check_same(q, ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("lengths", lengths))
     max_pages = block_table.shape[1]
     if max_pages > 1 and block_table.stride(1) != 1 or B > 1 and block_table.stride(0) < max_pages:

@@ -309,10 +309,11 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       const int k0 = kt.key0(it);
       ad.refresh();
       if (k0 <= r0 + 31 && (r0 - (k0 + BK - 1) < a.window || k0 < a.sinks)) {
-        // The products of a tile in one sequence, half (32 keys) after half: scores (KS), go v (KS), dq (2 DT fragments,
-        // two products each). The fragment of each is read PD - 1 steps ahead, and the exponentials stand between the
-        // products of go v. ds goes into dq as what it rounds to and what that leaves over: with one rounding alone dq
-        // was off by 2.5e-3 of its norm in bf16 (1.7e-3 is the rounding of dq itself), with the rest 1.9e-3.
+        // The products of a tile in one sequence, half (32 keys) after half: scores (KS), go v (KS), dq (2 DT). The fragment
+        // of each is read PD - 1 steps ahead, and the exponentials stand between the products of go v. Rounding ds is what
+        // dq loses most by; of every second slice of 16 keys what the rounding leaves over goes into dq as well. In units
+        // of dq's own rounding it is off by 1.3 to 1.4 then, for 3% of a training step; by 1.5 without any of the rest, by
+        // 1.1 to 1.2 with all of it, for 7%.
         constexpr int KS = DP / 16, DT = DP / 32, H = 2 * KS + 2 * DT, PD = 3;
         const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
         auto read = [&](int i) {
@@ -355,14 +356,14 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
             fence();
           }
           // ds of 16 keys as fragments
-          u32x4 hi[2], lo[2];
+          u32x4 hi[2], lo;
           auto split = [&](int sl, int i) {
             const int e = 8 * sl + 2 * i;
             const float x = s[e] * ds[e], y = s[e + 1] * ds[e + 1];
             sum += x + y;
             const uint32_t w = pack2<T>(x, y);
             hi[sl][i] = w;
-            lo[sl][i] = pack2<T>(x - lo_f32<T>(w), y - hi_f32<T>(w));
+            if (sl == 0) lo[i] = pack2<T>(x - lo_f32<T>(w), y - hi_f32<T>(w));
           };
 #pragma unroll
           for (int i = 0; i < 4; ++i) split(0, i);
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
             const int sl = i / DT, dt = i % DT;
             const u32x4& x = step(2 * KS + i);
             acc[dt] = mfma<T>(x, hi[sl], acc[dt]);
-            acc[dt] = mfma<T>(x, lo[sl], acc[dt]);
+            if (sl == 0) acc[dt] = mfma<T>(x, lo, acc[dt]);
             if (sl == 0) {
 #pragma unroll
               for (int e = dt * 4 / DT; e < (dt + 1) * 4 / DT; ++e) split(1, e);
@@ -614,7 +615,7 @@ Args make_args(Strided q, Strided k, Strided v, const int32_t* lengths, int64_t 
   a.Hkv = (int)Hkv;
   a.grp = (int)(Hq / Hkv);
   a.D = (int)D;
-  a.window = window == 0 || window > T ? INT32_MAX : (int)window;
+  a.window = window == 0 || window >= T ? INT32_MAX : (int)window;
   a.sinks = a.window == INT32_MAX ? 0 : (int)(sinks > T ? T : sinks);
   a.scale = scale;
   return a;

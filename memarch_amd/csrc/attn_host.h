@@ -30,7 +30,8 @@ inline int check_strided(const void* p, int64_t sb, int64_t st, int64_t sh, int6
   return MCE_ATTN_OK;
 }
 
-inline bool good_scale(float s) { return s > 0.f && s <= 3.0e38f; }
+// Scales outside this range leave no room for the logarithms and products that are formed with them.
+inline bool good_scale(float s) { return s >= 1e-30f && s <= 1e30f; }
 
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 

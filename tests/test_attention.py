@@ -159,7 +159,7 @@ def test_window_attention_refusals():
         with pytest.raises(ValueError):
             wa(*bad)
     for kw, match in ((dict(window=0, sinks=3), "window"), (dict(window=-2), "window"), (dict(window=4, sinks=-1), "sinks"),
-                      (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"),
+                      (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=1e-31), "scale"),
                       (dict(scale=float("nan")), "scale"), (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths"),
                       (dict(lengths=torch.zeros(2)), "lengths"), (dict(lengths=torch.zeros(2, 1, dtype=torch.int32)), "lengths"),
                       (dict(lengths=torch.zeros(2, dtype=torch.int32)), "lengths is on cpu")):
@@ -267,7 +267,7 @@ def test_attn_c_abi_checks_need_no_gpu(lib):
 
     for kw in (dict(B=-1), dict(T=-1), dict(Hq=3, Hkv=2), dict(Hkv=0), dict(D=60), dict(D=136), dict(D=0),
                dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")),
-               dict(dtype=0), dict(q=None), dict(out=None), dict(st=56), dict(st=1 << 22), dict(T=(1 << 27) + 1),
+               dict(scale=1e-31), dict(dtype=0), dict(q=None), dict(out=None), dict(st=56), dict(st=1 << 22), dict(T=(1 << 27) + 1),
                dict(B=1 << 40)):
         assert fwd(**kw) == 1, kw
     for kw in (dict(q=p + 2), dict(out=p + 8), dict(res=p + 4), dict(st=68), dict(sh=4)):

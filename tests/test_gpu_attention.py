@@ -74,6 +74,25 @@ def test_padded_batches(lens, window, sinks):
         assert all(not x[i, max(n, 0):].any() for x in got)
 
 
+@pytest.mark.parametrize("b,t,hq,hkv,d,window,sinks", [
+    (1, 2300, 4, 1, 64, 0, 0),         # every earlier key: rows of a key block shared by several workgroups
+    (1, 2300, 4, 1, 128, 1000, 4),     # a window long enough for that, and the block with the first tokens apart
+    (1, 2100, 2, 2, 64, 70, 200),      # two blocks with first tokens, each shared
+    (2, 1300, 8, 1, 96, 300, 130)])
+def test_shared_key_blocks(b, t, hq, hkv, d, window, sinks):
+    print(f"attn shared {b} {t} {window} {sinks}", flush=True)
+    lens = None if b == 1 else torch.tensor([t, 700])
+    _check(*_inputs(b, t, hq, hkv, d, BF, seed=t + d), window, sinks, lens)
+
+
+def test_window_as_long_as_the_text_and_longer():
+    """A window that holds the whole text is no window; sinks change nothing then."""
+    x = [t.cuda() for t in _inputs(2, 200, 4, 2, 64, HF, seed=12)]
+    base = _step(*x, 0, 0)
+    for window, sinks in ((200, 0), (200, 7), (201, 3), (2 ** 40, 2 ** 40)):
+        assert all(torch.equal(a, b) for a, b in zip(_step(*x, window, sinks), base)), window
+
+
 @pytest.mark.parametrize("scale", [1e-4, 1.0, 3.0])
 def test_scales(scale):
     _check(*_inputs(1, 100, 2, 1, 64, BF, seed=6), 30, 0, None, scale)
