@@ -93,6 +93,11 @@ struct Place {
   }
 };
 
+// Whether rows r0 .. r0 + 31 see one of the 32 keys from k0 on.
+__device__ __forceinline__ bool some_keys(const Args& a, int r0, int k0) {
+  return k0 <= r0 + 31 && (r0 - (k0 + 31) < a.window || k0 < a.sinks);
+}
+
 // Masks a 32 x 32 block of scores held as [keys][rows]: accumulator element e of lane l is key
 // k0h + 8*(e/4) + e%4 (k0h = first key + 4*(l/32)) and row `row` (of lane l%32). Both forms are free of branches; the
 // one without first tokens in the block is a compare and a select per element.
@@ -308,32 +313,36 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
       const int k0 = kt.key0(it);
       ad.refresh();
-      if (k0 <= r0 + 31 && (r0 - (k0 + BK - 1) < a.window || k0 < a.sinks)) {
+      // the halves of the tile (32 keys) that the wave's rows see a key of: first .. last - 1
+      const bool see0 = some_keys(a, r0, k0), see1 = some_keys(a, r0, k0 + 32);
+      const int first = see0 ? 0 : 1, last = see1 ? 2 : 1;
+      if (see0 || see1) {
         // The products of a tile in one sequence, half (32 keys) after half: scores (KS), go v (KS), dq (2 DT). The fragment
         // of each is read PD - 1 steps ahead, and the exponentials stand between the products of go v. Rounding ds is what
         // dq loses most by; of every second slice of 16 keys what the rounding leaves over goes into dq as well. In units
         // of dq's own rounding it is off by 1.3 to 1.4 then, for 3% of a training step; by 1.5 without any of the rest, by
         // 1.1 to 1.2 with all of it, for 7%.
         constexpr int KS = DP / 16, DT = DP / 32, H = 2 * KS + 2 * DT, PD = 3;
-        const bool all = k0 + BK - 1 <= r0 && r0 + 31 - k0 < a.window;
-        auto read = [&](int i) {
-          const int kb = i / H;
-          i %= H;
-          if (i < 2 * KS) return frag_rows<DP>(lds, ad, img + i / KS * IMG, kb, i % KS);
+        static_assert(H % PD == 0, "each half starts at the ring's first place");
+        auto read = [&](int kb, int i) {
+          const int rows = img + kb * 32 * DP * 2;
+          if (i < 2 * KS) return frag_rows<DP>(lds, ad, rows + i / KS * IMG, 0, i % KS);
           i -= 2 * KS;
-          return frag_tr<DP>(lds, ad, img, i % DT, 2 * kb + i / DT);
+          return frag_tr<DP>(lds, ad, rows, i % DT, i / DT);
         };
         u32x4 f[PD];
 #pragma unroll
-        for (int i = 0; i < PD - 1; ++i) f[i] = read(i);
+        for (int i = 0; i < PD - 1; ++i) f[i] = read(first, i);
         fence();
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          auto step = [&](int i) -> const u32x4& {         // the half's i-th fragment; reads the one PD - 1 further
-            const int at = kb * H + i;
-            if (at + PD - 1 < 2 * H) f[(at + PD - 1) % PD] = read(at + PD - 1);
-            return f[at % PD];
+        for (int kb = first; kb < last; ++kb) {
+          // the half's i-th fragment; reads the one PD - 1 further (behind the last half: the last's again)
+          auto step = [&](int i) {
+            const u32x4 x = f[i % PD];
+            const int at = i + PD - 1;
+            f[at % PD] = at < H ? read(kb, at) : read(last - 1, at - H);
+            return x;
           };
+          const int kh = k0 + 32 * kb;
           f32x16 s, ds;
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[e] = now(nl);
@@ -342,9 +351,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
             s = mfma<T>(step(i), qf[i], s);
             fence();
           }
-          if (!all) {
+          if (!(kh + 31 <= r0 && r0 + 31 - kh < a.window)) {
             const int ln = lane_now();
-            mask_keys(s, r0 + (ln & 31), k0 + 32 * kb + 4 * (ln >> 5), a.window, a.sinks, k0 < a.sinks);
+            mask_keys(s, r0 + (ln & 31), kh + 4 * (ln >> 5), a.window, a.sinks, kh < a.sinks);
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) ds[e] = now(-delta);
@@ -370,7 +379,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
 #pragma unroll
           for (int i = 0; i < 2 * DT; ++i) {
             const int sl = i / DT, dt = i % DT;
-            const u32x4& x = step(2 * KS + i);
+            const u32x4 x = step(2 * KS + i);
             acc[dt] = mfma<T>(x, hi[sl], acc[dt]);
             if (sl == 0) acc[dt] = mfma<T>(x, lo, acc[dt]);
             if (sl == 0) {
