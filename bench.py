@@ -24,6 +24,11 @@ FETCH_SIZE / WRITE_SIZE counters) and prints its size.
 d = 2048 model (rows = N = 32768, H = 4d = 8192, bf16, lm.py:45-50): one line with the forward + backward HBM
 throughput against the 8 TB/s roofline (algorithmic bytes: forward reads gu and writes out, 3 rows x H
 elements; backward reads gu and go and writes d gu, 5 rows x H elements).
+
+`--op qk_norm_rope`, `--op window_attention` and `--op paged_attention` measure the attention operators of the same
+model (32 texts of 1024 tokens, 16 heads of 128, bf16; `--window`, `--sinks`): one line each with the pass (forward and
+backward; the paged cache: one new token for each of 64 sequences of up to 8192) and its share of the peak that bounds
+it, from the bytes or operations that it cannot do without.
 """
 import argparse
 import ctypes
@@ -70,6 +75,7 @@ def kernel_names(d, folded, dbias):
     return [k.format(**fmt) for k in PROF_KERNELS]
 # the siblings of the north-star op (--op): the same contractions on the same configuration inputs
 SIBLING_OPS = ("linear_ce", "linear_ce_sparse", "chunk_ce")
+ATTENTION_OPS = ("qk_norm_rope", "window_attention", "paged_attention")
 
 
 def fold_nr(d):
@@ -89,10 +95,14 @@ def _args():
     ap.add_argument("--stage-reps", type=int, default=0,
                     help="extra isolated timed repetitions of each C-ABI stage after the timed steps (0: none)")
     ap.add_argument("--calibrate-copy", action="store_true", help="time a 1 GiB device copy and exit")
-    ap.add_argument("--op", choices=("fused_ce",) + SIBLING_OPS + ("induct", "swiglu"), default="fused_ce",
+    ap.add_argument("--op", choices=("fused_ce",) + SIBLING_OPS + ("induct", "swiglu") + ATTENTION_OPS,
+                    default="fused_ce",
                     help="fused_ce: the north-star operator (default); linear_ce, linear_ce_sparse, chunk_ce: its "
                          "siblings (fused_ops.py:39-101, full2.py:753-836) on the same inputs; induct: the "
-                         "keys-and-locks producer (full2.py:1499-1535); swiglu: the SwiGLU gate kernels")
+                         "keys-and-locks producer (full2.py:1499-1535); swiglu: the SwiGLU gate kernels; the others: "
+                         "the attention operators")
+    ap.add_argument("--window", type=int, default=512, help="the attention operators: window (0: every earlier token)")
+    ap.add_argument("--sinks", type=int, default=4, help="the attention operators: first tokens that stay visible")
     ap.add_argument("--path", choices=("one-pass", "recompute"), default="one-pass",
                     help="one-pass: the logits gradient formed in the forward (default); recompute: the backward "
                          "recomputes the logits")
@@ -660,6 +670,63 @@ def bench_swiglu(args):
     print(json.dumps(res), flush=True)
 
 
+def bench_attention(args):
+    """One attention operator (--op) through its public entry point, timed with torch events on the current stream."""
+    from memarch_amd import attention, rotary
+    dev = torch.device("cuda", 0)
+    gen = torch.Generator(device=dev).manual_seed(2024)
+    texts, t, h, d = 32, 1024, 16, 128
+    mk = lambda *s: torch.randn(*s, generator=gen, device=dev).bfloat16()
+    window, sinks = (args.window or None), (args.sinks if args.window else 0)
+    if args.op == "paged_attention":
+        b, most, page, hkv = 64, 8192, 64, 4
+        pages = b * most // page
+        kc, vc, q = mk(pages, page, hkv, d), mk(pages, page, hkv, d), mk(b, h, d)
+        table = torch.randperm(pages, generator=gen, device=dev).view(b, -1).int()
+        lens = torch.randint(most // 3, most + 1, (b,), generator=gen, device=dev).int()
+        seen = lens.clamp(max=args.window + sinks) if window else lens
+        step = lambda: attention.paged_attention(q, kc, vc, table, lens, window=window, sinks=sinks)
+        nbytes, flops = int(seen.sum()) * 4 * hkv * d + 4 * b * h * d, int(seen.sum()) * 4 * h * d
+        config = {"sequences": b, "tokens": most, "page": page, "heads": h, "kv_heads": hkv, "head_dim": d}
+    else:
+        q, k, v, g = (mk(texts, t, h, d).requires_grad_() for _ in range(4))
+        config = {"texts": texts, "tokens": t, "heads": h, "kv_heads": h, "head_dim": d}
+        if args.op == "qk_norm_rope":
+            cos, sin = rotary.rope_table(t, d, device=dev)
+            w = torch.ones(d, device=dev, requires_grad=True)
+            step = lambda: torch.autograd.grad(rotary.qk_norm_rope(q, k, cos, sin, w, w), (q, k, w), (g, g))
+            nbytes, flops = 5 * 2 * q.numel() * 2, 0
+        else:
+            step = lambda: torch.autograd.grad(attention.window_attention(q, k, v, window=window, sinks=sinks),
+                                               (q, k, v), g)
+            i = torch.arange(t)[:, None]
+            j = torch.arange(t)[None]
+            see = (j <= i) if window is None else (j <= i) & ((i - j < window) | (j < sinks))
+            nbytes, flops = 8 * q.numel() * 2, int(see.sum()) * texts * h * d * 14
+    if args.op != "qk_norm_rope":
+        config.update(window=args.window, sinks=sinks)
+    for _ in range(args.warmup):
+        step()
+    torch.cuda.synchronize()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    for _ in range(args.steps):
+        step()
+    e1.record()
+    torch.cuda.synchronize()
+    dt = e0.elapsed_time(e1) / args.steps * 1e-3
+    by_flops = flops / PEAK_BF16 > nbytes / PEAK_HBM
+    value, unit, peak = (flops / dt / 1e12, "TFLOP/s", PEAK_BF16 / 1e12) if by_flops else \
+        (nbytes / dt / 1e9, "GB/s", PEAK_HBM / 1e9)
+    what = "one new token" if args.op == "paged_attention" else "fwd+bwd"
+    print(json.dumps({
+        "metric": f"{unit} {args.op} {what}", "value": round(value, 1), "unit": unit, "n_gpus": 1, "steps": args.steps,
+        "warmup": args.warmup, "ms_per_step": round(dt * 1e3, 4), "higher_is_better": True, "scaling": "weak",
+        "vs_baseline": None, "dtype": "bf16", "data": "synthetic (seeded normal)", "config": config,
+        "roofline": {"bound": "mfma" if by_flops else "hbm", "achieved": round(value, 1), "peak": peak, "unit": unit,
+                     "frac": round(value / peak, 4), "bytes": nbytes, "flops": flops}}), flush=True)
+
+
 def main():
     global SPARSE_KC
     args = _args()
@@ -679,6 +746,9 @@ def main():
         return
     if args.op == "induct":
         bench_induct(args)
+        return
+    if args.op in ATTENTION_OPS:
+        bench_attention(args)
         return
     from memarch_amd import fused_ops
     from memarch_amd.chunk_ce import chunk_ce

@@ -203,6 +203,9 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sink
     if block_table.dim() != 2 or block_table.shape[0] != B or block_table.dtype is not torch.int32:
         raise ValueError(f"block_table must be int32 [B={B}, max_pages], got {tuple(block_table.shape)} "
                          f"{block_table.dtype}")
+    if block_table.shape[1] * page > min(2 ** 30, 2 ** 38 // page):
+        raise ValueError(f"{block_table.shape[1]} pages of {page} tokens per sequence are not supported (2^30 tokens, "
+                         "2^38 / page)")
     window, sinks = _mask_args(window, sinks)
     scale = _scale(scale, D)
     if lengths is None:

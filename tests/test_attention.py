@@ -186,6 +186,11 @@ def test_paged_attention_refusals():
             pa(*args)
     with pytest.raises(ValueError, match="sinks"):
         pa(q, kc, kc, table, lens, window=3, sinks=-1)
+    with pytest.raises(ValueError, match="per sequence"):
+        pa(q, kc, kc, torch.zeros(3, (1 << 26) + 1, **i32), lens)
+    big = _bf(2, 65536, 2, 64)
+    with pytest.raises(ValueError, match="per sequence"):
+        pa(q, big, big, torch.zeros(3, 65, **i32), lens)
     with pytest.raises(ValueError, match="lengths is on cpu"):
         pa(q, kc, kc, table, torch.zeros(3, dtype=torch.int32))
 
