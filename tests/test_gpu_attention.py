@@ -373,3 +373,30 @@ def test_decoding_follows_the_prompt():
             # both are within (u + u) of the same sum: u |out| each, and u P|v| <= u max|v| each
             tol = 2 * 1.05 * 2.0 ** -8 * (want.abs() + float(v.abs().max()))
             assert torch.isfinite(got).all() and ((got.float() - want).abs() <= tol).all()
+
+
+def test_backward_twice_inference_and_changed_inputs():
+    """A kept graph gives the same gradients again, inference mode the same values, and an input changed between forward
+    and backward an error."""
+    from memarch_amd.attention import window_attention
+    from memarch_amd.rotary import qk_norm_rope, rope_table
+    q, k, v, go = (x.cuda() for x in _inputs(2, 150, 4, 2, 64, BF, seed=21))
+    cos, sin = rope_table(150, 64, device="cuda")
+    w = torch.ones(64, device="cuda")
+
+    def run(q, k, v, n):
+        a, b = qk_norm_rope(q, k, cos, sin, w, w)
+        return window_attention(a, b, v, window=40, sinks=2, lengths=n)
+    n = torch.tensor([150, 77], dtype=torch.int32, device="cuda")
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    out = run(*leaves, n)
+    first = torch.autograd.grad(out, leaves, go, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(out, leaves, go)))
+    with torch.inference_mode():
+        assert torch.equal(run(q, k, v, n), out)
+    for change in (lambda: n.add_(1), lambda: mid.add_(1)):
+        mid = leaves[2] * 1
+        out = run(leaves[0], leaves[1], mid, n)
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, leaves, go)
