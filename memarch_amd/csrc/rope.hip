@@ -6,6 +6,8 @@
 // lanes neighbouring pieces. In the half layout a lane's two pieces are the two sides of its rotation pairs, interleaved
 // pairs lie inside a piece; either way the norm's sum is the only value that crosses lanes. A group takes UNR heads of one
 // token at once: their loads are issued together, kept as loaded until each is used, and share the token's table entries.
+// Measured (32 x 1024 tokens of 16 + 16 heads of 128, bf16, norm): forward 96 us, 5.6 TB/s; backward 149 us, 5.4 TB/s, and 5 us
+// for the weights' gradients (a large copy reaches 4.9 TB/s).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
