@@ -128,8 +128,11 @@ __device__ __forceinline__ void mask_keys(f32x16& s, int row, int k0h, int windo
 // Measured (bf16, D = 128, 16 heads): 32768 tokens, every earlier one seen, 4.1 ms, 1.06 PFLOP/s; 4 x 16384 tokens, window
 // 1024, 0.74 ms, 0.72 PFLOP/s of visible pairs with the matrix core busy 41% of the time; 32 x 1024, window 512, 0.27 ms,
 // 23% busy: its workgroups are 2 to 11 tiles long and 1.4 of 2 waves per SIMD are there at a time.
+// With D <= 64 vector work is busy half the time and the matrix core a quarter, so waves are what fills the gaps: four per
+// SIMD, in 128 registers with the tile's offsets made again for each tile, take 96 us where three take 102 (8 texts of up to
+// 2999 tokens, 12 heads, fp16). At D = 128 the registers leave room for two.
 template <typename T, int DP>
-__global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
+__global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) {
   constexpr int IMG = BK * DP * 2;                     // bytes of a tile
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];   // K and V, two tiles each
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -138,8 +141,6 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
   const int qb = nq - 1 - pl.blk, b = pl.b, hk = pl.hk, hq = hk * a.grp + pl.g, bh = b * a.Hq + hq;
   const int len = seq_len(a, b);
   const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
-  const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
-  float* const lp = a.lse == nullptr ? nullptr : a.lse + (int64_t)bh * a.T + row;
   f32x16 acc[DP / 32] = {};
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * LOG2E;
@@ -173,6 +174,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
       const int img = (it & 1) * 2 * IMG;
       if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
       const int k0 = kt.key0(it);
+      if constexpr (DP == 64) ad.refresh();            // 128 registers: four waves per SIMD
       // whether the wave's rows see a key of the tile
       if (k0 <= r0 + 31 && (r0 - (k0 + BK - 1) < a.window || k0 < a.sinks)) {
         f32x16 s[2] = {};
@@ -233,11 +235,12 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_fwd(Args a) {
     }
   }
   l = sum_halves(l);
+  const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
   const bool in = row < a.T, see = row < len;
   const float inv = see ? 1.f / l : 0.f;
   store_acc<T, DP>(acc, inv, a.o + ofs, a.D, in, h);
   if (a.r != nullptr) store_acc<T, DP, true>(acc, inv, a.r + ofs, a.D, in, h);
-  if (lp != nullptr && in && h == 0) *lp = see ? m + __builtin_amdgcn_logf(l) / c : INFINITY;
+  if (a.lse != nullptr && in && h == 0) a.lse[(int64_t)bh * a.T + row] = see ? m + __builtin_amdgcn_logf(l) / c : INFINITY;
 }
 
 // --------------------------------------------------------------------------------------------------------------- dq
