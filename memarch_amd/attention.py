@@ -11,6 +11,7 @@ that is not on a GPU raises, and there is no other code path.
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -30,6 +31,14 @@ def _check_same(ref, *named):
             raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
     if not ref.is_cuda:
         raise ValueError("memarch_amd.attention runs on the GPU only; got a tensor on " + str(ref.device))
+
+
+def _check_tangents(*tensors):
+    """Refuses dual tensors: the kernels have no forward-mode derivative, and their fresh outputs would carry no tangent,
+    which forward mode takes for zero. Outside a dual level (the usual case) no tensor is looked at."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError("the attention operators have no forward-mode derivative; got a dual tensor")
 
 
 class _On:
@@ -155,7 +164,7 @@ def window_attention(q, k, v, window=None, sinks=0, lengths=None, scale=None):
     by none, their output and gradients are 0 and what lies in their rows is not read (inside a length, a NaN or an
     infinity may reach rows near it that do not see it, as 0 * NaN does in a dense form). scale defaults to D^-0.5.
     Under torch.autocast fp32 tensors are cast to its type, as for scaled_dot_product_attention. Differentiable once
-    in q, k and v."""
+    in q, k and v, in reverse mode: a tensor with a forward-mode tangent raises."""
     if torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         q, k, v = (t.to(dt) if t.dtype is torch.float32 else t for t in (q, k, v))
@@ -167,6 +176,7 @@ def window_attention(q, k, v, window=None, sinks=0, lengths=None, scale=None):
     scale = _scale(scale, q.shape[3])
     lengths = _lengths(lengths, q.shape[0], q.shape[1])
     _check_same(q, ("k", k), ("v", v), ("lengths", lengths))
+    _check_tangents(q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
     return _forward(q, k, v, lengths, window, sinks, scale, False)[3]
@@ -191,7 +201,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sink
     page block_table[b, j // page] (int32 [B, max_pages]) at slot j % page; lengths [B] (int32 or int64) counts a
     sequence's cached tokens with the new one, whose keys and values are in the cache already. The mask is that of
     window_attention's last row. A sequence of length 0 gives 0; tokens in pages outside the cache (entries of -1, say)
-    and past max_pages are not seen. The caches are read where they lie, 16 bytes at a time. No gradient."""
+    and past max_pages are not seen. The caches are read where they lie, 16 bytes at a time. No gradient; a tensor with a
+    forward-mode tangent raises."""
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError(f"q {tuple(q.shape)} must be [B, Hq, D], k_cache {tuple(k_cache.shape)} and v_cache "
                          f"{tuple(v_cache.shape)} [pages, page, Hkv, D]")
@@ -212,6 +223,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sink
         raise ValueError("lengths must be given")
     lengths = _lengths(lengths, B, _MAX_INT)
     _check_same(q, ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("lengths", lengths))
+    _check_tangents(q, k_cache, v_cache)
     max_pages = block_table.shape[1]
     if max_pages > 1 and block_table.stride(1) != 1 or B > 1 and block_table.stride(0) < max_pages:
         block_table = block_table.contiguous()

@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .attention import _check_same, _On
+from .attention import _check_same, _check_tangents, _On
 from .fused_ops import _ptr, _stream
 
 # element-type codes of include/mce_rope.h
@@ -101,7 +101,7 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, *, norm=True, eps
     rotated by the angles whose cosines and sines are the rows of cos, sin [P, R/2] (fp32, rope_table): pairs
     (i, i + R/2), or (2i, 2i + 1) with interleaved=True. Returns q and k, contiguous. The tables take no gradient. A token's row is its index in
     the text, or positions [T] or [B, T] (int32 or int64); a position outside the table gives NaN. Differentiable once
-    in q, k and the weights."""
+    in q, k and the weights, in reverse mode: a tensor with a forward-mode tangent raises."""
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must be [B, T, Hq, D] and [B, T, Hkv, D]")
     B, T, Hq, D = q.shape
@@ -133,6 +133,7 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, *, norm=True, eps
             raise ValueError(f"positions {tuple(positions.shape)} must be [T] or [B, T] with B={B}, T={T}")
     _check_same(q, ("k", k), ("cos", cos), ("sin", sin), ("q_weight", q_weight), ("k_weight", k_weight),
                 ("positions", positions))
+    _check_tangents(q, k, cos, sin, q_weight, k_weight)
     if positions is not None:
         positions = positions.expand(B, T)
     cos, sin = cos.detach().contiguous(), sin.detach().contiguous()

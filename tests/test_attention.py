@@ -1,5 +1,6 @@
 """The attention operators without a GPU: the oracle pinned (oracle/attn_oracle.py), argument checks of the Python
 surface and the C ABI, the library's exports and what its kernels must not hold."""
+import contextlib
 import ctypes
 import inspect
 import os
@@ -9,6 +10,7 @@ import subprocess
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from memarch_amd import _lib, attention, rotary
 from oracle import attn_oracle as orc
@@ -223,6 +225,35 @@ def test_qk_norm_rope_refusals():
     with pytest.raises(ValueError):
         rotary.rope_table(4, 4, theta=0.0)
     assert rotary.rope_table(0, 4)[0].shape == (0, 2)
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A dual tensor among the inputs raises, whether or not one requires a gradient: no output loses a tangent. (The
+    launches are stubbed; outside a dual level the calls go through.)"""
+    launched = []
+    monkeypatch.setattr(_lib, "call", lambda *a: launched.append(a[0]))
+    for mod in (attention, rotary):
+        monkeypatch.setattr(mod, "_check_same", lambda *a: None)
+        monkeypatch.setattr(mod, "_stream", lambda dev: 0)
+        monkeypatch.setattr(mod, "_On", lambda dev: contextlib.nullcontext())
+    q, w, cos = _bf(1, 3, 2, 64, device="cpu"), torch.ones(64), torch.zeros(3, 32)
+    kc, table, lens = _bf(2, 8, 2, 64, device="cpu"), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    calls = [(attention.window_attention, (q, q, q), 3), (rotary.qk_norm_rope, (q, q, cos, cos, w, w), 6),
+             (attention.paged_attention, (q[0], kc, kc, table, lens), 3)]
+    for fn, args, n in calls:
+        fn(*args)
+        with fwAD.dual_level():
+            fn(*args)
+            count = len(launched)
+            for i in range(n):
+                for needs in (False, True):
+                    x = args[i].clone().requires_grad_(needs)
+                    dual = fwAD.make_dual(x, torch.ones_like(x))
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        fn(*args[:i], dual, *args[i + 1:])
+                    with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                        fn(*args[:i], dual, *args[i + 1:])
+            assert len(launched) == count
 
 
 # ------------------------------------------------------------------------------------------------------ the library
