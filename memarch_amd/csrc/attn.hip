@@ -237,9 +237,9 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) 
   l = sum_halves(l);
   const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
   const bool in = row < a.T, see = row < len;
-  const float inv = see ? 1.f / l : 0.f;
-  store_acc<T, DP>(acc, inv, a.o + ofs, a.D, in, h);
-  if (a.r != nullptr) store_acc<T, DP, true>(acc, inv, a.r + ofs, a.D, in, h);
+  const float inv = 1.f / l;
+  store_acc<T, DP>(acc, inv, a.o + ofs, a.D, in, see, h);
+  if (a.r != nullptr) store_acc<T, DP, true>(acc, inv, a.r + ofs, a.D, in, see, h);
   if (a.lse != nullptr && in && h == 0) a.lse[(int64_t)bh * a.T + row] = see ? m + __builtin_amdgcn_logf(l) / c : INFINITY;
 }
 
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
   const int ln = lane_now(), h = ln >> 5, row = r0 + (ln & 31);
   const int64_t ofs = ((int64_t)b * a.T + row) * a.Hq * a.D + (int64_t)hq * a.D;
   const bool in = row < a.T;
-  store_acc<T, DP>(acc, a.scale, a.dq + ofs, a.D, in, h);
+  store_acc<T, DP>(acc, a.scale, a.dq + ofs, a.D, in, row < len, h);
   if (in && h == 0) {
     // The output's probabilities were rounded, so delta is off by some of its rounding, and the sum of the row's ds, which
     // should be 0, by as much: what k_attn_dkv gets is put right by it (dk of 8 heads of 96, T = 1000: off by 1.42 times
@@ -580,15 +580,15 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
     }
   }
   const int ln = lane_now(), h = ln >> 5, key = j0 + (ln & 31);
-  const bool in = key < a.T;
+  const bool in = key < a.T, live = key < len;
   if (S == 1) {
     const int64_t ofs = (((int64_t)b * a.T + key) * a.Hkv + hk) * a.D;
-    store_acc<T, DP>(dk, a.scale, a.dk + ofs, a.D, in, h);
-    store_acc<T, DP>(dv, 1.f, a.dv + ofs, a.D, in, h);
+    store_acc<T, DP>(dk, a.scale, a.dk + ofs, a.D, in, live, h);
+    store_acc<T, DP>(dv, 1.f, a.dv + ofs, a.D, in, live, h);
   } else {
     float* const p = (sink ? a.part_s : a.part_r) + ((((int64_t)bh * nb + blk) * S + sp) * 2 * BKV + key - kb0) * a.D;
-    store_f32<DP>(dk, p, a.D, in, h);
-    store_f32<DP>(dv, p + BKV * a.D, a.D, in, h);
+    store_f32<DP>(dk, p, a.D, in, live, h);
+    store_f32<DP>(dv, p + BKV * a.D, a.D, in, live, h);
   }
 }
 

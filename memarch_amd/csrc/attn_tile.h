@@ -228,10 +228,13 @@ __device__ __forceinline__ float sum_halves(float x) {
 
 // Stores the accumulators acc[dt] (rows = columns 32 dt + ... of the result, accumulator column = its row l%32) scaled
 // by f: row `row` of p, DP/32 x 16 bytes x 2 per lane. The halves exchange 4 columns of every 16, so that each lane
-// stores 16 bytes. Only rows with ok and columns below d are written. RES: the values stored are what the rounding of
-// the same call without RES leaves over, rounded in their turn.
+// stores 16 bytes. Only rows with ok and columns below d are written, those that are not live as zeros (whatever acc
+// holds: 0 * NaN is no 0). RES: the values stored are what the rounding of the same call without RES leaves over, rounded
+// in their turn.
 template <typename T, int DP, bool RES = false>
-__device__ __forceinline__ void store_acc(const f32x16 (&acc)[DP / 32], float f, uint16_t* p, int d, bool ok, int h) {
+__device__ __forceinline__ void store_acc(const f32x16 (&acc)[DP / 32], float f, uint16_t* p, int d, bool ok, bool live,
+                                          int h) {
+  const uint32_t keep = live ? 0xFFFFFFFFu : 0u;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -241,7 +244,7 @@ __device__ __forceinline__ void store_acc(const f32x16 (&acc)[DP / 32], float f,
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = acc[dt][8 * s + 2 * e] * f, y = acc[dt][8 * s + 2 * e + 1] * f;
-        w[e] = RES ? pack2<T>(x - (float)(T)x, y - (float)(T)y) : pack2<T>(x, y);
+        w[e] = (RES ? pack2<T>(x - (float)(T)x, y - (float)(T)y) : pack2<T>(x, y)) & keep;
       }
       // swap(w[2], w[0])'s halves: low lanes end with columns 16 s + 0..7, high lanes with 16 s + 8..15
       const auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
@@ -258,7 +261,7 @@ __device__ __forceinline__ void store_acc(const f32x16 (&acc)[DP / 32], float f,
 
 // The same as fp32, unscaled: 16 bytes per lane and group of 4 columns.
 template <int DP>
-__device__ __forceinline__ void store_f32(const f32x16 (&acc)[DP / 32], float* p, int d, bool ok, int h) {
+__device__ __forceinline__ void store_f32(const f32x16 (&acc)[DP / 32], float* p, int d, bool ok, bool live, int h) {
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -266,7 +269,7 @@ __device__ __forceinline__ void store_f32(const f32x16 (&acc)[DP / 32], float* p
       const int col = 32 * dt + 8 * e4 + 4 * h;
       f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = acc[dt][4 * e4 + e];
+      for (int e = 0; e < 4; ++e) x[e] = live ? acc[dt][4 * e4 + e] : 0.f;
       if (ok && col < d) *reinterpret_cast<f32x4*>(p + col) = x;
     }
 }

@@ -74,6 +74,20 @@ def test_padded_batches(lens, window, sinks):
         assert all(not x[i, max(n, 0):].any() for x in got)
 
 
+@pytest.mark.parametrize("t,n,hq,hkv,d,window,sinks", [(150, 70, 4, 2, 64, 0, 0), (150, 97, 2, 1, 128, 20, 3),
+                                                       (2300, 2100, 4, 1, 64, 0, 0)])
+@pytest.mark.parametrize("bad", ["q", "k", "v", "go"])
+def test_padded_rows_stay_zero_beside_a_nan(bad, t, n, hq, hkv, d, window, sinks):
+    """What lies in a sequence's last rows, NaN among it, does not reach the rows behind its length: outputs and gradients
+    there are 0. (The third shape shares its key blocks among workgroups, so parts are joined.)"""
+    x = dict(zip(("q", "k", "v", "go"), _inputs(1, t, hq, hkv, d, BF, seed=n)))
+    x[bad][0, n - 3, 0], x[bad][0, n - 1, 0, 1] = float("nan"), float("inf")
+    got = _step(*(x[i].cuda() for i in ("q", "k", "v", "go")), window, sinks, torch.tensor([n], device="cuda"))
+    for name, y in zip(("out", "dq", "dk", "dv"), got):
+        assert not y[0, n:].any(), name
+    assert torch.isfinite(got[0][0, :n - 64]).all()
+
+
 @pytest.mark.parametrize("b,t,hq,hkv,d,window,sinks", [
     (1, 2300, 4, 1, 64, 0, 0),         # every earlier key: rows of a key block shared by several workgroups
     (1, 2300, 4, 1, 128, 1000, 4),     # a window long enough for that, and the block with the first tokens apart
