@@ -429,6 +429,8 @@ int group_of(int64_t D, int64_t R, int64_t n, bool interleaved) {
 
 // Workgroups of the backward's two sides: in proportion to their heads, at most MAX_BLOCKS (4 per CU) together.
 constexpr int64_t MAX_BLOCKS = 1024;
+// Workgroups of one side of the forward, at most.
+constexpr int64_t MAX_BLOCKS_F = int64_t(1) << 22;
 void bwd_blocks(int64_t tokens, int64_t Hq, int64_t Hkv, int64_t& nq, int64_t& nk) {
   const int64_t per = 16;   // head vectors below which another workgroup does not pay
   nq = (tokens * Hq + per - 1) / per;
@@ -470,17 +472,17 @@ void launch(Args& a, bool pieces, int64_t nq, int64_t nk, hipStream_t st) {
       hipLaunchKernelGGL((k_rope<T, NORM, IL, BWD, UNR_B>), dim3((unsigned)(nq + nk)), dim3(THREADS), 0, st, a);
     else
       hipLaunchKernelGGL((k_rope_any<T, NORM, IL, BWD>), dim3((unsigned)(nq + nk)), dim3(THREADS), 0, st, a);
-  } else if (!pieces) {
-    auto blocks = [&](int H) { return (uint32_t)(((int64_t)a.tokens * H + THREADS / 64 - 1) / (THREADS / 64)); };
-    a.blocks_q = blocks(a.side[0].H);
-    hipLaunchKernelGGL((k_rope_any<T, NORM, IL, BWD>), dim3(a.blocks_q + blocks(a.side[1].H)), dim3(THREADS), 0, st, a);
   } else {
-    auto blocks = [&](int H) {
-      return (uint32_t)(((int64_t)a.tokens * ((H + UNR_F - 1) / UNR_F) * a.G + THREADS - 1) / THREADS);
+    // lanes per head vector or per UNR_F of them; a launch holds fewer than 2^32 threads, the kernels stride over the rest
+    auto blocks = [&](int64_t H) {
+      const int64_t threads = pieces ? a.tokens * ((H + UNR_F - 1) / UNR_F) * a.G : a.tokens * H * 64;
+      const int64_t n = (threads + THREADS - 1) / THREADS;
+      return (uint32_t)(n < MAX_BLOCKS_F ? n : MAX_BLOCKS_F);
     };
     a.blocks_q = blocks(a.side[0].H);
-    hipLaunchKernelGGL((k_rope<T, NORM, IL, BWD, UNR_F>), dim3(a.blocks_q + blocks(a.side[1].H)), dim3(THREADS), 0, st,
-                       a);
+    const dim3 grid(a.blocks_q + blocks(a.side[1].H));
+    if (pieces) hipLaunchKernelGGL((k_rope<T, NORM, IL, BWD, UNR_F>), grid, dim3(THREADS), 0, st, a);
+    else hipLaunchKernelGGL((k_rope_any<T, NORM, IL, BWD>), grid, dim3(THREADS), 0, st, a);
   }
 }
 

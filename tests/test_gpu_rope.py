@@ -210,3 +210,19 @@ def test_graph_sync_and_repeats():
         ref, again = step(*vals[i]), step(*vals[i])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) and torch.equal(b, c) for a, b, c in zip(got, ref, again)), i
+
+
+def test_more_heads_than_one_launch_has_waves():
+    """2^26 head vectors element by element: one wave each would be more threads than a launch can hold. Each part of the
+    text alone gives the same bits."""
+    from memarch_amd.rotary import qk_norm_rope, rope_table
+    t, hq, parts = 1 << 22, 16, 8
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k = (torch.randn(1, t, h, 2, generator=gen, device="cuda").bfloat16() for h in (hq, 1))
+    cos, sin = rope_table(1000, 2, device="cuda")
+    pos = torch.arange(t, device="cuda") % 1000
+    got = qk_norm_rope(q, k, cos, sin, positions=pos)
+    for i in range(parts):
+        s = slice(i * t // parts, (i + 1) * t // parts)
+        for a, b in zip(got, qk_norm_rope(q[:, s], k[:, s], cos, sin, positions=pos[s])):
+            assert torch.equal(a[:, s], b), i
