@@ -21,7 +21,8 @@
  *
  * Buffers: q [B, T, Hq, D], k and v [B, T, Hkv, D], go like q: element strides (batch, token, head) are given, the last
  * dimension is contiguous; 16-byte aligned, strides multiples of 8, the token stride at least D. D is a multiple of 8 up to 128. out, dq
- * [B, T, Hq, D] and dk, dv [B, T, Hkv, D] are contiguous. lse is [B, Hq, T] fp32. Every call is asynchronous on
+ * [B, T, Hq, D] and dk, dv [B, T, Hkv, D] are contiguous. lse is [B, Hq, T] fp32. B Hq ceil(T / 128) is below 2^24 (what
+ * one launch can hold). Every call is asynchronous on
  * `stream`, allocates nothing, and returns 0 or an MCE_ATTN_E* code; arguments are checked before anything is launched.
  */
 #ifndef MCE_ATTN_H

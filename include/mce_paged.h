@@ -13,7 +13,7 @@
  *
  * Buffers: q [B, Hq, D] with element strides (batch, head); caches [pages, page, Hkv, D] with element strides (page,
  * slot, head), last dimensions contiguous, 16-byte aligned, strides multiples of 8; out contiguous [B, Hq, D]. D is a
- * multiple of 8 up to 128, page a multiple of 8. Every call is asynchronous on `stream`, allocates nothing, and returns
+ * multiple of 8 up to 128, page a multiple of 8; B Hq is at most 2^24, and B Hkv ceil(Hq / Hkv / 32) below it. Every call is asynchronous on `stream`, allocates nothing, and returns
  * 0 or an MCE_ATTN_E* code of mce_attn.h; arguments are checked before anything is launched.
  */
 #ifndef MCE_PAGED_H

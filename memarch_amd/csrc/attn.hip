@@ -624,9 +624,8 @@ int check_sizes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_
   if (B < 0 || T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || D > 128 || D % 8 || window < 0 || sinks < 0)
     return MCE_ATTN_EINVAL;
   if (T > (int64_t(1) << 27) || Hq * D > MAX_ST) return MCE_ATTN_EINVAL;
-  // one workgroup per 128 rows of every head
-  if (T > 0 && (B > (int64_t(1) << 31) / Hq || B * Hq * ((T + 127) / 128) >= (int64_t(1) << 31)))
-    return MCE_ATTN_EINVAL;
+  // one workgroup per 128 rows of every head (the backward's own are counted by its plan)
+  if (T > 0 && B > MAX_GROUPS / Hq / ((T + BQ - 1) / BQ)) return MCE_ATTN_EINVAL;
   return MCE_ATTN_OK;
 }
 
@@ -794,6 +793,8 @@ int mce_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const 
   a.res = static_cast<const uint16_t*>(res);
   a.lse = const_cast<float*>(lse);
   const Plan p = make_plan(B, T, Hq, Hkv, D, window, sinks);
+  const int64_t nr = (T + BKV - 1) / BKV - p.n_sb;
+  if (B * Hkv * ((int64_t)p.n_sb * p.S_s + nr * p.S_r) > MAX_GROUPS) return MCE_ATTN_EINVAL;
   a.n_sb = p.n_sb;
   a.S_s = p.S_s;
   a.S_r = p.S_r;

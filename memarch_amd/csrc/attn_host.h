@@ -14,6 +14,9 @@ namespace attn {
 // Token strides up to 2^21 elements keep every offset inside a tile of at most 128 rows in 31 bits.
 constexpr int64_t MAX_ST = int64_t(1) << 21;
 
+// Workgroups of up to 256 threads that a launch can hold: HIP takes fewer than 2^32 threads.
+constexpr int64_t MAX_GROUPS = (int64_t(1) << 24) - 1;
+
 inline int finish() {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {

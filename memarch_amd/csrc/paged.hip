@@ -297,6 +297,7 @@ int check_paged(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page, int
   if (B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || D > 128 || D % 8 || page < 8 || page % 8 || page > 65536 ||
       max_pages < 0 || window < 0 || sinks < 0 || Hq > 65536 || B > (int64_t(1) << 24) || B * Hq > (int64_t(1) << 24))
     return MCE_ATTN_EINVAL;
+  if (B * Hkv * ((Hq / Hkv + HC - 1) / HC) > MAX_GROUPS) return MCE_ATTN_EINVAL;
   // key numbers in 30 bits, and exact division of an 8-row group's number by page / 8 through a 32-bit product
   if (max_pages > (int64_t(1) << 30) / page || max_pages * page > (int64_t(1) << 38) / page) return MCE_ATTN_EINVAL;
   return MCE_ATTN_OK;

@@ -343,6 +343,35 @@ def test_paged_c_abi_checks_need_no_gpu(lib):
     assert call(most=4096) == 3 and call(most=4096, ws=p, nb=need - 1) == 3 and call(most=4096, ws=p + 16, nb=need) == 3
 
 
+def test_sizes_that_no_launch_can_hold_are_refused(lib):
+    """2^24 workgroups of 256 threads are 2^32 threads, one more than a launch takes: refused as arguments, not found out by
+    the launch. (Calls below that pass the checks: without a workspace or a sound address they end there.)"""
+    buf = ctypes.create_string_buffer(1 << 12)
+    p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 256
+    x = lambda q: (q, 64, 64, 64)
+
+    def fwd(B, T, Hq):
+        return lib.mce_attn_fwd(*x(p + 2), *x(p), *x(p), None, B, T, Hq, 1, 64, 0, 0, 0.1, 1, p, None, None, None)
+
+    def bwd(B, T, Hq):
+        return lib.mce_attn_bwd(*x(p), *x(p), *x(p), *x(p), None, B, T, Hq, 1, 64, 0, 0, 0.1, 1, p, p, p, p, p, p, None, 0,
+                                None)
+
+    for b, t, h in ((1 << 24, 1, 1), (1 << 20, 1, 16), (1 << 16, 129, 128), (1 << 27, 1, 1), (1 << 23, 129, 1)):
+        assert fwd(b, t, h) == 1 and bwd(b, t, h) == 1 and lib.mce_attn_bwd_ws_bytes(b, t, h, 1, 64, 0, 0) == 0, (b, t, h)
+    for b, t, h in (((1 << 24) - 1, 1, 1), ((1 << 24) - 1, 128, 1), ((1 << 20) - 1, 128, 16), ((1 << 16) - 1, 129, 128)):
+        assert fwd(b, t, h) == 2 and bwd(b, t, h) == 3, (b, t, h)
+
+    def paged(B, Hq, Hkv):
+        return lib.mce_paged(p + 2, 64, 64, p, 4096, 64, 64, p, 4096, 64, 64, p, 1, p, B, Hq, Hkv, 64, 1, 16, 1, 0, 0, 0.1,
+                             1, p, None, 0, None)
+
+    for b, hq, hkv in ((1 << 24, 1, 1), (1 << 20, 16, 16), (1 << 8, 65536, 65536)):
+        assert paged(b, hq, hkv) == 1 and lib.mce_paged_ws_bytes(b, hq, hkv, 64, 16, 1, 0, 0) == 0, (b, hq, hkv)
+    for b, hq, hkv in (((1 << 24) - 1, 1, 1), (1 << 20, 16, 8), (1 << 8, 65536, 16)):
+        assert paged(b, hq, hkv) == 2, (b, hq, hkv)
+
+
 def test_rope_c_abi_checks_need_no_gpu(lib):
     buf = ctypes.create_string_buffer(1 << 12)
     p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 256
