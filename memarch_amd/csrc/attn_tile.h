@@ -87,25 +87,20 @@ __device__ __forceinline__ u32x4 load16(const i32x4& rsrc, int voff) {
   return __builtin_bit_cast(u32x4, attn_buffer_load16(rsrc, voff, 0, 0));
 }
 
-// 16 bytes per lane from a resource straight into LDS at lds + dst + 16 * lane. Written as an instruction of its own
-// because the compiler waits for every pending load of a kind it knows before each transposing LDS read; the kernels
-// order these loads themselves (wait_vmcnt, then a barrier, before the tile's first read), and nothing else in them
-// uses M0.
+// 16 bytes per lane from a resource straight into LDS at lds + dst + 16 * lane (M0, which the compiler sets). Written as an
+// instruction of its own because the compiler waits for every pending load of a kind it knows before each transposing LDS
+// read; the kernels order these loads themselves (wait_vmcnt, then a barrier, before the tile's first read). A vector memory
+// instruction may read a scalar register only five states after a vector instruction (readfirstlane) has written it, and the
+// compiler does not look for that inside an asm block: the block waits them itself, whatever stands in front.
 __device__ __forceinline__ void dma16(const i32x4& rsrc, const char* lds, int dst, int voff) {
   const uint32_t a = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(LDS_AS const char*)lds + (uint32_t)dst);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(a), "v"(voff), "s"(rsrc)
-               : "memory");
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "{m0}"(a), "v"(voff), "s"(rsrc) : "memory");
 }
 
 // The same with 4 bytes per lane, at lds + dst + 4 * lane.
 __device__ __forceinline__ void dma4(const i32x4& rsrc, const char* lds, int dst, int voff) {
   const uint32_t a = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(LDS_AS const char*)lds + (uint32_t)dst);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :
-               : "s"(a), "v"(voff), "s"(rsrc)
-               : "memory");
+  asm volatile("s_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "{m0}"(a), "v"(voff), "s"(rsrc) : "memory");
 }
 
 // The swizzle: 8 consecutive rows at one chunk fall on the 8 different 16-byte bank groups of 128 bytes and 16 on the

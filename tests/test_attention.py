@@ -277,6 +277,40 @@ def test_exports_every_declared_symbol(lib):
         assert lib.mce_attn_error_string(code)
 
 
+def _kernels(tmp_path):
+    """{kernel: its instructions} of the built library."""
+    if not os.path.exists(OBJDUMP):
+        pytest.skip("no llvm-objdump")
+    shutil.copy(_lib.ATTN_LIB_PATH, tmp_path / "lib.so")
+    subprocess.run([OBJDUMP, "--offloading", "lib.so"], cwd=tmp_path, check=True, capture_output=True)
+    out, name = {}, None
+    for f in sorted(f for f in os.listdir(tmp_path) if f.endswith("gfx950")):
+        for line in subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", f], cwd=tmp_path, check=True, capture_output=True,
+                                   text=True).stdout.splitlines():
+            m = re.match(r"[0-9a-f]+ <(\w+)>:", line)
+            if m:
+                name = m[1]
+                out[name] = []
+            elif name and line.startswith("\t"):
+                out[name].append(line.split("//")[0].strip())
+    return out
+
+
+def test_loads_into_lds_wait_for_their_scalar_operands(lib, tmp_path):
+    """Each load into LDS stands behind five wait states of its own (a scalar register that a vector instruction has just
+    written may not be read earlier), and behind a write of M0 that the compiler knows of."""
+    loads = 0
+    for name, ins in _kernels(tmp_path).items():
+        for i, x in enumerate(ins):
+            if x.startswith("buffer_load") and x.endswith(" lds"):
+                loads += 1
+                m = re.fullmatch(r"s_nop (\d+)", ins[i - 1])
+                assert m and int(m[1]) >= 4, (name, ins[i - 2:i + 1])
+                back = next(y for y in ins[i - 1::-1] if re.match(r"\w+ m0,|s_c?branch|buffer_load.* lds$", y))
+                assert " m0," in back, (name, back)
+    assert loads > 100
+
+
 def test_kernels_hold_no_l2_writeback_and_no_packed_fp32(lib, tmp_path):
     """No device-scope release (buffer_wbl2), no scratch memory spills in the attention kernels' inner loops to speak of,
     and none of the packed fp32 operations that the build switches off."""
