@@ -139,10 +139,12 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 2 : 1) void k_paged(Args a) {
     return good;
   };
   int good = 0;
-  if (t0 + wave < t1) {
-    look_up(t0 + wave);
-    good = issue(t0 + wave, 0);
-  }
+  const bool work = t0 + wave < t1;
+  if (work) look_up(t0 + wave);
+  // The query fragments are here before the first tile's loads go out: a wait for them that the compiler put among the
+  // loop's products would be a wait for the next tile too, as loads return in order.
+  wait_vmcnt<0>();
+  if (work) good = issue(t0 + wave, 0);
   for (int it = t0 + wave, i = 0; it < t1; it += NW, ++i) {
     int next = 0;
     if (it + NW < t1) {

@@ -311,6 +311,25 @@ def test_loads_into_lds_wait_for_their_scalar_operands(lib, tmp_path):
     assert loads > 100
 
 
+@pytest.mark.parametrize("kernel,most", [("k_paged", {"Li64": {8}, "Li128": {16}})])
+def test_loops_wait_for_their_own_tile_only(lib, tmp_path, kernel, most):
+    """Loads return in order, so a wait for an operand from before the loop, put among the loop's products, would be a wait
+    for every tile under way. Behind the first load into LDS only the kernel's own waits are left: for the tile at hand (so
+    many later loads stay under way) and for all, where no product follows."""
+    found = 0
+    for name, ins in _kernels(tmp_path).items():
+        if kernel + "I" not in name:
+            continue
+        found += 1
+        first = next(i for i, x in enumerate(ins) if x.endswith(" lds"))
+        allowed = {0} | next(v for k, v in most.items() if k + "E" in name)
+        for i, x in enumerate(ins[first:], first):
+            m = re.match(r"s_waitcnt vmcnt\((\d+)\)", x)
+            if m:
+                assert int(m[1]) in allowed and not ins[i + 1].startswith("v_mfma"), (name, ins[i - 1:i + 2])
+    assert found == 4
+
+
 def test_kernels_hold_no_l2_writeback_and_no_packed_fp32(lib, tmp_path):
     """No device-scope release (buffer_wbl2), no scratch memory spills in the attention kernels' inner loops to speak of,
     and none of the packed fp32 operations that the build switches off."""
