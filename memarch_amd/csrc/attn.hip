@@ -487,6 +487,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
       kf[ks] = load16(kr, col < a.D ? r * (int)a.k.st * 2 + col * 2 : OOB);
       vf[ks] = load16(vr, col < a.D ? r * (int)a.v.st * 2 + col * 2 : OOB);
     }
+    // The key and value fragments are here before the loop: a wait for them that the compiler put among its products would
+    // be a wait for the tile just asked for too, as loads return in order.
+    wait_vmcnt<0>();
     for (int it = it0; it < it1; ++it) {
       const int buf = (it - it0) & (NS - 1), img = buf * 2 * IMG;
       // this wave's loads of tile `it` have arrived when only those of the later ones are under way; behind the barrier

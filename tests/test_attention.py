@@ -311,7 +311,8 @@ def test_loads_into_lds_wait_for_their_scalar_operands(lib, tmp_path):
     assert loads > 100
 
 
-@pytest.mark.parametrize("kernel,most", [("k_paged", {"Li64": {8}, "Li128": {16}})])
+@pytest.mark.parametrize("kernel,most", [("k_paged", {"Li64": {8}, "Li128": {16}}),
+                                         ("k_attn_dkv", {"Li64": {3, 6}, "Li128": {5, 10}})])
 def test_loops_wait_for_their_own_tile_only(lib, tmp_path, kernel, most):
     """Loads return in order, so a wait for an operand from before the loop, put among the loop's products, would be a wait
     for every tile under way. Behind the first load into LDS only the kernel's own waits are left: for the tile at hand (so
