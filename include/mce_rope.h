@@ -13,7 +13,7 @@
  * (weights NULL, both: 1). All arithmetic is fp32, results are rounded once to the element type of q and k; weights, tables and dw are fp32.
  *
  * The position of token t of sequence b is positions[b * pos_sb + t * pos_st] (int64 with pos_i64 != 0, else int32), or
- * t with positions NULL. A position outside [0, P) gives NaN in that token's heads (and in their gradients).
+ * t with positions NULL. A position outside [0, P) gives NaN in that token's heads, in their gradients and in all of dw.
  *
  * Buffers: q [B, T, Hq, D] and k [B, T, Hkv, D] with element strides (batch, token, head) and a contiguous last
  * dimension, gradients g like them; cos and sin [P, R/2] contiguous; outputs contiguous. Any alignment and any even

@@ -267,6 +267,10 @@ __global__ __launch_bounds__(THREADS, 4) void k_rope(Args a) {
       }
       // (a lane in which only one or none of its pieces turns has the identity in the other's place; half layout: both)
       if (ln.turn0) rotate<N, IL>(u, v, c, s);
+      if (row < 0) {   // NaN in the head, and through it in its gradient and the weights'
+#pragma unroll
+        for (int e = 0; e < N; ++e) u[e] = v[e] = __builtin_nanf("");
+      }
       if constexpr (NORM && BWD) {   // u, v: dn; heads past the last have zeros
         float dot = 0.f;
 #pragma unroll
@@ -283,11 +287,6 @@ __global__ __launch_bounds__(THREADS, 4) void k_rope(Args a) {
           u[e] = r * (u[e] - x0[e] * dot);
           v[e] = r * (v[e] - x1[e] * dot);
         }
-      }
-      if (row < 0) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) u[e] = v[e] = __builtin_nanf("");
-        if constexpr (NORM && BWD) dw0[0] = __builtin_nanf("");   // one NaN is enough to show
       }
       if (h0 + j < (uint32_t)sd.H) {
         if (ln.on0) store_piece(yp + (int64_t)(h0 + j) * a.D + ln.c0, P::pack(u));

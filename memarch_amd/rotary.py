@@ -99,9 +99,10 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, *, norm=True, eps
     """Each head vector of q [B, T, Hq, D] and k [B, T, Hkv, D] (fp32, bf16 or fp16, any strides) divided by its root
     mean square and multiplied by q_weight / k_weight [D] (None: 1; norm=False: neither), then its first R elements
     rotated by the angles whose cosines and sines are the rows of cos, sin [P, R/2] (fp32, rope_table): pairs
-    (i, i + R/2), or (2i, 2i + 1) with interleaved=True. Returns q and k, contiguous. The tables take no gradient. A token's row is its index in
-    the text, or positions [T] or [B, T] (int32 or int64); a position outside the table gives NaN. Differentiable once
-    in q, k and the weights, in reverse mode: a tensor with a forward-mode tangent raises."""
+    (i, i + R/2), or (2i, 2i + 1) with interleaved=True. Returns q and k, contiguous. The tables take no gradient. A
+    token's row is its index in the text, or positions [T] or [B, T] (int32 or int64); a position outside the table gives
+    NaN (in the weights' gradients as a whole). Differentiable once in q, k and the weights, in reverse mode: a tensor with
+    a forward-mode tangent raises."""
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must be [B, T, Hq, D] and [B, T, Hkv, D]")
     B, T, Hq, D = q.shape

@@ -122,6 +122,22 @@ def test_positions_outside_the_table_give_nan():
         assert torch.isfinite(dq[:, [0, 3]]).all() and dq[:, [1, 2]].isnan().all()
 
 
+@pytest.mark.parametrize("il", [False, True], ids=["half", "pairs"])
+@pytest.mark.parametrize("d,rot", [(64, 64), (128, 32), (66, 10)])
+def test_positions_outside_the_table_give_nan_weight_gradients(d, rot, il):
+    """One such token, and no column of the weights' gradients passes for a finite one; the other tokens' are as ever."""
+    from memarch_amd.rotary import qk_norm_rope
+    q, k, cos, sin, qw, kw, gq, gk = (t.cuda() for t in _inputs(1, 40, 2, 1, d, rot, torch.float32, rows=40))
+    pos = torch.arange(40, device="cuda")
+    pos[17] = 40
+    ls = [t.requires_grad_() for t in (q, k, qw, kw)]
+    grads = torch.autograd.grad(qk_norm_rope(q, k, cos, sin, qw, kw, positions=pos, interleaved=il), ls, (gq, gk))
+    assert grads[2].isnan().all() and grads[3].isnan().all()
+    good = torch.autograd.grad(qk_norm_rope(q, k, cos, sin, qw, kw, interleaved=il), ls, (gq, gk))
+    rest = pos < 40
+    assert all(torch.equal(a[:, rest], b[:, rest]) for a, b in zip(grads[:2], good[:2]))
+
+
 def test_strided_operands():
     """Slices of one packed projection, head-first layouts, strided last dimensions, unaligned bases, broadcast heads and
     expanded upstream gradients."""
