@@ -60,6 +60,19 @@ def test_parity(dt, b, t, hq, hkv, d, window, sinks):
     _check(*_inputs(b, t, hq, hkv, d, dt, seed=t), window, sinks)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,t,hq,hkv,window,sinks", [
+    (4, 300, 4, 2, 0, 0), (8, 190, 1, 1, 50, 3), (2, 333, 16, 8, 100, 130),   # whole heads per XCD: B Hkv = 8, 8, 16
+    (1, 520, 8, 8, 0, 0), (1, 260, 16, 8, 20, 0),
+    (2, 310, 8, 2, 0, 0), (1, 400, 8, 1, 70, 2), (3, 200, 8, 1, 0, 0)])       # B Hq = 16, 8, 24, B Hkv no multiple of 8
+def test_heads_placed_by_xcd(d, b, t, hq, hkv, window, sinks):
+    """Batches whose heads are a multiple of the 8 XCDs, with several blocks of rows and keys: every workgroup finds its
+    own."""
+    print(f"attn xcd {b} {t} {hq} {hkv} {d} {window} {sinks}", flush=True)
+    lens = None if b == 1 else torch.tensor([t - 37 * i for i in range(b)]).clamp(min=0)
+    _check(*_inputs(b, t, hq, hkv, d, BF, seed=t + d), window, sinks, lens)
+
+
 @pytest.mark.parametrize("lens", [[0, 0, 0], [1, 0, 150], [150, 64, 65], [127, 128, 129], [200, -3, 3]])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (40, 2)])
 def test_padded_batches(lens, window, sinks):
@@ -97,6 +110,18 @@ def test_shared_key_blocks(b, t, hq, hkv, d, window, sinks):
     print(f"attn shared {b} {t} {window} {sinks}", flush=True)
     lens = None if b == 1 else torch.tensor([t, 700])
     _check(*_inputs(b, t, hq, hkv, d, BF, seed=t + d), window, sinks, lens)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,t,hq,hkv,window,sinks", [(8, 1100, 4, 1, 0, 0), (4, 1200, 4, 2, 60, 140)])
+def test_shared_key_blocks_placed_by_xcd(d, b, t, hq, hkv, window, sinks):
+    """B Hkv = 8 and key blocks with several workgroups each (the first tokens', or all without a window)."""
+    from memarch_amd import _lib
+    need = _lib.load_attn().mce_attn_bwd_ws_bytes(b, t, hq, hkv, d, window, sinks)
+    assert need > b * hq * t * 8 + 4 * 128 * d * 4                            # parts there are
+    print(f"attn xcd shared {b} {t} {d} {window} {sinks}", flush=True)
+    lens = torch.tensor([t - 100 * i for i in range(b)])
+    _check(*_inputs(b, t, hq, hkv, d, HF, seed=t + d), window, sinks, lens)
 
 
 def test_window_as_long_as_the_text_and_longer():

@@ -48,6 +48,22 @@ def test_parity(dt, hq, hkv, d, page, most, lens):
     _check(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32))
 
 
+@pytest.mark.parametrize("hq,hkv,d,page,most,lens,window,sinks", [
+    (4, 1, 128, 64, 700, [44800], 0, 0),                 # 175 parts
+    (2, 1, 64, 16, 2500, [39999], 30000, 20),            # 118 parts of a window, the first tokens in the first of them
+    (1, 1, 8, 128, 3080, [393216], 0, 0),                # 1024 parts, the most
+    (2, 2, 64, 64, 700, [44800, 20000], 0, 0)])          # 175 parts a sequence at most, the second has fewer
+def test_many_parts(hq, hkv, d, page, most, lens, window, sinks):
+    """Few heads and long caches: more parts than the joining wave has lanes."""
+    from memarch_amd import _lib
+    b = len(lens)
+    need = _lib.load_attn().mce_paged_ws_bytes(b, hq, hkv, d, page, most, window, sinks)
+    assert need >= 65 * b * hq * (d + 2) * 4
+    print(f"paged parts {hq} {hkv} {d} {lens} {window}", flush=True)
+    q, kc, vc, table = _case(b, most, hq, hkv, d, page, BF, seed=most)
+    _check(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32), window, sinks)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (31, 0), (32, 1), (33, 7), (100, 64), (1000, 4), (100, 1000)])
 def test_windows(window, sinks):
     q, kc, vc, table = _case(4, 30, 4, 2, 64, 16, BF, seed=window)
