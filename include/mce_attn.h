@@ -17,7 +17,9 @@
  *   that share them)
  * Products take 16-bit operands and sum in fp32; softmax statistics are fp32; p and ds are rounded to the element type
  * as operands of the second products (half of dq's products take what the rounding of ds leaves over as well), results
- * are rounded once. In fp16, p (go v - d) has to stay in range, as the results have to.
+ * are rounded once. In fp16, p (go v - d) has to stay in range, as the results have to. Scores may have any finite size for
+ * out; the backward forms p from lse, an fp32 number of the scores' size, so that scores of S put p off by about S 2^-22 of
+ * itself: gradients ask for scores below 2^20 or so, and from 2^27 on they may not be finite.
  *
  * Buffers: q [B, T, Hq, D], k and v [B, T, Hkv, D], go like q: element strides (batch, token, head) are given, the last
  * dimension is contiguous; 16-byte aligned, strides multiples of 8, the token stride at least D. D is a multiple of 8 up to 128. out, dq

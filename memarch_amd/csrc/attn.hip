@@ -143,6 +143,7 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) 
   const int q0 = qb * BQ, r0 = q0 + wave * 32, row = r0 + (lane & 31);
   f32x16 acc[DP / 32] = {};
   float m = -INFINITY, l = 0.f;
+  bool large = false;   // some row's m is beyond LARGE
   const float c = a.scale * LOG2E;
   if (q0 < len) {
     const int q1 = (q0 + BQ < len ? q0 + BQ : len) - 1;
@@ -211,11 +212,20 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) 
         if (__builtin_amdgcn_ballot_w64((mx - m) * c > LAZY) != 0) {
           const float al = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mx) * c);
           m = mx;
+          large = __builtin_amdgcn_ballot_w64(fabsf(m * c) > LARGE && m != -INFINITY) != 0;
           l *= al;
 #pragma unroll
           for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= al;
         }
-        const float mc = (m == -INFINITY ? 0.f : m) * c;   // a row that has seen nothing yet
+        const float mu = m == -INFINITY ? 0.f : m;   // (a row that has seen nothing yet)
+        float mc = mu * c;
+        if (large) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kb][e] -= mu;
+          mc = 0.f;
+        }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll

@@ -35,6 +35,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+// Where a maximum's product m c (c = scale log2 e) is larger, the scores have m taken off before they are multiplied by c:
+// s c - m c would carry the rounding of m c, which makes the exponential of the maximum itself 0 or infinite from about 2^30
+// on. The difference is exact next to m; below the limit (a rounding of 2^-7 at most) one instruction does both.
+constexpr float LARGE = 131072.f;
 constexpr int OOB = 0x7FFFFFFF;          // a byte offset past every resource's records
 constexpr int BUF_DWORD3 = 0x00020000;   // gfx9 buffer resource word 3 (raw, 32-bit data format)
 

@@ -170,11 +170,17 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 2 : 1) void k_paged(Args a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[e]);
     mx = max_halves(mx);
-    const float mu = mx == -INFINITY ? 0.f : mx, al = __builtin_amdgcn_exp2f((m - mu) * c), mc = mu * c;
+    const float mu = mx == -INFINITY ? 0.f : mx, al = __builtin_amdgcn_exp2f((m - mu) * c);
+    float mc = mu * c;
     m = mx;
     l *= al;
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= al;
+    if (__builtin_amdgcn_ballot_w64(fabsf(mc) > LARGE) != 0) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] -= mu;
+      mc = 0.f;
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       sc[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -mc));

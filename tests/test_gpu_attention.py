@@ -144,6 +144,39 @@ def test_peaked_scores():
     _check(q, k, v, go, 0, 0, None, 1.0)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt,power,scale", [(BF, 0, 2e4), (BF, 10, None), (BF, 0, 1e9), (BF, 14, 1.0), (BF, 58, None),
+                                            (HF, 13, None), (HF, 15, None), (HF, 0, 1e12)])
+def test_scores_of_any_finite_size(dt, power, scale, d):
+    """Scores from 1e6 to 1e36: q and k hold -1, 0 and 1 times a power of two, so that scores are exact and either equal or
+    too far apart to share a softmax: a row's output is the mean of v over its highest scores. Exponentials are 1 and 0 then,
+    so what rounds is fp32 sums (2^-24 a term) and the result (u). The same from pages for the last row."""
+    from memarch_amd.attention import paged_attention, window_attention
+    t, n, window, sinks = 200, 183, 70, 3
+    g = torch.Generator().manual_seed(power + d)
+    q, k = (torch.randint(-1, 2, (2, t, 2, d), generator=g).to(dt) * 2.0 ** power for _ in range(2))
+    v = torch.randn(2, t, 2, d, generator=g).to(dt)
+    assert torch.isfinite(q).all() and q.dtype == dt
+    lens = torch.tensor([t, n])
+    see = torch.stack([orc.visible(t, int(i), window, sinks) for i in lens])[:, None]
+    s = (q.double().transpose(1, 2) @ k.double().transpose(1, 2).mT).masked_fill(~see, -torch.inf)
+    top = (s == s.amax(-1, keepdim=True)) & see
+    p = top / top.sum(-1, keepdim=True).clamp(min=1).double()
+    vd = v.double().transpose(1, 2)
+    ref, mag = p @ vd, p @ vd.abs()
+    tol = (torch.finfo(dt).eps / 2 * ref.abs() + (t + 2) * 2.0 ** -24 * mag).transpose(1, 2) * 1.01
+    got = window_attention(q.cuda(), k.cuda(), v.cuda(), window=window, sinks=sinks, lengths=lens.cuda(), scale=scale)
+    err = (got.double().cpu() - ref.transpose(1, 2)).abs()
+    assert (err <= tol).all(), float((err - tol).max())          # (NaN fails it too)
+    pad = torch.zeros(2, 8, 2, d, dtype=dt)
+    kc, vc = (torch.cat((x, pad), 1).view(26, 16, 2, d).cuda() for x in (k, v))
+    last = torch.stack((q[0, t - 1], q[1, n - 1])).cuda()
+    out = paged_attention(last, kc, vc, torch.arange(26, device="cuda", dtype=torch.int32).view(2, 13), lens.cuda(),
+                          window=window, sinks=sinks, scale=scale)
+    for i, r in ((0, t - 1), (1, n - 1)):
+        assert ((out[i].double().cpu() - ref[i, :, r]).abs() <= tol[i, r]).all(), i
+
+
 def test_strided_operands():
     """Slices of one packed projection, head-first layouts, a broadcast batch and head, an unaligned base, a strided last
     dimension; upstream gradients expanded from one value and transposed."""
