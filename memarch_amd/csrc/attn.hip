@@ -126,7 +126,7 @@ __device__ __forceinline__ void mask_keys(f32x16& s, int row, int k0h, int windo
 // operand of the second product where they are; 64 KiB of LDS let two workgroups share a CU, whose products and
 // exponentials fill each other's gaps. p is rounded to the element type: the matrix core takes no other.
 // Measured (bf16, D = 128, 16 heads): 32768 tokens, every earlier one seen, 4.1 ms, 1.06 PFLOP/s; 4 x 16384 tokens, window
-// 1024, 0.74 ms, 0.72 PFLOP/s of visible pairs with the matrix core busy 41% of the time; 32 x 1024, window 512, 0.27 ms,
+// 1024, 0.75 ms, 0.72 PFLOP/s of visible pairs with the matrix core busy 40% of the time; 32 x 1024, window 512, 0.27 ms,
 // 23% busy: its workgroups are 2 to 11 tiles long and 1.4 of 2 waves per SIMD are there at a time.
 // With D <= 64 vector work is busy half the time and the matrix core a quarter, so waves are what fills the gaps: four per
 // SIMD, in 128 registers with the tile's offsets made again for each tile, take 96 us where three take 102 (8 texts of up to
@@ -277,7 +277,7 @@ __device__ __forceinline__ u32x4 four(const uint32_t (&w)[8], int s) {
 
 // dq_i = scale sum_j ds_ij k_j, ds_ij = p_ij (go_i . v_j - d_i), p from the forward's lse: rows stay in registers and keys
 // pass, as in the forward, so that dq is summed by one wave in one order. It also forms d and leaves -lse and -d for
-// k_attn_dkv. Measured (bf16, D = 128): 4 x 16384 tokens of 16 heads, window 1024: 1.09 ms, 0.74 PFLOP/s of visible pairs
+// k_attn_dkv. Measured (bf16, D = 128): 4 x 16384 tokens of 16 heads, window 1024: 1.10 ms, 0.73 PFLOP/s of visible pairs
 // (6 D each), matrix core busy 46% of the time.
 template <typename T, int DP>
 __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
@@ -437,8 +437,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
 // dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij go_i over the rows of all query heads that share the head: keys stay in
 // registers, 32 per wave, and row tiles pass through a ring of NS. Scores and go v are formed a second time (seven
 // products in the backward for the formula's five), which needs neither atomics nor ds in memory.
-// Measured (bf16, D = 128): 4 x 16384 tokens of 16 heads over 4, window 1024: 1.26 ms, 0.85 PFLOP/s of visible pairs (8 D
-// each), matrix core busy 46% of the time; the join of the first tokens' blocks 7 us.
+// Measured (bf16, D = 128): 4 x 16384 tokens of 16 heads over 4, window 1024: 1.24 ms, 0.86 PFLOP/s of visible pairs (8 D
+// each), matrix core busy 45% of the time; the join of the first tokens' blocks 7 us.
 template <typename T, int DP>
 __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   constexpr int IMG = BR * DP * 2;

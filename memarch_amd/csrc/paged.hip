@@ -6,8 +6,8 @@
 // the columns of the products) and a run of 32-key tiles; each of its waves walks its own tiles with its own softmax
 // state and its own double-buffered LDS images, without barriers, so that the loads of one tile are under way while the
 // previous one is used. The waves' states are joined through LDS at the end, the workgroups' through fp32 parts and a
-// second launch. Measured (bf16, D = 128, bytes of the keys seen): 64 sequences of up to 8192 tokens, 155 us, 4.6 TB/s; 8 of up
-// to 131072, 289 us, 5.0 TB/s (a large copy reaches 4.9); one of 1000 tokens 9 us, latency. The joining launch takes 4 to 8.
+// second launch. Measured (bf16, D = 128, bytes of the keys seen): 64 sequences of up to 8192 tokens, 138 us, 4.9 TB/s; 8 of up
+// to 131072, 273 us, 5.6 TB/s (a large copy, half of it writes, reaches 4.9); one of 1000 tokens 9 us, latency. The joining launch takes 4 to 8.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -285,10 +285,11 @@ __global__ __launch_bounds__(64) void k_paged_join(Args a) {
 // -------------------------------------------------------------------------------------------------------- host side
 
 // Workgroups per key/value head of a sequence. From 512 heads on one each: they fill the GPU, and the second launch and the
-// parts cost more than even rounds gain (96 sequences of 8 heads of 64, window 1024: 42.8 us against 46.7 with two each).
-// With fewer, TARGET in all (256 heads of 128, up to 8192 keys: 170, 160 and 165 us with 2, 4 and 8 each; 32 heads, up to
-// 131072 keys: 304, 295 and 313 us with 16, 32 and 64), at most one per MIN_TILES tiles of the longest sequence that the
-// table can hold.
+// parts cost more than even rounds gain (96 sequences of 8 heads of 64, window 1024: 38.7 us against 43.8 with two each). Long
+// caches are the other way round (64 of 8 heads of 128, up to 8192 keys: 285 us against 265): the line lies where windows
+// want it. With fewer heads, TARGET in all (256 heads of 128, up to 8192 keys: 148, 143 and 144 us with 2, 4 and 8 each; 32
+// heads, up to 131072 keys: 293, 277 and 272 us with 16, 32 and 64), at most one per MIN_TILES tiles of the longest sequence
+// that the table can hold (twice as many: the calls above as they are, one head with 131072 keys 31 us instead of 47).
 int64_t splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t page, int64_t max_pages, int64_t window, int64_t sinks) {
   int64_t n = page * max_pages;
   if (window > 0 && window + sinks < n) n = window + sinks;
