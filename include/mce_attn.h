@@ -10,8 +10,8 @@
  *   s_ij = scale q_i . k_j;  p_i = softmax of s_ij over the j that i sees;  out_i = sum_j p_ij v_j
  * (window = 0: every earlier position; lengths NULL: T). A row that sees nothing (i >= lengths[b]) has out = 0, and the
  * gradients of such positions are 0; rows at or past lengths[b] are never read. Inside a sequence, masked pairs get a
- * weight of exactly 0: finite values there do not matter, a NaN or an infinity may reach rows of the same or the next
- * 128-row block that do not see it.
+ * weight of exactly 0: finite values there do not matter, a NaN or an infinity may reach rows that do not see it, up to 95
+ * positions from one that does, and keys likewise (dk and dv of keys beside the first tokens, in the same 32, from any row).
  *   d_i = go_i . out_i;  ds_ij = p_ij (go_i . v_j - d_i)
  *   dq_i = scale sum_j ds_ij k_j;  dk_j = scale sum_i ds_ij q_i;  dv_j = sum_i p_ij go_i  (dk, dv summed over the heads
  *   that share them)

@@ -59,6 +59,11 @@ struct KeyTiles {
     n = n_sink + q1 / BK - lo + 1;
   }
   __device__ __forceinline__ int key0(int it) const { return (it < n_sink ? it : lo + it - n_sink) * BK; }
+  // keys that are read of the tile's: of those before the window the first tokens only, so that what lies behind them (a
+  // NaN, say) meets no row that is far from it
+  __device__ __forceinline__ int end(int it, const Args& a, int len) const {
+    return it < n_sink && a.sinks < len ? a.sinks : len;
+  }
 };
 
 // Which sequence, heads and block of rows (or keys) a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an
@@ -156,9 +161,9 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) 
     const uint16_t* const kp = a.k.p + b * a.k.sb + hk * a.k.sh;
     const uint16_t* const vp = a.v.p + b * a.v.sb + hk * a.v.sh;
     auto issue = [&](int it, int buf) {
-      const int k0 = kt.key0(it);
-      tk.issue(tile_rsrc<BK>(kp, a.k.st, k0, len, a.D), lds, buf * 2 * IMG, wave);
-      tv.issue(tile_rsrc<BK>(vp, a.v.st, k0, len, a.D), lds, buf * 2 * IMG + IMG, wave);
+      const int k0 = kt.key0(it), end = kt.end(it, a, len);
+      tk.issue(tile_rsrc<BK>(kp, a.k.st, k0, end, a.D), lds, buf * 2 * IMG, wave);
+      tv.issue(tile_rsrc<BK>(vp, a.v.st, k0, end, a.D), lds, buf * 2 * IMG + IMG, wave);
     };
     issue(0, 0);
     // the wave's query rows as fragments: row l%32, columns 16 ks + 8 h + 0..7
@@ -304,9 +309,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
     const uint16_t* const kp = a.k.p + b * a.k.sb + hk * a.k.sh;
     const uint16_t* const vp = a.v.p + b * a.v.sb + hk * a.v.sh;
     auto issue = [&](int it, int buf) {
-      const int k0 = kt.key0(it);
-      tk.issue(tile_rsrc<BK>(kp, a.k.st, k0, len, a.D), lds, buf * 2 * IMG, wave);
-      tv.issue(tile_rsrc<BK>(vp, a.v.st, k0, len, a.D), lds, buf * 2 * IMG + IMG, wave);
+      const int k0 = kt.key0(it), end = kt.end(it, a, len);
+      tk.issue(tile_rsrc<BK>(kp, a.k.st, k0, end, a.D), lds, buf * 2 * IMG, wave);
+      tv.issue(tile_rsrc<BK>(vp, a.v.st, k0, end, a.D), lds, buf * 2 * IMG + IMG, wave);
     };
     issue(0, 0);
     u32x4 qf[DP / 16], gf[DP / 16];

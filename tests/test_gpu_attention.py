@@ -101,6 +101,21 @@ def test_padded_rows_stay_zero_beside_a_nan(bad, t, n, hq, hkv, d, window, sinks
     assert torch.isfinite(got[0][0, :n - 64]).all()
 
 
+@pytest.mark.parametrize("window,sinks,at", [(40, 3, 5), (40, 3, 63), (100, 70, 80), (64, 1, 33), (130, 0, 20)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_nan_stays_near_the_rows_that_see_it(d, window, sinks, at):
+    """A NaN key and value, beside the first tokens and in the same tile as they, reach no row more than 95 positions behind
+    the last that sees them: outputs and dq there have the bits that finite values give."""
+    t = 600
+    q, k, v, go = (x.cuda() for x in _inputs(1, t, 2, 1, d, BF, seed=at))
+    base = _step(q, k, v, go, window, sinks)
+    k[0, at], v[0, at] = float("nan"), float("inf")
+    got = _step(q, k, v, go, window, sinks)
+    far = at + window + 95
+    assert got[0][0, at].isnan().all()
+    assert all(torch.equal(a[0, far:], b[0, far:]) for a, b in zip(got[:2], base[:2]))
+
+
 @pytest.mark.parametrize("b,t,hq,hkv,d,window,sinks", [
     (1, 2300, 4, 1, 64, 0, 0),         # every earlier key: rows of a key block shared by several workgroups
     (1, 2300, 4, 1, 128, 1000, 4),     # a window long enough for that, and the block with the first tokens apart
