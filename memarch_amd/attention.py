@@ -5,8 +5,8 @@ sequence over a paged cache, on MI355X (libmce_attn.so).
 their block-window helpers (lm.py:448-554, full2.py:154-181): one kernel forward, two backward, no scores in memory.
 Position i of a sequence sees position j <= i when i - j < window or j < sinks. Products take bf16 or fp16 operands and
 sum in fp32; softmax statistics are fp32 (include/mce_attn.h, include/mce_paged.h). `paged_attention` is the last row of
-the same attention for each sequence, its keys and values lying in the pages of a cache. All device work runs on torch's current stream; a tensor
-that is not on a GPU raises, and there is no other code path.
+the same attention for each sequence, its keys and values lying in the pages of a cache. All device work runs on
+torch's current stream; a tensor that is not on a GPU raises, and there is no other code path.
 """
 import math
 

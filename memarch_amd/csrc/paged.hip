@@ -6,8 +6,9 @@
 // the columns of the products) and a run of 32-key tiles; each of its waves walks its own tiles with its own softmax
 // state and its own double-buffered LDS images, without barriers, so that the loads of one tile are under way while the
 // previous one is used. The waves' states are joined through LDS at the end, the workgroups' through fp32 parts and a
-// second launch. Measured (bf16, D = 128, bytes of the keys seen): 64 sequences of up to 8192 tokens, 138 us, 4.9 TB/s; 8 of up
-// to 131072, 273 us, 5.6 TB/s (a large copy, half of it writes, reaches 4.9); one of 1000 tokens 9 us, latency. The joining launch takes 4 to 8.
+// second launch. Measured (bf16, D = 128, bytes of the keys seen): 64 sequences of up to 8192 tokens, 138 us, 4.9 TB/s;
+// 8 of up to 131072, 273 us, 5.6 TB/s (a large copy, half of it writes, reaches 4.9); one of 1000 tokens 9 us, latency. The
+// joining launch takes 4 to 8.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -322,8 +322,8 @@ __global__ __launch_bounds__(THREADS, 4) void k_rope(Args a) {
 }
 
 // Any alignment, any even R: one wave per head vector, lane e the elements e, e + 64, ...; a rotation pair's other
-// element is read again (from the cache). A step of 32 x 1024 tokens of 16 + 16 heads in bf16, norm, takes 1.06 ms with D = 80,
-// R = 40 and 1.09 ms with D = 96, R = 24, where R = D in whole pieces takes 0.23 and 0.25.
+// element is read again (from the cache). A step of 32 x 1024 tokens of 16 + 16 heads in bf16, norm, takes 1.06 ms with
+// D = 80, R = 40 and 1.09 ms with D = 96, R = 24, where R = D in whole pieces takes 0.23 and 0.25.
 template <typename T, bool NORM, bool IL, bool BWD>
 __global__ __launch_bounds__(THREADS) void k_rope_any(Args a) {
   constexpr int E = 4;   // elements per lane: D <= 256
