@@ -1,0 +1,534 @@
+"""The serving operators' calls whose speed is measured: causal attention over packed sequences (with its gradients),
+writing keys and values into an 8-bit paged cache and reading them back, and one new token's attention over that cache.
+
+`listed()` gives the named cases, `draw(rng)` one more of the same ranges; `prepare` makes what a training or serving
+program holds before the call, `run` is one pass (the framework's entry points where `own` is true, elementary torch
+operations in fp32 otherwise), `exact` the same results in 64 bits, `work` the bytes and operations a pass needs.
+
+Sequences are of different lengths, from none at all to several times the mean. Keys are RMS-normalised head vectors
+with a gain of 1.5 that share a direction per head; values are N(0, 1) times a log-normal factor per token, so that the
+8-bit blocks differ in scale and a scale has to grow as tokens are added; upstream gradients are N(0, 1).
+
+The cache: float8_e4m3fn [pages, page, heads, dim]; `block` tokens of a page and a head share a scale, the smallest power
+of two with which the largest magnitude of the block's tokens so far is within 448; a block that grows keeps the larger
+scale, and its earlier codes are rounded again to it.
+"""
+import math
+
+import torch
+
+own = False
+
+_DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+_F8 = torch.float8_e4m3fn
+_DEV = "cuda"
+
+
+def listed():
+    return [
+        # a small model's training step on a few packed texts, as unit runs make it: launches and host time count
+        dict(name="packed_small", op="packed", b=6, tokens=700, earlier=0, pad=0, hq=4, hkv=4, d=64, window=0, sinks=0,
+             dtype="bf16", train=True),
+        # a training step of 32768 packed tokens at d = 2048
+        dict(name="packed_train", op="packed", b=24, tokens=32768, earlier=0, pad=0, hq=16, hkv=16, d=128, window=0,
+             sinks=0, dtype="bf16", train=True),
+        # texts of odd lengths in a buffer that they do not fill, window and first tokens, grouped heads, fp16
+        dict(name="packed_window", op="packed", b=13, tokens=49999, earlier=0, pad=113, hq=16, hkv=4, d=64, window=1024,
+             sinks=4, dtype="fp16", train=True),
+        # a batch of prompts read at once
+        dict(name="packed_prompts", op="packed", b=16, tokens=65536, earlier=0, pad=0, hq=16, hkv=4, d=128, window=0,
+             sinks=0, dtype="bf16", train=False),
+        # the next pieces of prompts that are read piece by piece: few queries behind many earlier keys
+        dict(name="packed_pieces", op="packed", b=8, tokens=8192, earlier=131072, pad=0, hq=16, hkv=4, d=128, window=0,
+             sinks=0, dtype="bf16", train=False),
+        # pieces of short prompts into the cache and all of it back: latency counts
+        dict(name="store_small", op="store", b=4, tokens=120, earlier=400, hkv=4, d=64, page=16, block=16, dtype="bf16"),
+        # a batch of prompts' pieces behind their earlier tokens
+        dict(name="store_prompts", op="store", b=16, tokens=65536, earlier=32768, hkv=8, d=128, page=64, block=32,
+             dtype="bf16"),
+        # few long prompts of odd length, large blocks, heads that fill no whole tile
+        dict(name="store_long", op="store", b=3, tokens=20011, earlier=100003, hkv=2, d=96, page=128, block=128,
+             dtype="fp16"),
+        # one sequence's next token after a short text: written, then its attention
+        dict(name="step_1x1000", op="step", b=1, tokens=1000, hq=16, hkv=16, d=128, page=16, block=16, window=0,
+             sinks=0, dtype="bf16", write=True),
+        # a decoding step of a batch of sequences
+        dict(name="step_64x5000", op="step", b=64, tokens=320000, hq=16, hkv=4, d=128, page=64, block=32, window=0,
+             sinks=0, dtype="bf16", write=True),
+        # a model with a window: few keys are read out of long caches
+        dict(name="step_window", op="step", b=96, tokens=1000000, hq=16, hkv=8, d=64, page=16, block=16, window=1024,
+             sinks=4, dtype="fp16", write=False),
+        # a few very long sequences: work has to be split over the cache's length
+        dict(name="step_8x131072", op="step", b=8, tokens=1048576, hq=16, hkv=4, d=128, page=64, block=64, window=0,
+             sinks=0, dtype="bf16", write=False),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["packed", "packed", "store", "step", "step"])
+    hkv = rng.choice([1, 2, 4, 8, 12, 16])
+    hq = hkv * rng.choice([g for g in (1, 1, 2, 4, 8, 16) if hkv * g <= 16])
+    dtype = rng.choice(["bf16", "bf16", "fp16"])
+    window = 0 if rng.random() < 0.6 else _log(rng, 16, 4096)
+    sinks = rng.choice([0, 1, 4, 16]) if window else 0
+    if op == "packed":
+        d = rng.choice([64, 128, 128, 80, 96])
+        while True:
+            tokens = _log(rng, 1, 65536)
+            b = _log(rng, 1, max(1, min(256, tokens)))
+            train = rng.random() < 0.6
+            earlier = _log(rng, 1, 131072) if rng.random() < 0.3 else 0
+            case = dict(op=op, b=b, tokens=tokens, earlier=earlier, pad=rng.choice([0, 0, 1, 200]), hq=hq, hkv=hkv, d=d,
+                        window=window, sinks=sinks, dtype=dtype, train=train)
+            # no more elements or operations than the largest listed case
+            if (tokens + earlier) * hkv * d <= 1 << 27 and work(case)["flops"] <= 1.4e12:
+                return case
+    d = rng.choice([64, 128, 128, 80, 96])
+    page = rng.choice([16, 16, 32, 64, 128])
+    block = rng.choice([x for x in (8, 16, 16, 32, 64, 128) if page % x == 0])
+    if op == "store":
+        tokens = _log(rng, 1, min(131072, (1 << 26) // (hkv * d)))
+        return dict(op=op, b=_log(rng, 1, min(256, tokens)), tokens=tokens,
+                    earlier=0 if rng.random() < 0.3 else _log(rng, 1, min(131072, (1 << 26) // (hkv * d))), hkv=hkv, d=d,
+                    page=page, block=block, dtype=dtype)
+    tokens = _log(rng, 1, (1 << 29) // (max(hkv, hq / 4) * d))
+    b = _log(rng, 1, min(256, tokens))
+    return dict(op=op, b=max(b, -(-tokens // 131072)), tokens=tokens, hq=hq, hkv=hkv, d=d, page=page, block=block,
+                window=window, sinks=sinks, dtype=dtype, write=rng.random() < 0.5)
+
+
+# ------------------------------------------------------------------------------------------------------ inputs
+
+
+def _spread(total, b, least=0):
+    """b lengths that add up to total, from `least` (a sequence of eight or more, where least is 0: none at all) to about
+    twice the mean."""
+    w = [0.2 + 1.8 * (0.5 + 0.6180339887498949 * i) % 1.8 for i in range(b)]
+    if least == 0 and b >= 8:
+        w[3] = 0.0
+    s, at, cuts = sum(w), 0.0, [0]
+    for x in w:
+        at += x
+        cuts.append(round((total - least * b) * at / s))
+    return [cuts[i + 1] - cuts[i] + least for i in range(b)]
+
+
+def _lengths(case):
+    """(new tokens, tokens with the earlier ones) of each sequence of a packed or store case."""
+    new = _spread(case["tokens"], case["b"])
+    return new, [n + e for n, e in zip(new, _spread(case["earlier"], case["b"])[::-1])]
+
+
+def _cu(lens):
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return torch.tensor(cu, dtype=torch.int32, device=_DEV)
+
+
+def _keys(g, *shape, gain=1.5):
+    """RMS-normalised head vectors [..., h, d] with a gain, sharing a direction per head."""
+    x = torch.randn(*shape, generator=g, device=_DEV)
+    x += 0.3 * torch.randn(*shape[-2:], generator=g, device=_DEV)
+    x *= gain * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + 1e-6)
+    return x
+
+
+def _values(g, *shape):
+    """N(0, 1) head vectors [tokens..., h, d] times a log-normal factor per token."""
+    x = torch.randn(*shape, generator=g, device=_DEV)
+    x *= (0.5 * torch.randn(*shape[:-2], 1, 1, generator=g, device=_DEV)).exp_()
+    return x
+
+
+def _pow2_scale(amax):
+    """The smallest power of two s with amax <= 448 s (2^-100 at least), fp32."""
+    m, e = torch.frexp(amax.clamp(min=448 * 2.0 ** -100))   # m 2^e, m in [0.5, 1); 448 = 0.875 2^9
+    return torch.ldexp(torch.ones_like(amax), e - 9 + (m > 0.875))
+
+
+def _filled(x, block):
+    """Codes and scales of a whole cache from its values [pages, page, h, d]."""
+    pages, page, h, d = x.shape
+    x = x.view(pages, page // block, block, h, d)
+    s = _pow2_scale(x.abs().amax((2, 4)))
+    return (x / s[:, :, None, :, None]).to(_F8).view(pages, page, h, d), s
+
+
+def _cache(st, g, lens):
+    """A cache in which the sequences' pages lie in any order, filled with tokens of earlier calls (also behind the
+    sequences' ends); table entries that a sequence does not need are -1."""
+    case = st["case"]
+    page, h, d = case["page"], case["hkv"], case["d"]
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + 3
+    order = torch.randperm(pages, generator=g, device=_DEV).int()
+    table = torch.full((case["b"], max(max(need), 1)), -1, dtype=torch.int32, device=_DEV)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[at:at + n]
+        at += n
+    st["table"] = table
+    st["kc"], st["ks"] = _filled(_keys(g, pages, page, h, d), case["block"])
+    st["vc"], st["vs"] = _filled(_values(g, pages, page, h, d), case["block"])
+    st["lens"] = torch.tensor(lens, dtype=torch.int32, device=_DEV)
+    st["host_lens"] = lens   # for the loops of the 64-bit form, and the plain form's longest row
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=_DEV).manual_seed(seed)
+    op, dt, b, hkv, d = case["op"], _DT[case["dtype"]], case["b"], case["hkv"], case["d"]
+    st = dict(case=case)
+    mix = torch.randperm(b, generator=torch.Generator().manual_seed(seed)).tolist()   # the sequences' order
+    if op == "step":
+        lens = _spread(case["tokens"], b, 1 if case["write"] and case["tokens"] >= b else 0)
+        _cache(st, g, [lens[i] for i in mix])
+        st["q"] = _keys(g, b, case["hq"], d).to(dt)
+        if case["write"]:
+            st["k"] = _keys(g, b, hkv, d).to(dt)
+            st["v"] = _values(g, b, hkv, d).to(dt)
+        return st
+    new, whole = ([x[i] for i in mix] for x in _lengths(case))
+    st["new"], st["whole"] = new, whole   # on the host, for the loops of the plain and the 64-bit form
+    st["cu"], st["cu_k"] = _cu(new), _cu(whole)
+    if op == "store":
+        _cache(st, g, whole)
+        # slices of one projection's output
+        x = torch.empty(case["tokens"], 2, hkv, d, dtype=dt, device=_DEV)
+        x[:, 0] = _keys(g, case["tokens"], hkv, d)
+        x[:, 1] = _values(g, case["tokens"], hkv, d)
+        st["k"], st["v"] = x[:, 0], x[:, 1]
+        return st
+    n, m = case["tokens"] + case["pad"], case["tokens"] + case["earlier"] + case["pad"]
+    st["q"] = _keys(g, n, case["hq"], d).to(dt)
+    st["k"] = _keys(g, m, hkv, d).to(dt)
+    st["v"] = torch.randn(m, hkv, d, generator=g, device=_DEV).to(dt)
+    if case["train"]:
+        st["go"] = torch.randn(n, case["hq"], d, generator=g, device=_DEV).to(dt)
+        for x in ("q", "k", "v"):
+            st[x].requires_grad_()
+    return st
+
+
+# ------------------------------------------------------------------------------------------- the framework's calls
+
+
+def _own(st):
+    from memarch_amd import attention, kv_cache
+    case = st["case"]
+    if case["op"] == "store":
+        cache = (st["kc"], st["vc"], st["ks"], st["vs"], st["table"])
+        kv_cache.cache_write(st["k"], st["v"], *cache, st["lens"], cu_seqlens=st["cu"])
+        rows = case["tokens"] + case["earlier"]
+        k, v = kv_cache.cache_read(*cache, st["cu_k"], rows, dtype=st["k"].dtype)
+        return k, v, st["ks"], st["vs"]
+    window = case["window"] or None
+    if case["op"] == "packed":
+        out = attention.packed_attention(st["q"], st["k"], st["v"], st["cu"],
+                                         cu_seqlens_k=st["cu_k"] if case["earlier"] else None, window=window,
+                                         sinks=case["sinks"])
+        if not case["train"]:
+            return (out,)
+        return (out, *torch.autograd.grad(out, (st["q"], st["k"], st["v"]), st["go"]))
+    if case["write"]:
+        kv_cache.cache_write(st["k"], st["v"], st["kc"], st["vc"], st["ks"], st["vs"], st["table"], st["lens"])
+    out = attention.paged_attention(st["q"], st["kc"], st["vc"], st["table"], st["lens"], window=window,
+                                    sinks=case["sinks"], k_scale=st["ks"], v_scale=st["vs"])
+    return (out, st["ks"], st["vs"]) if case["write"] else (out,)
+
+
+# --------------------------------------------------------------------------------------------------- plain forms
+
+_SCORES = 1 << 28   # scores of one block of rows
+
+
+def _plain_packed(st):
+    """Sequence after sequence, block after block of its query rows against the keys that any of them sees; the first
+    tokens before the window are put in front of them."""
+    case = st["case"]
+    hq, hkv, d, train = case["hq"], case["hkv"], case["d"], case["train"]
+    dt, grp, scale = st["q"].dtype, hq // hkv, 1 / math.sqrt(d)
+    q = st["q"].detach().float().transpose(0, 1).reshape(hkv, grp, -1, d)
+    k, v = (st[x].detach().float().transpose(0, 1)[:, None] for x in ("k", "v"))
+    out = torch.zeros_like(q)
+    if train:
+        go = st["go"].float().transpose(0, 1).reshape(hkv, grp, -1, d)
+        dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    q0 = k0 = 0
+    for n, m in zip(st["new"], st["whole"]):
+        window = case["window"] or m
+        pos = torch.arange(m, device=_DEV)
+        step = max(1, _SCORES // (hq * m)) if m else 1
+        for i0 in range(m - n, m, step):
+            i1 = min(m, i0 + step)
+            lo = max(0, i0 - window + 1)
+            first = min(case["sinks"], lo)
+            i, j = pos[i0:i1, None], torch.cat((pos[:first], pos[lo:i1]))[None]
+            see = (j <= i) & ((i - j < window) | (j < case["sinks"]))
+            rows = slice(q0 + i0 - (m - n), q0 + i1 - (m - n))
+            qb = q[:, :, rows]
+            kb = torch.cat((k[:, :, k0:k0 + first], k[:, :, k0 + lo:k0 + i1]), 2)
+            vb = torch.cat((v[:, :, k0:k0 + first], v[:, :, k0 + lo:k0 + i1]), 2)
+            s = torch.matmul(qb, kb.transpose(-1, -2).contiguous()) * scale
+            s = s.masked_fill(~see, -math.inf)
+            p = s.sub_(s.amax(-1, keepdim=True)).exp_()
+            p = p / p.sum(-1, keepdim=True)
+            ob = torch.matmul(p, vb)
+            out[:, :, rows] = ob
+            if train:
+                gb = go[:, :, rows]
+                dvb = torch.matmul(p.transpose(-1, -2).contiguous(), gb).sum(1, keepdim=True)
+                ds = torch.matmul(gb, vb.transpose(-1, -2).contiguous())
+                ds = p * (ds - (gb * ob).sum(-1, keepdim=True)) * scale
+                dq[:, :, rows] = torch.matmul(ds, kb)
+                dkb = torch.matmul(ds.transpose(-1, -2).contiguous(), qb).sum(1, keepdim=True)
+                for acc, part in ((dk, dkb), (dv, dvb)):
+                    acc[:, :, k0:k0 + first] += part[:, :, :first]
+                    acc[:, :, k0 + lo:k0 + i1] += part[:, :, first:]
+        q0, k0 = q0 + n, k0 + m
+
+    def back(x):
+        return x.reshape(-1, x.shape[2], d).transpose(0, 1).to(dt).contiguous()
+    return (back(out), back(dq), back(dk), back(dv)) if train else (back(out),)
+
+
+def _plain_write(st, seq, pos, starts):
+    """The rows of st["k"] and st["v"] become tokens pos of the sequences seq; starts: each sequence's first new token."""
+    case = st["case"]
+    page, block, hkv = case["page"], case["block"], case["hkv"]
+    per = page // block
+    at = st["table"][seq, pos // page].long()            # page of each row
+    blk = at * per + pos % page // block                 # and its block, of the cache's
+    live = starts[seq] == pos                            # each sequence's first new row, to find its first block
+    older = torch.zeros(st["ks"].shape[0] * per, device=_DEV)
+    older = older.index_add_(0, blk, (live & (pos % block > 0)).float()) > 0
+    touched = torch.zeros_like(older)
+    touched[blk] = True
+    for x, cache, scale in ((st["k"], st["kc"], st["ks"]), (st["v"], st["vc"], st["vs"])):
+        x = x.float()
+        amax = torch.zeros(older.shape[0], hkv, device=_DEV)
+        amax.scatter_reduce_(0, blk[:, None].expand(-1, hkv), x.abs().amax(-1), "amax")
+        had = scale.view(-1, hkv)
+        s = _pow2_scale(amax)
+        s = torch.where(older[:, None], torch.maximum(s, had), s)
+        s = torch.where(touched[:, None], s, had)
+        grown = (s != had) & older[:, None]
+        codes = cache.view(torch.uint8).view(-1, block, hkv, case["d"])
+        again = torch.where(grown.any(1))[0]
+        part = codes[again].view(_F8).float()
+        part = torch.where(grown[again][:, None, :, None], part * (had[again] / s[again])[:, None, :, None], part)
+        codes[again] = part.to(_F8).view(torch.uint8)
+        cache.view(torch.uint8)[at, pos % page] = (x / s[blk][:, :, None]).to(_F8).view(torch.uint8)
+        scale.copy_(s.view_as(scale))
+
+
+def _plain_store(st):
+    case = st["case"]
+    page, block = case["page"], case["block"]
+    cu, lens = st["cu"].long(), st["lens"].long()
+    row = torch.arange(case["tokens"], device=_DEV)
+    seq = torch.searchsorted(cu[1:], row, right=True)
+    starts = lens - (cu[1:] - cu[:-1])
+    _plain_write(st, seq, starts[seq] + row - cu[seq], starts)
+    cu = st["cu_k"].long()
+    row = torch.arange(case["tokens"] + case["earlier"], device=_DEV)
+    seq = torch.searchsorted(cu[1:], row, right=True)
+    pos = row - cu[seq]
+    at = st["table"][seq, pos // page].long()
+    dt = st["k"].dtype
+    k, v = ((c.view(torch.uint8)[at, pos % page].view(_F8).float() * s[at, pos % page // block][:, :, None]).to(dt)
+            for c, s in ((st["kc"], st["ks"]), (st["vc"], st["vs"])))
+    return k, v, st["ks"], st["vs"]
+
+
+def _plain_step(st):
+    """All sequences at once, as rows of the longest; with a window, its keys and the first tokens alone."""
+    case = st["case"]
+    grp, d, page, block = case["hq"] // case["hkv"], case["d"], case["page"], case["block"]
+    b, lens = case["b"], st["lens"].long()
+    if case["write"]:
+        live = torch.where(lens > 0)[0] if min(st["host_lens"]) == 0 else torch.arange(b, device=_DEV)
+        sub = dict(st, k=st["k"][live], v=st["v"][live])
+        _plain_write(sub, live, lens[live] - 1, lens - 1)
+    longest = max(max(st["host_lens"]), 1)
+    if case["window"]:
+        near = torch.arange(min(longest, case["window"]), device=_DEV)
+        first = torch.arange(min(case["sinks"], longest), device=_DEV).expand(b, -1)
+        lo = (lens - case["window"]).clamp_(min=0)[:, None]
+        pos = torch.cat((first, lo + near), 1)
+        see = torch.cat((first < lo, lo + near < lens[:, None]), 1)
+    else:
+        pos = torch.arange(longest, device=_DEV).expand(b, -1)
+        see = pos < lens[:, None]
+    at = torch.where(see, st["table"].gather(1, (pos // page).clamp(max=st["table"].shape[1] - 1)), 0).long()
+    k, v = (c.view(torch.uint8)[at, pos % page].view(_F8).float() * s[at, pos % page // block][..., None]
+            for c, s in ((st["kc"], st["ks"]), (st["vc"], st["vs"])))
+    q = st["q"].float().view(b, -1, grp, d) / math.sqrt(d)
+    s = torch.matmul(q, k.permute(0, 2, 3, 1).contiguous())
+    s = s.masked_fill(~see[:, None, None], -math.inf)
+    p = (s - s.amax(-1, keepdim=True).clamp(min=-1e30)).exp()
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-30)
+    out = torch.matmul(p, v.transpose(1, 2).contiguous()).reshape(b, -1, d).to(st["q"].dtype)
+    return (out, st["ks"], st["vs"]) if case["write"] else (out,)
+
+
+_PLAIN = {"packed": _plain_packed, "store": _plain_store, "step": _plain_step}
+
+
+def run(state):
+    return _own(state) if own else _PLAIN[state["case"]["op"]](state)
+
+
+# ------------------------------------------------------------------------------------------------------ 64 bits
+
+
+def _exact_packed(case, st):
+    """One sequence and one query head at a time, dense scores of a band of rows, gradients by autograd."""
+    hq, hkv, d, train = case["hq"], case["hkv"], case["d"], case["train"]
+    grp = hq // hkv
+    out = torch.zeros(st["q"].shape, dtype=torch.float64, device=_DEV)
+    grads = [torch.zeros(st[x].shape, dtype=torch.float64, device=_DEV) for x in "qkv"]
+    cq, ck = st["cu"].tolist(), st["cu_k"].tolist()
+    for i in range(case["b"]):
+        n, m = cq[i + 1] - cq[i], ck[i + 1] - ck[i]
+        band = max(1, min(n, (1 << 27) // max(m, 1)))
+        for h in range(hq):
+            for r0 in range(0, n, band):
+                r1 = min(n, r0 + band)
+                far = m - n + r1
+                rows, cols = slice(cq[i] + r0, cq[i] + r1), slice(ck[i], ck[i] + far)
+                q = st["q"][rows, h].detach().double().requires_grad_(train)
+                k = st["k"][cols, h // grp].detach().double().requires_grad_(train)
+                v = st["v"][cols, h // grp].detach().double().requires_grad_(train)
+                dist = torch.arange(m - n + r0, far, device=_DEV)[:, None] - torch.arange(far, device=_DEV)[None]
+                hide = dist < 0
+                if case["window"]:
+                    out_of = dist >= case["window"]
+                    out_of[:, :case["sinks"]] = False
+                    hide = hide | out_of
+                s = (q @ k.T / d ** 0.5).masked_fill(hide, float("-inf"))
+                o = torch.softmax(s, -1) @ v
+                out[rows, h] = o.detach()
+                if train:
+                    dq, dk, dv = torch.autograd.grad(o, (q, k, v), st["go"][rows, h].double())
+                    grads[0][rows, h] = dq
+                    grads[1][cols, h // grp] += dk
+                    grads[2][cols, h // grp] += dv
+    return (out, *grads) if train else (out,)
+
+
+def _nearest8(x):
+    """x rounded to the nearest e4m3 value, ties to even: 3 bits behind the leading one, steps of 2^-9 at least."""
+    step = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -6))) - 3)
+    return torch.round(x / step) * step
+
+
+def _exact_cache(st, first):
+    """The cache's values and scales in 64 bits after the new tokens were written, sequence after sequence and block after
+    block; first: position of each sequence's first new token, whose rows lie in order."""
+    case = st["case"]
+    page, block = case["page"], case["block"]
+    table, at = st["table"].tolist(), 0
+    done = []
+    for x, cache, scale in ((st["k"], st["kc"], st["ks"]), (st["v"], st["vc"], st["vs"])):
+        scale = scale.double()
+        x = x.double()
+        values = cache.float().double()
+        values *= scale.repeat_interleave(block, 1)[..., None]
+        at = 0
+        for i, n in enumerate(st["host_lens"]):
+            p = first[i]
+            while p < n:
+                stop = min(n, p // block * block + block)
+                pg, sl = table[i][p // page], p % page
+                b, had = sl // block, sl % block
+                rows = x[at:at + stop - p]
+                top = rows.abs().amax((0, 2))
+                s = torch.exp2(torch.ceil(torch.log2(top / 448)).clamp(min=-100))
+                if had:
+                    s = torch.maximum(s, scale[pg, b])
+                    old = values[pg, sl - had:sl]
+                    values[pg, sl - had:sl] = _nearest8(old / s[:, None]) * s[:, None]
+                values[pg, sl:sl + stop - p] = _nearest8(rows / s[:, None]) * s[:, None]
+                scale[pg, b] = s
+                at += stop - p
+                p = stop
+        done += [values, scale]
+    return done
+
+
+def _exact_store(case, st):
+    if case["tokens"] // case["block"] + 2 * case["b"] > 4096:   # one block after the other takes too long
+        return None
+    kv, ks, vv, vs = _exact_cache(st, [m - n for n, m in zip(st["new"], st["whole"])])
+
+    def rows(values):
+        parts = [values[st["table"][i].long().clamp(min=0)].flatten(0, 1)[:m] for i, m in enumerate(st["whole"])]
+        return torch.cat(parts)
+    return rows(kv), rows(vv), ks, vs
+
+
+def _exact_step(case, st):
+    """The cache of one sequence laid out in order, one head after the other."""
+    grp, block = case["hq"] // case["hkv"], case["block"]
+    lens = st["host_lens"]
+    if case["write"]:
+        live = [i for i in range(case["b"]) if lens[i]]
+        kv, ks, vv, vs = _exact_cache(dict(st, k=st["k"][live], v=st["v"][live]), [n - 1 if n else 0 for n in lens])
+    out = torch.zeros(st["q"].shape, dtype=torch.float64, device=_DEV)
+    for i, n in enumerate(lens):
+        pages = st["table"][i].long().clamp(min=0)
+        if case["write"]:
+            k, v = kv[pages].flatten(0, 1)[:n], vv[pages].flatten(0, 1)[:n]
+        else:
+            k, v = ((c.view(torch.uint8)[pages].view(_F8).double() * s[pages].double().repeat_interleave(block, 1)[..., None]).flatten(0, 1)[:n]
+                    for c, s in ((st["kc"], st["ks"]), (st["vc"], st["vs"])))
+        ago = n - 1 - torch.arange(n, device=_DEV)
+        for h in range(case["hq"] if n else 0):
+            s = k[:, h // grp] @ st["q"][i, h].double() / case["d"] ** 0.5
+            if case["window"]:
+                hide = ago >= case["window"]
+                hide[:case["sinks"]] = False
+                s[hide] = float("-inf")
+            out[i, h] = torch.softmax(s, 0) @ v[:, h // grp]
+    return (out, ks, vs) if case["write"] else (out,)
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    return {"packed": _exact_packed, "store": _exact_store, "step": _exact_step}[case["op"]](case, st)
+
+
+# --------------------------------------------------------------------------------------------------------- work
+
+
+def _pairs(n, m, window, sinks):
+    """Visible (query, key) pairs of the last n of m tokens."""
+    def upto(t):
+        if not window or window >= t:
+            return t * (t + 1) // 2
+        return window * (window + 1) // 2 + (t - window) * window + sum(max(0, t - window - j) for j in range(sinks))
+    return upto(m) - upto(m - n)
+
+
+def work(case):
+    hkv, d = case["hkv"], case["d"]
+    if case["op"] == "packed":
+        pairs = sum(_pairs(n, m, case["window"], case["sinks"]) for n, m in zip(*_lengths(case)))
+        q, k = case["tokens"] * case["hq"] * d * 2, (case["tokens"] + case["earlier"]) * hkv * d * 2
+        train = case["train"]
+        return {"bytes": q * (4 if train else 2) + k * (4 if train else 2),
+                "flops": pairs * case["hq"] * d * (14 if train else 4)}
+    if case["op"] == "store":
+        new, whole = case["tokens"] * hkv, (case["tokens"] + case["earlier"]) * hkv
+        scales = (new + whole) * 4 // case["block"]
+        return {"bytes": 2 * (new * d * 3 + whole * d * 3 + scales), "flops": 4 * (new + whole) * d}
+    keys = sum(min(n, case["window"] + case["sinks"]) if case["window"] else n
+               for n in _spread(case["tokens"], case["b"], 1 if case["write"] and case["tokens"] >= case["b"] else 0))
+    new = case["b"] * hkv * d * 3 if case["write"] else 0
+    return {"bytes": 2 * (keys * hkv * (d + 4 / case["block"]) + new + case["b"] * case["hq"] * d * 2),
+            "flops": keys * case["hq"] * d * 4}
