@@ -236,8 +236,8 @@ def _own(st):
         return (out, *torch.autograd.grad(out, (st["q"], st["k"], st["v"]), st["go"]))
     if case["write"]:
         kv_cache.cache_write(st["k"], st["v"], st["kc"], st["vc"], st["ks"], st["vs"], st["table"], st["lens"])
-    out = attention.paged_attention(st["q"], st["kc"], st["vc"], st["table"], st["lens"], window=window,
-                                    sinks=case["sinks"], k_scale=st["ks"], v_scale=st["vs"])
+    out = kv_cache.cache_attention(st["q"], st["kc"], st["vc"], st["ks"], st["vs"], st["table"], st["lens"],
+                                   window=window, sinks=case["sinks"])
     return (out, st["ks"], st["vs"]) if case["write"] else (out,)
 
 
