@@ -1,5 +1,5 @@
-"""ctypes binding of libmce.so (declarations in include/mce.h) and libmce_attn.so (include/mce_attn.h, mce_paged.h,
-mce_rope.h).
+"""ctypes binding of libmce.so (declarations in include/mce.h), libmce_attn.so (include/mce_attn.h, mce_paged.h,
+mce_rope.h) and libmce_serve.so (include/mce_pack.h, mce_cache.h).
 
 torch is imported before the library is loaded: torch ships its own libamdhip64.so with the same SONAME as
 /opt/rocm's, so loading torch first makes libmce.so bind to the one HIP runtime that owns torch's streams
@@ -13,6 +13,7 @@ import torch  # noqa: F401  (must precede the CDLL load, see module docstring)
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmce.so")
 ATTN_LIB_PATH = os.path.join(HERE, "libmce_attn.so")
+SERVE_LIB_PATH = os.path.join(HERE, "libmce_serve.so")
 
 _P = ctypes.c_void_p
 _F = ctypes.c_float
@@ -89,8 +90,19 @@ ATTN_SIGNATURES = {
                      [_INT, _F, _INT, _INT, _P, _P, _P, _P, _P, _S, _P]),
 }
 
+# the library of packed sequences and of the 8-bit cache, in the order of include/mce_pack.h, include/mce_cache.h
+_ROWS = [_P, _I, _I]   # pointer and element strides (token, head)
+SERVE_SIGNATURES = {
+    "mce_serve_error_string": (ctypes.c_char_p, [_INT]),
+    "mce_serve_last_hip_error": (_INT, []),
+    "mce_pack_fwd": (_INT, 3 * _ROWS + [_P, _P] + 8 * [_I] + [_F, _INT, _P, _P, _P, _P]),
+    "mce_pack_bwd_ws_bytes": (_S, 8 * [_I]),
+    "mce_pack_bwd": (_INT, 4 * _ROWS + [_P, _P] + 8 * [_I] + [_F, _INT, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+}
+
 _lib = None
 _attn_lib = None
+_serve_lib = None
 _call_hook = None  # optional callable(name, phase) run around every C-ABI call, phase "begin" / "end"
 
 
@@ -125,8 +137,20 @@ def load_attn():
     return _attn_lib
 
 
+def load_serve():
+    """Load libmce_serve.so once. Raises if the library has not been built: there is no fallback path."""
+    global _serve_lib
+    if _serve_lib is None:
+        _serve_lib = _load(SERVE_LIB_PATH, SERVE_SIGNATURES)
+    return _serve_lib
+
+
 def check(rc, what):
     if rc != 0:
+        if what in SERVE_SIGNATURES:
+            lib = load_serve()
+            msg = lib.mce_serve_error_string(rc).decode()
+            raise MceError(f"{what} failed: {msg} (code {rc}, hipError {lib.mce_serve_last_hip_error()})")
         if what in ATTN_SIGNATURES:
             lib = load_attn()
             msg = lib.mce_attn_error_string(rc).decode()
@@ -149,7 +173,7 @@ def call(name, *args):
     hook = _call_hook
     if hook is not None:
         hook(name, "begin")
-    lib = load_attn() if name in ATTN_SIGNATURES else load()
+    lib = load_serve() if name in SERVE_SIGNATURES else load_attn() if name in ATTN_SIGNATURES else load()
     check(getattr(lib, name)(*args), name)
     if hook is not None:
         hook(name, "end")

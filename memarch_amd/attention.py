@@ -1,5 +1,5 @@
-"""Causal attention over a sliding window with first tokens that stay visible, and its form for one new token per
-sequence over a paged cache, on MI355X (libmce_attn.so).
+"""Causal attention over a sliding window with first tokens that stay visible, over a padded batch or packed sequences, and
+its form for one new token per sequence over a paged cache, on MI355X (libmce_attn.so, libmce_serve.so).
 
 `window_attention(q, k, v, window, sinks, lengths)` stands where memarch's blocks call scaled_dot_product_attention or
 their block-window helpers (lm.py:448-554, full2.py:154-181): one kernel forward, two backward, no scores in memory.
@@ -180,6 +180,119 @@ def window_attention(q, k, v, window=None, sinks=0, lengths=None, scale=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
     return _forward(q, k, v, lengths, window, sinks, scale, False)[3]
+
+
+def _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, train):
+    N, Hq, D = q.shape
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    out = torch.empty(N, Hq, D, dtype=q.dtype, device=q.device)
+    res = torch.empty_like(out) if train else None
+    lse = torch.empty(Hq, N, dtype=torch.float32, device=q.device) if train else None
+    with _On(q.device):
+        _lib.call("mce_pack_fwd", *qs, *ks, *vs, cu.data_ptr(), _ptr(cu_k), cu.shape[0] - 1, N, k.shape[0], Hq, k.shape[1],
+                  D, window, sinks, scale, _DTYPES[q.dtype], out.data_ptr(), _ptr(res), _ptr(lse), _stream(q.device))
+    return q, k, v, out, res, lse
+
+
+def _mark_leaves(out, dev):
+    """Leaves the current stream's number on the gradient accumulators of the call's leaves, which live as long as a graph
+    that uses them."""
+    for node, _ in out.grad_fn.next_functions:
+        if node is not None and type(node).__name__ == "AccumulateGrad":
+            node.metadata.setdefault("memarch_stream", torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _check_capture(ctx, dev):
+    """Refuses to capture a backward whose leaves an earlier graph still holds: autograd makes their accumulators wait on
+    the stream where that graph was made, which draws the stream into the capture and ends the process."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    here = torch.cuda.current_stream(dev).cuda_stream
+    for node, _ in ctx.next_functions:
+        if node is not None and type(node).__name__ == "AccumulateGrad" and \
+                node.metadata.get("memarch_stream", here) != here:
+            raise RuntimeError("a backward cannot be captured while a graph of the same leaves that was made on another "
+                               "stream is alive: delete its outputs first, or capture with detached leaves")
+
+
+class _PackedAttention(torch.autograd.Function):
+    """forward(ctx, q, k, v, cu, cu_k, window, sinks, scale) -> out; backward -> dq, dk, dv."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu, cu_k, window, sinks, scale):
+        q, k, v, out, res, lse = _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, out, res, lse, cu, cu_k)
+        ctx.mask = (window, sinks, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go):
+        q, k, v, out, res, lse, cu, cu_k = ctx.saved_tensors
+        _check_capture(ctx, q.device)
+        window, sinks, scale = ctx.mask
+        (N, Hq, D), (M, Hkv, _) = q.shape, k.shape
+        nseq = cu.shape[0] - 1
+        (q, qs), (k, ks), (v, vs), (go, gs) = _rows(q), _rows(k), _rows(v), _rows(go)
+        dq = torch.empty(N, Hq, D, dtype=q.dtype, device=q.device)
+        dk = torch.empty(M, Hkv, D, dtype=q.dtype, device=q.device)
+        dv = torch.empty_like(dk)
+        n = _lib.load_serve().mce_pack_bwd_ws_bytes(nseq, N, M, Hq, Hkv, D, window, sinks)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        with _On(q.device):
+            _lib.call("mce_pack_bwd", *qs, *ks, *vs, *gs, cu.data_ptr(), _ptr(cu_k), nseq, N, M, Hq, Hkv, D, window, sinks,
+                      scale, _DTYPES[q.dtype], out.data_ptr(), res.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                      dv.data_ptr(), ws.data_ptr(), n, _stream(q.device))
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _rows(t):
+    """_strided of a packed [N, H, D] operand: (tensor, (pointer, token, head strides))."""
+    t, (p, _, st, sh) = _strided(t.detach().unsqueeze(0))
+    return t[0], (p, st, sh)
+
+
+def _starts(t, name):
+    """[nseq + 1] int32 device starts of packed sequences."""
+    if t.dim() != 1 or t.shape[0] < 1 or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be [sequences + 1] int32 or int64, got {tuple(t.shape)} {t.dtype}")
+    if t.dtype is torch.int64:
+        t = t.clamp(0, _MAX_INT).int()
+    return t.contiguous()
+
+
+@torch.compiler.disable
+def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, window=None, sinks=0, scale=None):
+    """Causal attention over packed sequences of different lengths, q [N, Hq, D] over k, v [M, Hkv, D] -> [N, Hq, D]: the
+    types, heads, mask, scale, autocast and derivatives of window_attention without its padding. Sequence b holds rows
+    cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 or int64 [sequences + 1], not falling). With cu_seqlens_k, k and v have
+    rows of their own for each sequence, and a sequence's queries are the last of its positions (the next piece of a text
+    whose earlier keys are at hand): row i of n is position i + m - n of m. Rows that see nothing (m < n, or outside every
+    sequence) and the gradients of rows that nothing sees are 0. The numbers stay on the device: they are not checked, a
+    call does not wait for them, and a captured call may be replayed with others. Capturing a backward raises while an
+    earlier graph of the same leaves, made by this function on another stream, is alive."""
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        q, k, v = (t.to(dt) if t.dtype is torch.float32 else t for t in (q, k, v))
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"q {tuple(q.shape)} must be [N, Hq, D], k {tuple(k.shape)} and v {tuple(v.shape)} [M, Hkv, D]")
+    _check_heads(q, k, v, "q, k and v")
+    if cu_seqlens_k is None and k.shape[0] != q.shape[0]:
+        raise ValueError(f"{q.shape[0]} rows of q and {k.shape[0]} of k ask for cu_seqlens_k")
+    if cu_seqlens_k is not None and cu_seqlens_k.shape != cu_seqlens.shape:
+        raise ValueError(f"cu_seqlens {tuple(cu_seqlens.shape)} and cu_seqlens_k {tuple(cu_seqlens_k.shape)} must have one "
+                         "shape")
+    window, sinks = _mask_args(window, sinks)
+    scale = _scale(scale, q.shape[2])
+    cu = _starts(cu_seqlens, "cu_seqlens")
+    cu_k = None if cu_seqlens_k is None else _starts(cu_seqlens_k, "cu_seqlens_k")
+    _check_same(q, ("k", k), ("v", v), ("cu_seqlens", cu), ("cu_seqlens_k", cu_k))
+    _check_tangents(q, k, v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out = _PackedAttention.apply(q, k, v, cu, cu_k, window, sinks, scale)
+        _mark_leaves(out, q.device)
+        return out
+    return _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, False)[3]
 
 
 def _cache(t, name):

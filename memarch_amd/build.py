@@ -1,5 +1,5 @@
-"""Build recipe for the HIP libraries `libmce.so` (loss head, pointer candidates, SwiGLU gate) and `libmce_attn.so`
-(attention), gfx950 only.
+"""Build recipe for the HIP libraries `libmce.so` (loss head, pointer candidates, SwiGLU gate), `libmce_attn.so`
+(attention) and `libmce_serve.so` (packed sequences, the 8-bit cache), gfx950 only.
 
 Run `python -m memarch_amd.build` (or `__graft_entry__.build()`). The libraries are written in-tree next to this file
 so that they travel with the source tree; they are plain C-ABI shared objects loaded through ctypes.
@@ -15,6 +15,8 @@ SRCS = [os.path.join(HERE, "csrc", f) for f in ("mce.hip", "induct.hip", "swiglu
 LIB = os.path.join(HERE, "libmce.so")
 ATTN_SRCS = [os.path.join(HERE, "csrc", f) for f in ("attn.hip", "paged.hip", "rope.hip")]
 ATTN_LIB = os.path.join(HERE, "libmce_attn.so")
+SERVE_SRCS = [os.path.join(HERE, "csrc", f) for f in ("packed.hip",)]
+SERVE_LIB = os.path.join(HERE, "libmce_serve.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 # -packed-fp32-ops off: hipcc may otherwise emit packed fp32 VALU ops on its own.
@@ -27,10 +29,11 @@ FLAGS = [
 
 
 def build(verbose=False):
-    """Compile both libraries from source every time it is called; raises CalledProcessError on failure. Returns the
+    """Compile the libraries from source every time it is called; raises CalledProcessError on failure. Returns the
     path of libmce.so."""
-    with ThreadPoolExecutor(2) as pool:
-        jobs = [pool.submit(_compile, srcs, lib, verbose) for srcs, lib in ((SRCS, LIB), (ATTN_SRCS, ATTN_LIB))]
+    with ThreadPoolExecutor(3) as pool:
+        jobs = [pool.submit(_compile, srcs, lib, verbose)
+                for srcs, lib in ((SRCS, LIB), (ATTN_SRCS, ATTN_LIB), (SERVE_SRCS, SERVE_LIB))]
         for job in jobs:
             job.result()
     return LIB
@@ -40,6 +43,12 @@ def build_attn(verbose=False):
     """Compile libmce_attn.so alone; returns its path."""
     _compile(ATTN_SRCS, ATTN_LIB, verbose)
     return ATTN_LIB
+
+
+def build_serve(verbose=False):
+    """Compile libmce_serve.so alone; returns its path."""
+    _compile(SERVE_SRCS, SERVE_LIB, verbose)
+    return SERVE_LIB
 
 
 def _compile(srcs, lib, verbose):

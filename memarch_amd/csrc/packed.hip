@@ -1,0 +1,197 @@
+// packed.hip — causal attention over packed sequences, forward and backward, for MI355X (gfx950): the host side. The C ABI
+// is in include/mce_pack.h, the kernels in attn_kernels.h (PK).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/mce_pack.h"
+#include "attn_host.h"
+#include "attn_kernels.h"
+
+namespace {
+
+using namespace attn;
+
+constexpr int64_t MAX_ROWS = int64_t(1) << 27;
+
+struct Plan {
+  int64_t uq, uk;           // units of rows of q and of keys
+  int n_sb, S_s, S_r;
+  int64_t part_s, part_r;   // floats of the parts
+};
+
+// How many workgroups may share a key block's rows (the kernels use fewer where its rows are few). Lengths are not known
+// here: key blocks are shared where there are too few of them to fill the GPU, blocks with first tokens of windowed
+// sequences, which every later row sees, until there are 2048 workgroups for them.
+Plan make_plan(int64_t nseq, int64_t N, int64_t M, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
+  Plan p = {N / BQ + nseq + 2, M / BKV + nseq + 2, 0, 1, 1, 0, 0};
+  if (window > 0 && window < M && sinks > 0) {
+    const int64_t most = M / BKV + 1, n = (sinks + BKV - 1) / BKV;
+    p.n_sb = (int)(n < most ? n : most);
+    const int64_t units = nseq * p.n_sb * Hkv;
+    int64_t s = units > 0 ? (2048 + units - 1) / units : 1;
+    p.S_s = (int)(s > 64 ? 64 : s);
+  }
+  const int64_t s = (1024 + p.uk * Hkv - 1) / (p.uk * Hkv);
+  p.S_r = (int)(s > 16 ? 16 : s);
+  p.part_s = p.S_s > 1 ? nseq * p.n_sb * Hkv * p.S_s * 2 * BKV * D : 0;
+  p.part_r = p.S_r > 1 ? p.uk * Hkv * p.S_r * 2 * BKV * D : 0;
+  return p;
+}
+
+int check_sizes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
+  if (nseq < 0 || N < 0 || M < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || D > 128 || D % 8 || window < 0 || sinks < 0)
+    return MCE_ATTN_EINVAL;
+  if (N > MAX_ROWS || M > MAX_ROWS || nseq > MAX_GROUPS || Hq * D > MAX_ST) return MCE_ATTN_EINVAL;
+  const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  // the sums are below 2^63: sinks' blocks are at most M / BKV + 1 per sequence
+  if (p.uq > MAX_GROUPS / Hq || p.uk * p.S_r > MAX_GROUPS / Hkv ||
+      nseq * p.n_sb * p.S_s > MAX_GROUPS / Hkv - p.uk * p.S_r)
+    return MCE_ATTN_EINVAL;
+  return MCE_ATTN_OK;
+}
+
+Args make_args(Strided q, Strided k, Strided v, const int32_t* cu, const int32_t* cu_k, int64_t nseq, int64_t N, int64_t M,
+               int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks, float scale, const Plan& p) {
+  Args a = {};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.cu = cu;
+  a.cu_k = cu_k == nullptr ? cu : cu_k;
+  a.nseq = (int)nseq;
+  a.B = 1;
+  a.T = (int)N;
+  a.M = (int)M;
+  a.uq = (int)p.uq;
+  a.uk = (int)p.uk;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.grp = (int)(Hq / Hkv);
+  a.D = (int)D;
+  a.window = window == 0 || window >= M ? INT32_MAX : (int)window;
+  a.sinks = a.window == INT32_MAX ? 0 : (int)(sinks > M ? M : sinks);
+  a.n_sb = p.n_sb;
+  a.S_s = p.S_s;
+  a.S_r = p.S_r;
+  a.scale = scale;
+  return a;
+}
+
+template <typename T, int DP>
+int launch_fwd(const Args& a, hipStream_t st) {
+  hipLaunchKernelGGL((k_attn_fwd<T, DP, true>), dim3((unsigned)(a.Hq * a.uq)), dim3(THREADS), 0, st, a);
+  return finish();
+}
+
+template <typename T, int DP>
+int launch_bwd(const Args& a, hipStream_t st) {
+  if (a.T > 0) {
+    hipLaunchKernelGGL((k_attn_dq<T, DP, true>), dim3((unsigned)(a.Hq * a.uq)), dim3(THREADS), 0, st, a);
+    const int rc = finish();
+    if (rc) return rc;
+  }
+  if (a.M == 0) return MCE_ATTN_OK;
+  const int64_t nsink = (int64_t)a.nseq * a.n_sb;
+  hipLaunchKernelGGL((k_attn_dkv<T, DP, true>), dim3((unsigned)(a.Hkv * (nsink * a.S_s + (int64_t)a.uk * a.S_r))),
+                     dim3(THREADS), 0, st, a);
+  const int64_t join = a.Hkv * ((a.S_s > 1 ? nsink : 0) + (a.S_r > 1 ? (int64_t)a.uk : 0));
+  const int pieces = (2 * BKV * (a.D / 4) + 255) / 256;
+  if (join > 0)
+    hipLaunchKernelGGL((k_attn_dkv_join<T, true>), dim3((unsigned)(join * pieces)), dim3(256), 0, st, a, pieces);
+  return finish();
+}
+
+}  // namespace
+
+thread_local int mce_attn_hip_error = 0;
+
+extern "C" {
+
+const char* mce_serve_error_string(int code) {
+  switch (code) {
+    case MCE_ATTN_OK: return "ok";
+    case MCE_ATTN_EINVAL: return "invalid argument (size, stride, head count, scale, element type or null pointer)";
+    case MCE_ATTN_EALIGN: return "misaligned (a pointer or a stride)";
+    case MCE_ATTN_EWORKSPACE: return "workspace missing, too small or not 256-byte aligned";
+    case MCE_ATTN_ELAUNCH: return "a HIP launch failed";
+    default: return "unknown error";
+  }
+}
+
+int mce_serve_last_hip_error(void) { return mce_attn_hip_error; }
+
+int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+                 int64_t v_st, int64_t v_sh, const int32_t* cu, const int32_t* cu_k, int64_t nseq, int64_t N, int64_t M,
+                 int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks, float scale, int dtype, void* out,
+                 void* res, float* lse, void* stream) {
+  int rc = check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks);
+  if (rc) return rc;
+  if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16) || (cu_k == nullptr && N != M))
+    return MCE_ATTN_EINVAL;
+  if (N == 0) return MCE_ATTN_OK;
+  if (cu == nullptr || out == nullptr || (rc = check_strided(q, 0, q_st, q_sh, D))) return rc ? rc : MCE_ATTN_EINVAL;
+  if (M > 0 && ((rc = check_strided(k, 0, k_st, k_sh, D)) || (rc = check_strided(v, 0, v_st, v_sh, D)))) return rc;
+  if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(res)) & 15) return MCE_ATTN_EALIGN;
+  Args a = make_args({static_cast<const uint16_t*>(q), 0, q_st, q_sh}, {static_cast<const uint16_t*>(k), 0, k_st, k_sh},
+                     {static_cast<const uint16_t*>(v), 0, v_st, v_sh}, cu, cu_k, nseq, N, M, Hq, Hkv, D, window, sinks,
+                     scale, make_plan(nseq, N, M, Hkv, D, window, sinks));
+  a.o = static_cast<uint16_t*>(out);
+  a.r = static_cast<uint16_t*>(res);
+  a.lse = lse;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == MCE_ATTN_BF16) return D <= 64 ? launch_fwd<__bf16, 64>(a, st) : launch_fwd<__bf16, 128>(a, st);
+  return D <= 64 ? launch_fwd<_Float16, 64>(a, st) : launch_fwd<_Float16, 128>(a, st);
+}
+
+size_t mce_pack_bwd_ws_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                             int64_t sinks) {
+  if (check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks)) return 0;
+  const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  return (size_t)(align256(N * Hq * 8) + align256(p.part_s * 4) + align256(p.part_r * 4));
+}
+
+int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+                 int64_t v_st, int64_t v_sh, const void* go, int64_t go_st, int64_t go_sh, const int32_t* cu,
+                 const int32_t* cu_k, int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
+                 int64_t window, int64_t sinks, float scale, int dtype, const void* out, const void* res,
+                 const float* lse, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks);
+  if (rc) return rc;
+  if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16) || (cu_k == nullptr && N != M))
+    return MCE_ATTN_EINVAL;
+  if (N == 0 && M == 0) return MCE_ATTN_OK;
+  if (cu == nullptr) return MCE_ATTN_EINVAL;
+  if (N > 0) {
+    if ((rc = check_strided(q, 0, q_st, q_sh, D)) || (rc = check_strided(go, 0, go_st, go_sh, D))) return rc;
+    if (out == nullptr || res == nullptr || lse == nullptr || dq == nullptr) return MCE_ATTN_EINVAL;
+  }
+  if (M > 0) {
+    if ((rc = check_strided(k, 0, k_st, k_sh, D)) || (rc = check_strided(v, 0, v_st, v_sh, D))) return rc;
+    if (dk == nullptr || dv == nullptr) return MCE_ATTN_EINVAL;
+  }
+  for (const void* p : {out, res, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return MCE_ATTN_EALIGN;
+  const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  const int64_t stat = align256(N * Hq * 8), part_s = align256(p.part_s * 4), part_r = align256(p.part_r * 4);
+  if (stat + part_s + part_r > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) ||
+                                     ws_bytes < (size_t)(stat + part_s + part_r)))
+    return MCE_ATTN_EWORKSPACE;
+  Args a = make_args({static_cast<const uint16_t*>(q), 0, q_st, q_sh}, {static_cast<const uint16_t*>(k), 0, k_st, k_sh},
+                     {static_cast<const uint16_t*>(v), 0, v_st, v_sh}, cu, cu_k, nseq, N, M, Hq, Hkv, D, window, sinks,
+                     scale, p);
+  a.go = {static_cast<const uint16_t*>(go), 0, go_st, go_sh};
+  a.out = static_cast<const uint16_t*>(out);
+  a.res = static_cast<const uint16_t*>(res);
+  a.lse = const_cast<float*>(lse);
+  a.stat = static_cast<float*>(ws);
+  a.part_s = a.stat + stat / 4;
+  a.part_r = a.part_s + part_s / 4;
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == MCE_ATTN_BF16) return D <= 64 ? launch_bwd<__bf16, 64>(a, st) : launch_bwd<__bf16, 128>(a, st);
+  return D <= 64 ? launch_bwd<_Float16, 64>(a, st) : launch_bwd<_Float16, 128>(a, st);
+}
+
+}  // extern "C"

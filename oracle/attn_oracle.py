@@ -97,6 +97,36 @@ def attention(q, k, v, window=0, sinks=0, lengths=None, scale=None, go=None, dty
     return tuple(res), tuple(tol)
 
 
+def packed(q, k, v, cu, cu_k=None, window=0, sinks=0, scale=None, go=None, dtype=None):
+    """attention() of packed sequences, q, go [N, Hq, D], k, v [M, Hkv, D]: each sequence alone, its queries as the last
+    rows of a square problem whose first rows have no weight. Rows outside every sequence: 0."""
+    cu = [min(max(int(x), 0), q.shape[0]) for x in cu]
+    cu_k = cu if cu_k is None else [min(max(int(x), 0), k.shape[0]) for x in cu_k]
+    like = (q, q, k, v)[:1 if go is None else 4]
+    res = tuple(torch.zeros(x.shape, dtype=torch.float64) for x in like)
+    tol = tuple(torch.zeros_like(x) for x in res)
+    for s in range(len(cu) - 1):
+        n, m = cu[s + 1] - cu[s], cu_k[s + 1] - cu_k[s]
+        if m == 0 or n == 0:
+            continue
+        use = min(n, m)
+        rows, keys = slice(cu[s + 1] - use, cu[s + 1]), slice(cu_k[s], cu_k[s + 1])
+        front = lambda x: torch.cat((x.new_zeros(m - use, *x.shape[1:]), x[rows]))[None]
+        r = attention(front(q), k[keys][None], v[keys][None], window, sinks, None, scale, None if go is None else front(go),
+                      dtype)
+        if dtype is None:
+            r = (((r,) if go is None else r), tol)
+        for to, part in zip((res, tol), r if dtype is not None else r[:1]):
+            for i, x in enumerate(part):
+                if i < 2:
+                    to[i][rows] = x[0, m - use:]
+                else:
+                    to[i][keys] = x[0]
+    if dtype is None:
+        return res[0] if go is None else res
+    return res, tol
+
+
 def paged(q, k_cache, v_cache, table, lengths, window=0, sinks=0, scale=None, dtype=None):
     """out [B, Hq, D] of q [B, Hq, D] over the pages of the caches; with dtype also its bound."""
     b, hq, d = q.shape
