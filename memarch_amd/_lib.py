@@ -98,6 +98,11 @@ SERVE_SIGNATURES = {
     "mce_pack_fwd": (_INT, 3 * _ROWS + [_P, _P] + 8 * [_I] + [_F, _INT, _P, _P, _P, _P]),
     "mce_pack_bwd_ws_bytes": (_S, 8 * [_I]),
     "mce_pack_bwd": (_INT, 4 * _ROWS + [_P, _P] + 8 * [_I] + [_F, _INT, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    # include/mce_cache.h
+    "mce_cache_write": (_INT, 2 * _ROWS + 2 * _TENSOR + [_P, _P, _P, _I, _P, _P] + 8 * [_I] + [_INT, _P]),
+    "mce_cache_read": (_INT, 2 * _TENSOR + [_P, _P, _P, _I, _P] + 8 * [_I] + [_INT, _P, _P, _P]),
+    "mce_cache_attn_ws_bytes": (_S, 8 * [_I]),
+    "mce_cache_attn": (_INT, [_P, _I, _I] + 2 * _TENSOR + [_P, _P, _P, _I, _P] + 10 * [_I] + [_F, _INT, _P, _P, _S, _P]),
 }
 
 _lib = None

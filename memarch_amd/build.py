@@ -15,7 +15,7 @@ SRCS = [os.path.join(HERE, "csrc", f) for f in ("mce.hip", "induct.hip", "swiglu
 LIB = os.path.join(HERE, "libmce.so")
 ATTN_SRCS = [os.path.join(HERE, "csrc", f) for f in ("attn.hip", "paged.hip", "rope.hip")]
 ATTN_LIB = os.path.join(HERE, "libmce_attn.so")
-SERVE_SRCS = [os.path.join(HERE, "csrc", f) for f in ("packed.hip",)]
+SERVE_SRCS = [os.path.join(HERE, "csrc", f) for f in ("packed.hip", "cache.hip", "cache_attn.hip")]
 SERVE_LIB = os.path.join(HERE, "libmce_serve.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 

@@ -9,6 +9,7 @@
 
 #include "attn_host.h"
 #include "attn_tile.h"
+#include "seq_find.h"
 
 namespace {
 
@@ -59,9 +60,7 @@ struct Args {
 // >= ceil(n / BLK), so that a unit finds its sequence from the starts alone, whatever the lengths, which the host need
 // not know; at most one unit per sequence is left over. Starts outside 0 .. rows count as the nearest of the two.
 __device__ __forceinline__ int start_of(const int32_t* cu, int nseq, int rows, int s) {
-  if (s == 0) return 0;
-  const int x = cu[(s <= nseq + 1 ? s : nseq + 1) - 1];
-  return s > nseq + 1 ? rows : (x < 0 ? 0 : (x > rows ? rows : x));
+  return s == 0 ? 0 : (s > nseq + 1 ? rows : start_in(cu, s - 1, rows));
 }
 struct Seq {
   int q0, k0;      // first rows
@@ -77,19 +76,10 @@ struct Seq {
     outside = s == 0 || s == a.nseq + 1;
   }
 };
-// The sequence of unit u, found by all 64 lanes at once: the last one whose first unit is not behind it.
+// The sequence of unit u.
 template <int BLK>
 __device__ __forceinline__ int seq_of(const int32_t* cu, int nseq, int rows, int u) {
-  const int lane = threadIdx.x & 63, n = nseq + 2;
-  int first = 0, step = 1;
-  while (step * 64 < n) step *= 64;
-  for (;; step /= 64) {
-    const int s = first + lane * step;
-    const bool at = s < n && start_of(cu, nseq, rows, s) / BLK + s <= u;
-    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at));
-    first += (c > 0 ? c - 1 : 0) * step;
-    if (step == 1) return __builtin_amdgcn_readfirstlane(first);
-  }
+  return last_from(nseq + 2, u, [&](int s) { return start_of(cu, nseq, rows, s) / BLK + s; });
 }
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) {

@@ -15,6 +15,7 @@
 #include "../../include/mce_paged.h"
 #include "attn_host.h"
 #include "attn_tile.h"
+#include "seq_find.h"
 
 namespace {
 
@@ -39,28 +40,6 @@ struct Args {
   float scale;
 };
 
-// The 32-key tiles that the last of n tokens sees: those of the first `sinks` positions, then those of the window.
-struct Seen {
-  int n, lo, n_sink, lo_tile, tiles;
-  __device__ __forceinline__ Seen(const Args& a, int b) {
-    n = a.lengths[b];
-    const int64_t cap = (int64_t)a.max_pages * a.page;
-    n = n < 0 ? 0 : (n > cap ? (int)cap : n);
-    lo = n - a.window;
-    lo = lo < 0 ? 0 : lo;
-    lo_tile = lo / BK;
-    n_sink = (a.sinks + BK - 1) / BK;
-    n_sink = n_sink < lo_tile ? n_sink : lo_tile;
-    tiles = n_sink + (n + BK - 1) / BK - lo_tile;
-  }
-  __device__ __forceinline__ int key0(int it) const { return (it < n_sink ? it : lo_tile + it - n_sink) * BK; }
-  // tiles per workgroup when they are shared among S, a multiple of the waves
-  __device__ __forceinline__ int run(int S) const {
-    const int r = ((tiles + S - 1) / S + NW - 1) / NW * NW;
-    return r < MIN_TILES ? MIN_TILES : r;
-  }
-};
-
 template <typename T, int DP>
 __global__ __launch_bounds__(THREADS, DP == 64 ? 2 : 1) void k_paged(Args a) {
   constexpr int IMG = BK * DP * 2, WAVE = 4 * IMG;     // a wave's LDS: K and V, two tiles each
@@ -70,8 +49,8 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 2 : 1) void k_paged(Args a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int s = blockIdx.x % a.S, unit = blockIdx.x / a.S;
   const int gi = unit % a.ng, hk = unit / a.ng % a.Hkv, b = unit / a.ng / a.Hkv;
-  const Seen sn(a, b);
-  const int run = sn.run(a.S), t0 = s * run;
+  const Seen<BK> sn(a, b);
+  const int run = sn.run<NW>(a.S, MIN_TILES), t0 = s * run;
   int t1 = t0 + run;
   t1 = t1 < sn.tiles ? t1 : sn.tiles;
   if (t0 >= sn.tiles && a.S > 1) return;               // the joining launch does not read this part
@@ -254,8 +233,8 @@ template <typename T>
 __global__ __launch_bounds__(64) void k_paged_join(Args a) {
   __shared__ float f[TARGET];
   const int64_t row = blockIdx.x;
-  const Seen sn(a, (int)(row / a.Hq));
-  const int run = sn.run(a.S), n = (sn.tiles + run - 1) / run, lane = threadIdx.x, d = lane * 2;
+  const Seen<BK> sn(a, (int)(row / a.Hq));
+  const int run = sn.run<NW>(a.S, MIN_TILES), n = (sn.tiles + run - 1) / run, lane = threadIdx.x, d = lane * 2;
   const float c = a.scale * LOG2E;
   const float* const ml = a.ml + row * a.S * 2;
   float mm = -INFINITY;
