@@ -129,7 +129,8 @@ __global__ __launch_bounds__(THREADS, NL <= 16 ? 4 : 2) void k_cache_write(Write
       u32x2 o = *p;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const f32x2 lo2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)o[e], false), hi2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)o[e], true);
+        const f32x2 lo2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)o[e], false);
+        const f32x2 hi2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)o[e], true);
         const int t = __builtin_amdgcn_cvt_pk_fp8_f32(lo2[0] * again, lo2[1] * again, 0, false);
         o[e] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi2[0] * again, hi2[1] * again, t, true);
       }
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(THREADS) void k_cache_read(ReadArgs a) {
   int pg = -1;
   uint32_t slot = 0;
   if (s > 0 && s <= a.B && j0 < (int64_t)g.max_pages * g.page) {
-    const uint32_t pi = Paged::div((uint32_t)j0 >> 3, g.mpage);
+    const uint32_t pi = g.page8((uint32_t)j0 >> 3);
     slot = j0 - pi * g.page;
     pg = g.table[(s - 1) * g.bt_sb + pi];
     if (pg >= g.pages) pg = -1;
@@ -213,7 +214,8 @@ __global__ __launch_bounds__(THREADS) void k_cache_read(ReadArgs a) {
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const f32x2 x = k ? __builtin_amdgcn_cvt_pk_f32_fp8((int)v[i][e], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)v[i][e], false);
+          const int c4 = (int)v[i][e];
+          const f32x2 x = k ? __builtin_amdgcn_cvt_pk_f32_fp8(c4, true) : __builtin_amdgcn_cvt_pk_f32_fp8(c4, false);
           float y = x[0] * f[i], z = x[1] * f[i];
           if (__is_same(T, _Float16)) {   // (a NaN stays one)
             y = y > 65504.f ? 65504.f : (y < -65504.f ? -65504.f : y);

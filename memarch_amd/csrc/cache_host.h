@@ -16,21 +16,26 @@ struct Codes {
   float* scale;
 };
 
+// x / d for x d < 2^32: the high word of x * ceil(2^32 / d), and x itself for d = 1, without a branch.
+struct Div {
+  uint32_t m, one;
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return __umulhi(x, m) + (x & one); }
+};
+inline Div div_by(int64_t d) {
+  return d == 1 ? Div{0, 0xFFFFFFFFu} : Div{(uint32_t)((uint64_t(1) << 32) / (uint64_t)d + 1), 0};
+}
+
 struct Paged {
   const int32_t* table;
   int64_t bt_sb;
   int pages, page, max_pages, Hkv, D;
   int per;                 // blocks per page
-  uint32_t mpage, mblock;  // of the divisions by page / 8 and block / 8 (0: by 1)
-  __device__ __forceinline__ static uint32_t div(uint32_t x, uint32_t magic) { return magic ? __umulhi(x, magic) : x; }
+  Div page8, block8;       // by page / 8 and block / 8
   // the scale of the 8 slots from slot8 * 8 on of page pg
   __device__ __forceinline__ int64_t scale_at(int pg, uint32_t slot8, int h) const {
-    return ((int64_t)pg * per + div(slot8, mblock)) * Hkv + h;
+    return ((int64_t)pg * per + block8(slot8)) * Hkv + h;
   }
 };
-
-// x / d = the high word of x * magic_of(d) while x d < 2^32 (d = 1: 0)
-inline uint32_t magic_of(int64_t d) { return d == 1 ? 0 : (uint32_t)((uint64_t(1) << 32) / (uint64_t)d + 1); }
 
 inline int check_paged_sizes(int64_t B, int64_t Hkv, int64_t D, int64_t pages, int64_t page, int64_t block,
                              int64_t max_pages, int64_t bt_sb) {
@@ -43,8 +48,11 @@ inline int check_paged_sizes(int64_t B, int64_t Hkv, int64_t D, int64_t pages, i
   return MCE_ATTN_OK;
 }
 
+// Page strides in units of 16 bytes stay in 31 bits.
+constexpr int64_t MAX_SP = int64_t(1) << 34;
+
 inline int check_codes(const void* p, int64_t sp, int64_t st, int64_t sh, const void* scale, int64_t D) {
-  if (p == nullptr || scale == nullptr || sp < 0 || sh < 0 || st < D || st > MAX_ST) return MCE_ATTN_EINVAL;
+  if (p == nullptr || scale == nullptr || sp < 0 || sp > MAX_SP || sh < 0 || st < D || st > MAX_ST) return MCE_ATTN_EINVAL;
   if ((reinterpret_cast<uintptr_t>(p) & 15) || (sp | st | sh) % 16 || (reinterpret_cast<uintptr_t>(scale) & 3))
     return MCE_ATTN_EALIGN;
   return MCE_ATTN_OK;
@@ -61,8 +69,8 @@ inline Paged make_paged(const int32_t* table, int64_t bt_sb, int64_t Hkv, int64_
   g.Hkv = (int)Hkv;
   g.D = (int)D;
   g.per = (int)(page / block);
-  g.mpage = magic_of(page / 8);
-  g.mblock = magic_of(block / 8);
+  g.page8 = div_by(page / 8);
+  g.block8 = div_by(block / 8);
   return g;
 }
 
