@@ -188,10 +188,13 @@ def _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, train):
     out = torch.empty(N, Hq, D, dtype=q.dtype, device=q.device)
     res = torch.empty_like(out) if train else None
     lse = torch.empty(Hq, N, dtype=torch.float32, device=q.device) if train else None
+    n = _lib.load_serve().mce_pack_plan_bytes(cu.shape[0] - 1, N, k.shape[0], Hq, k.shape[1], D, window, sinks)
+    plan = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     with _On(q.device):
         _lib.call("mce_pack_fwd", *qs, *ks, *vs, cu.data_ptr(), _ptr(cu_k), cu.shape[0] - 1, N, k.shape[0], Hq, k.shape[1],
-                  D, window, sinks, scale, _DTYPES[q.dtype], out.data_ptr(), _ptr(res), _ptr(lse), _stream(q.device))
-    return q, k, v, out, res, lse
+                  D, window, sinks, scale, _DTYPES[q.dtype], out.data_ptr(), _ptr(res), _ptr(lse), _ptr(plan), n,
+                  _stream(q.device))
+    return q, k, v, out, res, lse, plan
 
 
 def _mark_leaves(out, dev):
@@ -220,15 +223,15 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu, cu_k, window, sinks, scale):
-        q, k, v, out, res, lse = _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, True)
-        ctx.save_for_backward(q, k, v, out, res, lse, cu, cu_k)
+        q, k, v, out, res, lse, plan = _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, out, res, lse, plan, cu, cu_k)
         ctx.mask = (window, sinks, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        q, k, v, out, res, lse, cu, cu_k = ctx.saved_tensors
+        q, k, v, out, res, lse, plan, cu, cu_k = ctx.saved_tensors
         _check_capture(ctx, q.device)
         window, sinks, scale = ctx.mask
         (N, Hq, D), (M, Hkv, _) = q.shape, k.shape
@@ -241,15 +244,26 @@ class _PackedAttention(torch.autograd.Function):
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         with _On(q.device):
             _lib.call("mce_pack_bwd", *qs, *ks, *vs, *gs, cu.data_ptr(), _ptr(cu_k), nseq, N, M, Hq, Hkv, D, window, sinks,
-                      scale, _DTYPES[q.dtype], out.data_ptr(), res.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                      dv.data_ptr(), ws.data_ptr(), n, _stream(q.device))
+                      scale, _DTYPES[q.dtype], out.data_ptr(), res.data_ptr(), lse.data_ptr(), _ptr(plan), dq.data_ptr(),
+                      dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, _stream(q.device))
         return dq, dk, dv, None, None, None, None, None
 
 
 def _rows(t):
     """_strided of a packed [N, H, D] operand: (tensor, (pointer, token, head strides))."""
-    t, (p, _, st, sh) = _strided(t.detach().unsqueeze(0))
-    return t[0], (p, st, sh)
+    n, h, d = t.shape
+    st, sh, sd = t.stride()
+    if n < 2:
+        st = d
+    if h < 2:
+        sh = 0
+    at = t.data_ptr()
+    if sd != 1 or (st | sh) & 7 or not d <= st <= _MAX_STRIDE or at & 15:
+        t = t.detach().contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone()
+        at, st, sh = t.data_ptr(), h * d, d
+    return t, (at, st, sh)
 
 
 def _starts(t, name):

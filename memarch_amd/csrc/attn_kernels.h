@@ -50,6 +50,7 @@ struct Args {
   const int32_t *cu, *cu_k;  // starts of the nseq sequences in the rows of q and of k, and their ends
   int nseq, M;               // M: rows of k
   int uq, uk;                // units of BQ rows of q and of BKV rows of k
+  struct Unit* plan;         // those of q and then those of k, the longest first; null: in their own order
 };
 
 // Packed sequences: rows of different sequences lie behind each other, sequence s in rows cu[s] .. cu[s + 1] - 1 of q and
@@ -62,24 +63,46 @@ struct Args {
 __device__ __forceinline__ int start_of(const int32_t* cu, int nseq, int rows, int s) {
   return s == 0 ? 0 : (s > nseq + 1 ? rows : start_in(cu, s - 1, rows));
 }
-struct Seq {
+// A block of BQ rows of q or BKV rows of k: what its workgroup has to know of its sequence.
+struct Unit {
   int q0, k0;      // first rows
-  int lq, lk;      // rows of q and of k
-  bool outside;    // rows before the first sequence or behind the last: those of q and those of k have nothing in common
-  __device__ __forceinline__ Seq(const Args& a, int s) {
-    q0 = start_of(a.cu, a.nseq, a.T, s);
-    lq = start_of(a.cu, a.nseq, a.T, s + 1) - q0;
-    k0 = start_of(a.cu_k, a.nseq, a.M, s);
-    lk = start_of(a.cu_k, a.nseq, a.M, s + 1) - k0;
-    lq = lq < 0 ? 0 : lq;
-    lk = lk < 0 ? 0 : lk;
-    outside = s == 0 || s == a.nseq + 1;
-  }
+  int lq, lk;      // rows of q and of k (outside every sequence they have nothing in common: the other's are 0)
+  int blk;         // which of the sequence's blocks (below 0, where starts fall: none)
+  int outside;
+  int pad[2];
 };
-// The sequence of unit u.
-template <int BLK>
-__device__ __forceinline__ int seq_of(const int32_t* cu, int nseq, int rows, int u) {
-  return last_from(nseq + 2, u, [&](int s) { return start_of(cu, nseq, rows, s) / BLK + s; });
+template <bool KEYS>
+__device__ __forceinline__ Unit unit_of(const Args& a, int s, int u) {
+  Unit x;
+  x.q0 = start_of(a.cu, a.nseq, a.T, s);
+  x.lq = start_of(a.cu, a.nseq, a.T, s + 1) - x.q0;
+  x.k0 = start_of(a.cu_k, a.nseq, a.M, s);
+  x.lk = start_of(a.cu_k, a.nseq, a.M, s + 1) - x.k0;
+  x.outside = s == 0 || s == a.nseq + 1;
+  x.blk = u - (KEYS ? x.k0 / BKV : x.q0 / BQ) - s;
+  x.lq = x.lq < 0 || (KEYS && x.outside) ? 0 : x.lq;
+  x.lk = x.lk < 0 || (!KEYS && x.outside) ? 0 : x.lk;
+  return x;
+}
+// The u-th unit of the launch's order.
+template <bool KEYS>
+__device__ __forceinline__ Unit unit_at(const Args& a, int u) {
+  if (a.plan != nullptr) {
+    typedef const int __attribute__((address_space(4))) * Ints;
+    const Ints p = (Ints)(a.plan + (KEYS ? a.uq : 0) + u);
+    Unit x;
+    x.q0 = p[0];
+    x.k0 = p[1];
+    x.lq = p[2];
+    x.lk = p[3];
+    x.blk = p[4];
+    x.outside = p[5];
+    return x;
+  }
+  constexpr int BLK = KEYS ? BKV : BQ;
+  const int32_t* const cu = KEYS ? a.cu_k : a.cu;
+  const int rows = KEYS ? a.M : a.T;
+  return unit_of<KEYS>(a, last_from(a.nseq + 2, u, [&](int s) { return start_of(cu, a.nseq, rows, s) / BLK + s; }), u);
 }
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
@@ -95,17 +118,17 @@ template <bool PK>
 struct Rows {
   int q0, len, off, own;
   int64_t qrow, krow;   // first row of q and of k (packed)
+  __device__ __forceinline__ explicit Rows(const Unit& x) {
+    own = x.blk < 0 ? 0 : x.lq;
+    len = x.blk < 0 ? 0 : x.lk;
+    off = len - own;
+    qrow = x.q0;
+    krow = x.k0;
+    q0 = (x.blk < 0 ? 0 : x.blk) * BQ + off;
+  }
   __device__ __forceinline__ Rows(const Args& a, int b, int blk) {
     if constexpr (PK) {
-      const int s = seq_of<BQ>(a.cu, a.nseq, a.T, blk);
-      const Seq sq(a, s);
-      const int i = blk - sq.q0 / BQ - s;   // (below 0 where starts fall: nothing)
-      own = i < 0 ? 0 : sq.lq;
-      len = i < 0 || sq.outside ? 0 : sq.lk;
-      off = len - own;
-      qrow = sq.q0;
-      krow = sq.k0;
-      q0 = (i < 0 ? 0 : i) * BQ + off;
+      *this = Rows(unit_at<false>(a, blk));
     } else {
       q0 = blk * BQ;
       len = seq_len(a, b);
@@ -149,14 +172,15 @@ struct KeyTiles {
 // without a window the longest blocks of all the XCD's heads run first, so that none is left over at the end.
 struct Place {
   int b, hk, g, blk;   // sequence, key/value head, query head of its group, block (0: the longest without a window)
-  // n: blocks per head; sub: query heads of a group that are workgroups of their own (grp, or 1)
-  __device__ __forceinline__ Place(const Args& a, uint32_t bid, uint32_t n, uint32_t sub) {
+  // n: blocks per head; sub: query heads of a group that are workgroups of their own (grp, or 1); sorted: block 0 is the
+  // longest all the same
+  __device__ __forceinline__ Place(const Args& a, uint32_t bid, uint32_t n, uint32_t sub, bool sorted) {
     const uint32_t kv = (uint32_t)a.B * a.Hkv;
     const bool whole = kv % 8 == 0, heads = !whole && kv * sub % 8 == 0;
     const uint32_t units = heads ? kv * sub : kv, in = heads ? 1 : sub;   // units per XCD set, workgroups inside a unit
     const uint32_t x = whole || heads ? 8 : 1, xcd = bid % x, slot = bid / x, ux = units / x;
     uint32_t u, i;
-    if (a.window == INT32_MAX) {
+    if (sorted || a.window == INT32_MAX) {
       blk = slot / (ux * in);
       const uint32_t r = slot - blk * (ux * in);
       u = r / in;
@@ -219,9 +243,9 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) 
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];   // K and V, two tiles each
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int nq = PK ? a.uq : (a.T + BQ - 1) / BQ;
-  const Place pl(a, blockIdx.x, nq, a.grp);
+  const Place pl(a, blockIdx.x, nq, a.grp, PK && a.plan != nullptr);
   const int b = pl.b, hk = pl.hk, hq = hk * a.grp + pl.g, bh = b * a.Hq + hq;
-  const Rows<PK> at(a, b, nq - 1 - pl.blk);
+  const Rows<PK> at(a, b, PK && a.plan ? pl.blk : nq - 1 - pl.blk);
   const int len = at.len, q0 = at.q0, r0 = q0 + wave * 32, row = r0 + (lane & 31);
   f32x16 acc[DP / 32] = {};
   float m = -INFINITY, l = 0.f;
@@ -367,9 +391,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nq = PK ? a.uq : (a.T + BQ - 1) / BQ;
-  const Place pl(a, blockIdx.x, nq, a.grp);
+  const Place pl(a, blockIdx.x, nq, a.grp, PK && a.plan != nullptr);
   const int b = pl.b, hk = pl.hk, hq = hk * a.grp + pl.g, bh = b * a.Hq + hq;
-  const Rows<PK> at(a, b, nq - 1 - pl.blk);
+  const Rows<PK> at(a, b, PK && a.plan ? pl.blk : nq - 1 - pl.blk);
   const int len = at.len, q0 = at.q0, r0 = q0 + wave * 32;
   f32x16 acc[DP / 32] = {};
   float delta = 0.f, nl = -INFINITY, sum = 0.f;
@@ -526,39 +550,43 @@ struct Keys {
   int64_t qrow, krow;
   // blk: the block among those with first tokens, or among the others
   __device__ __forceinline__ Keys(const Args& a, int b, bool sink, int blk) {
-    skip = false;
     if constexpr (PK) {
-      int s;
-      if (sink) s = 1 + blk / a.n_sb;
-      else s = seq_of<BKV>(a.cu_k, a.nseq, a.M, blk);
-      const Seq sq(a, s);
-      own = sq.outside ? 0 : sq.lq;
-      len = sq.lk;
-      off = len - own;
-      qrow = sq.q0;
-      krow = sq.k0;
-      const int kblk = sink ? blk % a.n_sb : blk - sq.k0 / BKV - s;
-      kb0 = kblk * BKV;
-      skip = kblk < 0 || kb0 >= len || (!sink && kblk < a.n_sb && !sq.outside);
+      if (sink) {
+        Unit x = unit_of<true>(a, 1 + blk / a.n_sb, 0);
+        x.blk = blk % a.n_sb;
+        set(a, x, true);
+      } else {
+        set(a, unit_at<true>(a, blk), false);
+      }
     } else {
+      skip = false;
       kb0 = (sink ? blk : a.n_sb + blk) * BKV;
       len = seq_len(a, b);
       off = 0;
       own = a.T;
       qrow = krow = 0;
-    }
-    // rows kb0 .. q_end - 1 may see a key of the block
-    const int64_t q_end64 = kb0 < a.sinks ? len : (int64_t)kb0 + BKV - 1 + a.window;
-    const int q_end = q_end64 < len ? (int)q_end64 : len;
-    if constexpr (PK) {
-      const int first = kb0 - off;
-      t0 = (first < 0 ? 0 : first) / BR;
-      nt = (q_end - off + BR - 1) / BR - t0;
-      nt = q_end <= off || nt < 0 ? 0 : nt;
-    } else {
       t0 = kb0 / BR;
-      nt = (q_end + BR - 1) / BR - t0;
+      nt = (end_row(a) + BR - 1) / BR - t0;
     }
+  }
+  __device__ __forceinline__ Keys(const Args& a, const Unit& x) { set(a, x, false); }
+  __device__ __forceinline__ void set(const Args& a, const Unit& x, bool sink) {
+    own = x.lq;
+    len = x.lk;
+    off = len - own;
+    qrow = x.q0;
+    krow = x.k0;
+    kb0 = x.blk * BKV;
+    skip = x.blk < 0 || kb0 >= len || (!sink && x.blk < a.n_sb && !x.outside);
+    const int first = kb0 - off, end = end_row(a) - off;
+    t0 = (first < 0 ? 0 : first) / BR;
+    nt = (end + BR - 1) / BR - t0;
+    nt = end <= 0 || nt < 0 ? 0 : nt;
+  }
+  // rows kb0 .. end_row - 1 may see a key of the block
+  __device__ __forceinline__ int end_row(const Args& a) const {
+    const int64_t end = kb0 < a.sinks ? len : (int64_t)kb0 + BKV - 1 + a.window;
+    return end < len ? (int)end : len;
   }
   __device__ __forceinline__ int read() const { return PK ? own : len; }
   // workgroups that share the block
@@ -588,7 +616,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   const bool sink = blockIdx.x < sink_wgs;
   const uint32_t w = sink ? blockIdx.x : blockIdx.x - sink_wgs;
   const int S = sink ? a.S_s : a.S_r, nb = sink ? nsink : nr;
-  const Place pl(a, w, nb * S, 1);
+  const Place pl(a, w, nb * S, 1, PK && a.plan != nullptr && !sink);
   const int sp = pl.blk % S, blk = pl.blk / S, b = pl.b, hk = pl.hk, bh = b * a.Hkv + hk;
   const Keys<PK> at(a, b, sink, blk);
   const int len = at.len, kb0 = at.kb0, j0 = kb0 + wave * 32;

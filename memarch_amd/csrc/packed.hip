@@ -1,5 +1,5 @@
-// packed.hip — causal attention over packed sequences, forward and backward, for MI355X (gfx950): the host side. The C ABI
-// is in include/mce_pack.h, the kernels in attn_kernels.h (PK).
+// packed.hip — causal attention over packed sequences, forward and backward, for MI355X (gfx950): the order of the work and
+// the host side. The C ABI is in include/mce_pack.h, the attention's kernels in attn_kernels.h (PK).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -11,6 +11,100 @@ namespace {
 
 using namespace attn;
 
+// The units of packed sequences in the order in which they are taken, so that no long one is left over at the end (few queries
+// behind many keys, 8 pieces of 8192 rows over 139264 keys, 16 heads: 1370 us in their own order, with half of the workgroups
+// waiting for the longest from 60% of the time on). Without a window: the sequences with the most keys first, each one's
+// blocks together, from the longest on, as they share keys (taken by their own lengths from everywhere, 16 prompts of up to
+// 7491 tokens read all keys from HBM: 1531 us instead of 1463 in their own order). With a window: the longest blocks first,
+// few of which are shorter than the others and fill the end. Counting sorts by length in steps of 1/16, one workgroup for
+// the units of q and one for those of k; which of two alike comes first is open, and no result hangs on it.
+constexpr int PLAN_THREADS = 1024;
+template <bool KEYS>
+__device__ __forceinline__ void plan_units(const Args& a) {
+  constexpr int BLK = KEYS ? BKV : BQ, BUCKETS = 512;
+  __shared__ int count[BUCKETS], wsum[PLAN_THREADS / 64];
+  const int t = threadIdx.x, n = KEYS ? a.uk : a.uq, rows = KEYS ? a.M : a.T, seqs = a.nseq + 2;
+  const int32_t* const cu = KEYS ? a.cu_k : a.cu;
+  Unit* const out = a.plan + (KEYS ? a.uq : 0);
+  int* const place = reinterpret_cast<int*>(a.plan + a.uq + a.uk) + (KEYS ? seqs : 0);   // a sequence's first unit
+  const bool whole = a.window == INT32_MAX;
+  auto find = [&](int u, int* s) {
+    int lo = 0, hi = seqs;                             // the last s with its first unit not behind u
+    while (hi - lo > 1) {
+      const int m = (lo + hi) / 2;
+      if (start_of(cu, a.nseq, rows, m) / BLK + m <= u) lo = m;
+      else hi = m;
+    }
+    *s = lo;
+    return unit_of<KEYS>(a, lo, u);
+  };
+  auto blocks = [&](const Unit& x) { return ((KEYS ? x.lk : x.lq) + BLK - 1) / BLK; };
+  // 0: the longest; exponent and four bits behind it (lengths are below 2^28)
+  auto bucket = [&](int len) {
+    const int b = (int)(__builtin_bit_cast(uint32_t, (float)len) >> 19) - (127 << 4);
+    return BUCKETS - 1 - (b < 0 ? 0 : b);
+  };
+  auto tiles = [&](const Unit& x) {
+    if constexpr (KEYS) {
+      const Keys<true> at(a, x);
+      return at.skip ? 0 : at.nt + 1;
+    } else {
+      const Rows<true> at(x);
+      return at.any() ? KeyTiles(a, at.first(), at.last()).n + 1 : 1;
+    }
+  };
+  for (int i = t; i < BUCKETS; i += PLAN_THREADS) count[i] = 0;
+  // units that are left over have no block (nor those that nobody writes where starts fall)
+  for (int u = t; u < n; u += PLAN_THREADS) {
+    Unit x = {};
+    x.blk = -1;
+    out[u] = x;
+  }
+  __syncthreads();
+  if (whole) {
+    for (int s = t; s < seqs; s += PLAN_THREADS) {
+      const Unit x = unit_of<KEYS>(a, s, 0);
+      atomicAdd(&count[bucket(KEYS ? x.lq : x.lk)], blocks(x));
+    }
+  } else {
+    for (int u = t, s; u < n; u += PLAN_THREADS) {
+      const Unit x = find(u, &s);
+      if (x.blk < blocks(x)) atomicAdd(&count[bucket(tiles(x))], 1);
+    }
+  }
+  __syncthreads();
+  const int own = t < BUCKETS ? count[t] : 0;
+  int sum = own;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(sum, o);
+    sum += (t & 63) >= o ? up : 0;
+  }
+  if ((t & 63) == 63) wsum[t >> 6] = sum;
+  __syncthreads();
+  for (int w = 0; w < t >> 6; ++w) sum += wsum[w];
+  if (t < BUCKETS) count[t] = sum - own;
+  __syncthreads();
+  if (whole) {
+    for (int s = t; s < seqs; s += PLAN_THREADS) {
+      const Unit x = unit_of<KEYS>(a, s, 0);
+      place[s] = atomicAdd(&count[bucket(KEYS ? x.lq : x.lk)], blocks(x));
+    }
+    __syncthreads();
+  }
+  for (int u = t, s; u < n; u += PLAN_THREADS) {
+    const Unit x = find(u, &s);
+    const int nb = blocks(x);
+    if (x.blk < 0 || x.blk >= nb) continue;
+    const int to = whole ? place[s] + (KEYS ? x.blk : nb - 1 - x.blk) : atomicAdd(&count[bucket(tiles(x))], 1);
+    if ((unsigned)to < (unsigned)n) out[to] = x;       // (more than n blocks: where starts fall)
+  }
+}
+__global__ __launch_bounds__(PLAN_THREADS) void k_attn_plan(Args a) {
+  if (blockIdx.x == 0) plan_units<false>(a);
+  else plan_units<true>(a);
+}
+
+// -------------------------------------------------------------------------------------------------------- host side
 constexpr int64_t MAX_ROWS = int64_t(1) << 27;
 
 struct Plan {
@@ -77,8 +171,19 @@ Args make_args(Strided q, Strided k, Strided v, const int32_t* cu, const int32_t
   return a;
 }
 
+// Bytes of the plan: none where all workgroups of the forward run at once.
+int64_t plan_bytes_of(const Plan& p, int64_t Hq) {
+  const int64_t seqs = p.uq;   // (nseq + 2 of them at most)
+  return p.uq * Hq <= 512 ? 0 : (p.uq + p.uk) * (int64_t)sizeof(Unit) + 8 * seqs;
+}
+
 template <typename T, int DP>
 int launch_fwd(const Args& a, hipStream_t st) {
+  if (a.plan != nullptr) {
+    hipLaunchKernelGGL(k_attn_plan, dim3(a.r != nullptr ? 2 : 1), dim3(PLAN_THREADS), 0, st, a);
+    const int rc = finish();
+    if (rc) return rc;
+  }
   hipLaunchKernelGGL((k_attn_fwd<T, DP, true>), dim3((unsigned)(a.Hq * a.uq)), dim3(THREADS), 0, st, a);
   return finish();
 }
@@ -123,7 +228,7 @@ int mce_serve_last_hip_error(void) { return mce_attn_hip_error; }
 int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                  int64_t v_st, int64_t v_sh, const int32_t* cu, const int32_t* cu_k, int64_t nseq, int64_t N, int64_t M,
                  int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks, float scale, int dtype, void* out,
-                 void* res, float* lse, void* stream) {
+                 void* res, float* lse, void* plan, size_t plan_bytes, void* stream) {
   int rc = check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks);
   if (rc) return rc;
   if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16) || (cu_k == nullptr && N != M))
@@ -132,15 +237,26 @@ int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   if (cu == nullptr || out == nullptr || (rc = check_strided(q, 0, q_st, q_sh, D))) return rc ? rc : MCE_ATTN_EINVAL;
   if (M > 0 && ((rc = check_strided(k, 0, k_st, k_sh, D)) || (rc = check_strided(v, 0, v_st, v_sh, D)))) return rc;
   if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(res)) & 15) return MCE_ATTN_EALIGN;
+  const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  const int64_t need = plan_bytes_of(p, Hq);
+  if (need > 0 && (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 255) || plan_bytes < (size_t)need))
+    return MCE_ATTN_EWORKSPACE;
   Args a = make_args({static_cast<const uint16_t*>(q), 0, q_st, q_sh}, {static_cast<const uint16_t*>(k), 0, k_st, k_sh},
                      {static_cast<const uint16_t*>(v), 0, v_st, v_sh}, cu, cu_k, nseq, N, M, Hq, Hkv, D, window, sinks,
-                     scale, make_plan(nseq, N, M, Hkv, D, window, sinks));
+                     scale, p);
+  a.plan = need > 0 ? static_cast<Unit*>(plan) : nullptr;
   a.o = static_cast<uint16_t*>(out);
   a.r = static_cast<uint16_t*>(res);
   a.lse = lse;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dtype == MCE_ATTN_BF16) return D <= 64 ? launch_fwd<__bf16, 64>(a, st) : launch_fwd<__bf16, 128>(a, st);
   return D <= 64 ? launch_fwd<_Float16, 64>(a, st) : launch_fwd<_Float16, 128>(a, st);
+}
+
+size_t mce_pack_plan_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                           int64_t sinks) {
+  if (check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks) || N == 0) return 0;
+  return (size_t)plan_bytes_of(make_plan(nseq, N, M, Hkv, D, window, sinks), Hq);
 }
 
 size_t mce_pack_bwd_ws_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
@@ -154,7 +270,8 @@ int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
                  int64_t v_st, int64_t v_sh, const void* go, int64_t go_st, int64_t go_sh, const int32_t* cu,
                  const int32_t* cu_k, int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
                  int64_t window, int64_t sinks, float scale, int dtype, const void* out, const void* res,
-                 const float* lse, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream) {
+                 const float* lse, const void* plan, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes,
+                 void* stream) {
   int rc = check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks);
   if (rc) return rc;
   if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16) || (cu_k == nullptr && N != M))
@@ -172,6 +289,8 @@ int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   for (const void* p : {out, res, (const void*)dq, (const void*)dk, (const void*)dv})
     if (reinterpret_cast<uintptr_t>(p) & 15) return MCE_ATTN_EALIGN;
   const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  const bool planned = N > 0 && plan_bytes_of(p, Hq) > 0;
+  if (planned && (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 255))) return MCE_ATTN_EWORKSPACE;
   const int64_t stat = align256(N * Hq * 8), part_s = align256(p.part_s * 4), part_r = align256(p.part_r * 4);
   if (stat + part_s + part_r > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) ||
                                      ws_bytes < (size_t)(stat + part_s + part_r)))
@@ -179,6 +298,7 @@ int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   Args a = make_args({static_cast<const uint16_t*>(q), 0, q_st, q_sh}, {static_cast<const uint16_t*>(k), 0, k_st, k_sh},
                      {static_cast<const uint16_t*>(v), 0, v_st, v_sh}, cu, cu_k, nseq, N, M, Hq, Hkv, D, window, sinks,
                      scale, p);
+  a.plan = planned ? static_cast<Unit*>(const_cast<void*>(plan)) : nullptr;
   a.go = {static_cast<const uint16_t*>(go), 0, go_st, go_sh};
   a.out = static_cast<const uint16_t*>(out);
   a.res = static_cast<const uint16_t*>(res);

@@ -18,54 +18,63 @@ from .fused_ops import _ptr, _stream
 MAX_BLOCK = 128   # slots that share a scale
 
 
+_F8, _F32, _I32 = torch.float8_e4m3fn, torch.float32, torch.int32
+
+
 def _check_same(ref, *named):
     """All tensors on ref's GPU."""
+    dev = ref.device
     for name, t in named:
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
-    if not ref.is_cuda:
-        raise ValueError("memarch_amd.kv_cache runs on the GPU only; got a tensor on " + str(ref.device))
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if dev.type != "cuda":
+        raise ValueError("memarch_amd.kv_cache runs on the GPU only; got a tensor on " + str(dev))
 
 
-def _codes(cache, scale, name):
+def _codes(cache, scale, shape, name):
     """(pointer, byte strides of page, slot and head, scale's pointer) of a cache, which is read and written where it lies."""
-    pages, page, h, d = cache.shape
     sp, st, sh, sd = cache.stride()
-    sp, sh = sp if pages > 1 else 0, sh if h > 1 else 0
-    if cache.numel() and (sd != 1 or (sp | st | sh) & 15 or not d <= st <= _MAX_STRIDE or cache.data_ptr() & 15):
+    if shape[0] < 2:
+        sp = 0
+    if shape[2] < 2:
+        sh = 0
+    at = cache.data_ptr()
+    if (sd != 1 or (sp | st | sh | at) & 15 or not shape[3] <= st <= _MAX_STRIDE) and shape[0]:
         raise ValueError(f"{name} must have a contiguous last dimension, a 16-byte aligned base, strides that are multiples "
-                         f"of 16 and slots at least {d} elements apart, got strides {cache.stride()}")
+                         f"of 16 and slots at least {shape[3]} elements apart, got strides {cache.stride()}")
     if not scale.is_contiguous():
         raise ValueError(f"{name}'s scales must be contiguous")
-    return cache.data_ptr(), sp, st, sh, scale.data_ptr()
+    return at, sp, st, sh, scale.data_ptr()
 
 
 def _check_cache(k_cache, v_cache, k_scale, v_scale, block_table):
-    """The cache's sizes: pages, page, block, Hkv, D, max_pages, and the two caches' addresses."""
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.dim() != 4 or t.dtype is not torch.float8_e4m3fn:
-            raise ValueError(f"{name} must be float8_e4m3fn [pages, page, Hkv, D], got {tuple(t.shape)} {t.dtype}")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} must have one shape")
-    pages, page, h, d = k_cache.shape
+    """The cache's shape [pages, page, Hkv, D], its block and the table's max_pages."""
+    shape = k_cache.shape
+    if k_cache.dtype is not _F8 or v_cache.dtype is not _F8 or len(shape) != 4 or v_cache.dim() != 4:
+        raise ValueError("k_cache and v_cache must be float8_e4m3fn [pages, page, Hkv, D], got "
+                         f"{tuple(shape)} {k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
+    if v_cache.shape != shape:
+        raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(v_cache.shape)} must have one shape")
+    pages, page, h, d = shape
     if h < 1 or d % 16 or not 16 <= d <= MAX_HEAD_DIM:
         raise ValueError(f"the head dimension must be a multiple of 16 up to {MAX_HEAD_DIM}, got {h} heads of {d}")
     if page < 8 or page % 8 or page > 65536:
         raise ValueError(f"pages of {page} tokens are not supported (a multiple of 8 up to 65536 is)")
+    per = k_scale.shape[1] if k_scale.dim() == 3 else 0
+    want = (pages, per, h)
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dim() != 3 or t.dtype is not torch.float32 or t.shape[0] != pages or t.shape[2] != h or t.shape[1] < 1 or \
-                t.shape != k_scale.shape or page % t.shape[1]:
+        if t.dtype is not _F32 or t.shape != want or per < 1 or page % per:
             raise ValueError(f"{name} must be float32 [pages={pages}, page / block, Hkv={h}], alike for both, got "
                              f"{tuple(t.shape)} {t.dtype}")
-    block = page // k_scale.shape[1]
+    block = page // per
     if block < 8 or block % 8 or block > MAX_BLOCK:
         raise ValueError(f"blocks of {block} tokens are not supported (a multiple of 8 up to {MAX_BLOCK} is)")
-    if block_table.dim() != 2 or block_table.dtype is not torch.int32:
+    if block_table.dim() != 2 or block_table.dtype is not _I32:
         raise ValueError(f"block_table must be int32 [B, max_pages], got {tuple(block_table.shape)} {block_table.dtype}")
     most = block_table.shape[1]
     if most * page > min(2 ** 30, 2 ** 38 // page):
         raise ValueError(f"{most} pages of {page} tokens per sequence are not supported (2^30 tokens, 2^38 / page)")
-    return pages, page, block, h, d, most
+    return shape, block, most
 
 
 def _table(t):
@@ -77,7 +86,6 @@ def _table(t):
 
 
 @torch.compiler.disable
-@torch.no_grad()
 def cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lengths, cu_seqlens=None):
     """Writes the keys and values of new tokens, k and v [N, Hkv, D] (bf16 or fp16, any strides), into the cache in place.
     cu_seqlens [B + 1] (int32 or int64): rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 are the last tokens of sequence b, which
@@ -89,7 +97,8 @@ def cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lengths, 
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, Hkv, D]")
     if k.dtype not in _DTYPES or v.dtype != k.dtype:
         raise ValueError(f"k and v must both be bfloat16 or both float16, got {k.dtype} and {v.dtype}")
-    pages, page, block, h, d, most = _check_cache(k_cache, v_cache, k_scale, v_scale, block_table)
+    shape, block, most = _check_cache(k_cache, v_cache, k_scale, v_scale, block_table)
+    pages, page, h, d = shape
     if k.shape[1:] != (h, d):
         raise ValueError(f"k {tuple(k.shape)} does not fit a cache of {h} heads of {d}")
     B, N = block_table.shape[0], k.shape[0]
@@ -104,24 +113,23 @@ def cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lengths, 
     _check_same(k, ("v", v), ("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale),
                 ("block_table", block_table), ("lengths", lengths), ("cu_seqlens", cu))
     _check_tangents(k, v, k_cache, v_cache, k_scale, v_scale)
-    kc, vc = _codes(k_cache, k_scale, "k_cache"), _codes(v_cache, v_scale, "v_cache")
+    kc, vc = _codes(k_cache, k_scale, shape, "k_cache"), _codes(v_cache, v_scale, shape, "v_cache")
     (k, ks), (v, vs) = _rows(k), _rows(v)
     block_table, bt = _table(block_table)
     with _On(k.device):
         _lib.call("mce_cache_write", *ks, *vs, *kc[:4], *vc[:4], kc[4], vc[4], block_table.data_ptr(), bt,
                   lengths.data_ptr(), _ptr(cu), B, N, h, d, pages, page, block, most, _DTYPES[k.dtype], _stream(k.device))
-    for t in (k_cache, v_cache, k_scale, v_scale):   # they were changed, as by an operation in place
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+    # they were changed, as by an operation in place
+    torch.autograd.graph.increment_version([t for t in (k_cache, v_cache, k_scale, v_scale) if not t.is_inference()])
 
 
 @torch.compiler.disable
-@torch.no_grad()
 def cache_read(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, rows, dtype=torch.bfloat16):
     """The first tokens of each sequence out of the cache, (k, v) [rows, Hkv, D] of bf16 or fp16: token j of sequence b in
     row cu_seqlens[b] + j, up to cu_seqlens[b + 1] - 1 (int32 or int64 [B + 1]). packed_attention takes them with
     cu_seqlens_k = cu_seqlens. Rows outside every sequence, and tokens whose page is outside the cache, are 0."""
-    pages, page, block, h, d, most = _check_cache(k_cache, v_cache, k_scale, v_scale, block_table)
+    shape, block, most = _check_cache(k_cache, v_cache, k_scale, v_scale, block_table)
+    pages, page, h, d = shape
     if dtype not in _DTYPES:
         raise ValueError(f"dtype must be bfloat16 or float16, got {dtype}")
     rows = int(rows)
@@ -134,7 +142,7 @@ def cache_read(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, rows
     _check_same(k_cache, ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale), ("block_table", block_table),
                 ("cu_seqlens", cu))
     _check_tangents(k_cache, v_cache, k_scale, v_scale)
-    kc, vc = _codes(k_cache, k_scale, "k_cache"), _codes(v_cache, v_scale, "v_cache")
+    kc, vc = _codes(k_cache, k_scale, shape, "k_cache"), _codes(v_cache, v_scale, shape, "v_cache")
     block_table, bt = _table(block_table)
     k = torch.empty(rows, h, d, dtype=dtype, device=k_cache.device)
     v = torch.empty_like(k)
@@ -145,13 +153,13 @@ def cache_read(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, rows
 
 
 @torch.compiler.disable
-@torch.no_grad()
 def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, window=None, sinks=0, scale=None):
     """paged_attention over the 8-bit cache: attention of one new token per sequence, q [B, Hq, D] (bf16 or fp16, Hq a
     multiple of Hkv) -> [B, Hq, D]. lengths [B] (int32 or int64) counts a sequence's tokens with the new one, which
     cache_write has put there. The mask is that of window_attention's last row. A sequence of length 0 gives 0; tokens in
     pages outside the cache (entries of -1, say) and past max_pages are not seen."""
-    pages, page, block, h, d, most = _check_cache(k_cache, v_cache, k_scale, v_scale, block_table)
+    shape, block, most = _check_cache(k_cache, v_cache, k_scale, v_scale, block_table)
+    pages, page, h, d = shape
     if q.dim() != 3 or q.shape[2] != d or q.shape[1] < 1 or q.shape[1] % h:
         raise ValueError(f"q {tuple(q.shape)} must be [B, Hq, {d}], Hq a multiple of {h}")
     if q.dtype not in _DTYPES:
@@ -167,12 +175,12 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths,
     _check_same(q, ("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale),
                 ("block_table", block_table), ("lengths", lengths))
     _check_tangents(q, k_cache, v_cache, k_scale, v_scale)
-    kc, vc = _codes(k_cache, k_scale, "k_cache"), _codes(v_cache, v_scale, "v_cache")
+    kc, vc = _codes(k_cache, k_scale, shape, "k_cache"), _codes(v_cache, v_scale, shape, "v_cache")
     block_table, bt = _table(block_table)
     sb, sh, sd = q.stride()
     sb, sh = sb if B > 1 else 0, sh if Hq > 1 else d
     if sd != 1 or (sb | sh) & 7 or not d <= sh <= _MAX_STRIDE or q.data_ptr() & 15:
-        q = q.contiguous()
+        q = q.detach().contiguous()
         if q.data_ptr() & 15:
             q = q.clone()
         sb, sh = Hq * d, d

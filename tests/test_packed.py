@@ -176,9 +176,9 @@ def test_pack_c_abi_checks_need_no_gpu(lib):
     p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 256
 
     def fwd(q=p, st=64, sh=64, k=p, cu=p, cu_k=p, nseq=2, N=8, M=9, Hq=2, Hkv=1, D=64, window=0, sinks=0, scale=0.1, dtype=1,
-            out=p, res=None):
+            out=p, res=None, plan=None, nb=0):
         return lib.mce_pack_fwd(q, st, sh, k, 64, 64, p, 64, 64, cu, cu_k, nseq, N, M, Hq, Hkv, D, window, sinks, scale,
-                                dtype, out, res, None, None)
+                                dtype, out, res, None, plan, nb, None)
 
     for kw in (dict(N=-1), dict(M=-1), dict(nseq=-1), dict(Hq=3, Hkv=2), dict(Hkv=0), dict(D=60), dict(D=136), dict(D=0),
                dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(dtype=0), dict(q=None),
@@ -189,13 +189,19 @@ def test_pack_c_abi_checks_need_no_gpu(lib):
     for kw in (dict(q=p + 2), dict(out=p + 8), dict(res=p + 4), dict(st=68), dict(sh=4)):
         assert fwd(**kw) == 2, kw
     assert fwd(N=0, q=None, out=None, cu=None) == 0
+    plan = lib.mce_pack_plan_bytes(2, 8000, 9000, 64, 1, 64, 0, 0)
+    assert plan > 0 and lib.mce_pack_plan_bytes(2, 8, 9, 2, 1, 64, 0, 0) == 0
+    big = dict(N=8000, M=9000, Hq=64)
+    assert fwd(**big) == 3 and fwd(**big, plan=p, nb=plan - 1) == 3 and fwd(**big, plan=p + 16, nb=plan) == 3
 
     need = lib.mce_pack_bwd_ws_bytes(2, 8, 9, 2, 1, 64, 0, 0)
     assert need >= 2 * 2 * 8 * 4 and lib.mce_pack_bwd_ws_bytes(2, 8, 9, 3, 2, 64, 0, 0) == 0
 
-    def bwd(ws=p, nb=need, go=p, lse=p, dq=p, dk=p, st=64, N=8, M=9):
-        return lib.mce_pack_bwd(p, 64, 64, p, 64, 64, p, 64, 64, go, st, 64, p, p, 2, N, M, 2, 1, 64, 0, 0, 0.1, 1, p, p, lse,
-                                dq, dk, p, ws, nb, None)
+    def bwd(ws=p, nb=need, go=p, lse=p, dq=p, dk=p, st=64, N=8, M=9, Hq=2, plan=None):
+        return lib.mce_pack_bwd(p, 64, 64, p, 64, 64, p, 64, 64, go, st, 64, p, p, 2, N, M, Hq, 1, 64, 0, 0, 0.1, 1, p, p, lse,
+                                plan, dq, dk, p, ws, nb, None)
+
+    assert bwd(**big) == 3 and bwd(**big, plan=p + 16) == 3   # the forward's plan is missing
 
     assert bwd(ws=None) == 3 and bwd(nb=need - 1) == 3 and bwd(ws=p + 16) == 3
     assert bwd(go=None) == 1 and bwd(lse=None) == 1 and bwd(dq=None) == 1 and bwd(dk=None) == 1 and bwd(st=8) == 1
