@@ -12,7 +12,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int WAVES = 4;   // waves per workgroup; each works alone
+constexpr int WAVES = 4;   // waves per workgroup
 constexpr int THREADS = 64 * WAVES;
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -56,16 +56,20 @@ __device__ __forceinline__ int codes2(float x, float y, float f, int w) {
 }
 
 // A wave takes the new tokens of one block, one head, of the keys or the values: they stay in registers between the
-// largest magnitude and the rounding (NL loads of 64 pieces of 8 elements), so that memory is passed once. Earlier codes
-// are read only when the scale grows. Sequence b's blocks are the units from floor(cu[b] / block) + 2 b on: n tokens
-// touch at most floor(n / block) + 2 blocks.
-template <typename T, int DP, int NL>
-__global__ __launch_bounds__(THREADS, NL <= 16 ? 4 : 2) void k_cache_write(WriteArgs a) {
+// largest magnitude and the rounding (NL loads of 64 pieces of 8 elements), so that memory is passed once. Large blocks
+// are shared by a workgroup's waves (SPLIT): as one wave each they left the GPU short of waves (20011 tokens, 2 heads of
+// 96, blocks of 128: 12.1 us, 10.1 so). Earlier codes are read only when the scale grows. Sequence b's blocks are the units
+// from floor(cu[b] / block) + 2 b on: n tokens touch at most floor(n / block) + 2 blocks.
+// Bound by HBM: 65536 tokens, 8 heads of 128, blocks of 32, 403 MB: 74 us, 5.5 TB/s.
+// ONCE: the new rows are read past the caches.
+template <typename T, int DP, int NL, bool SPLIT, bool ONCE>
+__global__ __launch_bounds__(THREADS, 4) void k_cache_write(WriteArgs a) {
   constexpr int CH = DP / 8, RPI = 64 / CH;   // pieces per row, rows per load
-  const int lane = threadIdx.x & 63;
-  const int64_t w64 = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+  __shared__ uint32_t most[WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t w64 = SPLIT ? blockIdx.x : (int64_t)blockIdx.x * WAVES + wave;
   if (w64 >= a.waves) return;
-  const uint32_t w = __builtin_amdgcn_readfirstlane((uint32_t)w64);
+  const uint32_t w = (uint32_t)w64;
   const Paged& g = a.g;
   const int h = w % g.Hkv, which = w / g.Hkv & 1, u = w / g.Hkv >> 1;
   int b = u, first = u, fresh = 1, i = 0;
@@ -88,22 +92,34 @@ __global__ __launch_bounds__(THREADS, NL <= 16 ? 4 : 2) void k_cache_write(Write
   const Codes& c = which ? a.c[1] : a.c[0];
   float* const scale = c.scale + g.scale_at(pg, slot >> 3, h);
   const float old = had > 0 ? *scale : 0.f;
-  const int row = lane / CH, col = lane % CH * 8;
+  const int row = lane / CH, col = lane % CH * 8, j0 = SPLIT ? wave * NL : 0;
   const bool ok = col < g.D;
   const i32x4 r = make_rsrc(x.p + (first + (int64_t)(lo - p0)) * x.st + h * x.sh, (int)((cnt - 1) * x.st + g.D) * 2);
   u32x4 v[NL];
 #pragma unroll
   for (int j = 0; j < NL; ++j) {
     v[j] = u32x4{};
-    if (j * RPI < cnt) v[j] = load16(r, ok ? (j * RPI + row) * (int)x.st * 2 + col * 2 : OOB);
+    const int o = ok ? ((j0 + j) * RPI + row) * (int)x.st * 2 + col * 2 : OOB;
+    if ((j0 + j) * RPI < cnt) v[j] = __builtin_bit_cast(u32x4, attn_buffer_load16(r, o, 0, ONCE ? 2 : 0));
   }
   uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < NL; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = max2(m, v[j][e] & 0x7FFF7FFFu);
-  for (int o = 32; o > 0; o >>= 1) m = max2(m, __shfl_xor(m, o));
-  m = max2(m, m >> 16) & 0xFFFFu;
+  // over the wave's lanes, and the waves that share the block
+  auto share = [&](uint32_t x) {
+    for (int o = 32; o > 0; o >>= 1) x = max2(x, __shfl_xor(x, o));
+    x = max2(x, x >> 16) & 0xFFFFu;
+    if constexpr (SPLIT) {
+      most[wave] = x;
+      __syncthreads();
+      x = max2(max2(most[0], most[1]), max2(most[2], most[3]));
+      __syncthreads();
+    }
+    return x;
+  };
+  m = share(m);
   if (m >= inf_bits<T>()) {   // some element is not finite: the others' largest
     m = 0;
 #pragma unroll
@@ -114,16 +130,13 @@ __global__ __launch_bounds__(THREADS, NL <= 16 ? 4 : 2) void k_cache_write(Write
         m = l < inf_bits<T>() && l > m ? l : m;
         m = t < inf_bits<T>() && t > m ? t : m;
       }
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint32_t t = __shfl_xor(m, o);
-      m = t > m ? t : m;
-    }
+    m = share(m);
   }
   const float s = fmaxf(scale_for(lo_f32<T>(m)), old), f = 1.f / s;
   uint8_t* const out = c.p + (int64_t)pg * c.sp + (int64_t)slot * c.st + h * c.sh;
   if (old > 0.f && s > old) {   // (a scale that is no positive number has codes that mean nothing)
     const float again = old / s;
-    for (int j = 0; j < had; j += RPI) {
+    for (int j = SPLIT ? wave * RPI : 0; j < had; j += SPLIT ? WAVES * RPI : RPI) {
       if (j + row >= had || !ok) continue;
       u32x2* const p = reinterpret_cast<u32x2*>(out + (int64_t)(j + row) * c.st + col);
       u32x2 o = *p;
@@ -137,17 +150,17 @@ __global__ __launch_bounds__(THREADS, NL <= 16 ? 4 : 2) void k_cache_write(Write
       *p = o;
     }
   }
-  if (lane == 0) *scale = s;
+  if (lane == 0 && j0 == 0) *scale = s;
 #pragma unroll
   for (int j = 0; j < NL; ++j) {
-    if (j * RPI + row >= cnt || !ok) continue;
+    if ((j0 + j) * RPI + row >= cnt || !ok) continue;
     u32x2 o;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t p = v[j][2 * e], q = v[j][2 * e + 1];
       o[e] = (uint32_t)codes2<true>(lo_f32<T>(q), hi_f32<T>(q), f, codes2<false>(lo_f32<T>(p), hi_f32<T>(p), f, 0));
     }
-    *reinterpret_cast<u32x2*>(out + (int64_t)(had + j * RPI + row) * c.st + col) = o;
+    *reinterpret_cast<u32x2*>(out + (int64_t)(had + (j0 + j) * RPI + row) * c.st + col) = o;
   }
 }
 
@@ -166,8 +179,10 @@ constexpr int HEADS = 4;   // loads of 16 bytes per lane under way at once
 
 // A wave takes 8 neighbouring tokens (which lie in one page) of the keys or the values, and some of the heads: 16 codes per
 // lane and load, whole 128-byte lines on both sides. Rows before the first sequence and behind the last are taken as
-// sequences without pages, so every row is written. Sequence s's groups are the units from floor(start / 8) + s on.
-template <typename T, int DP>
+// sequences without pages, so every row is written. Bound by HBM: 98304 tokens, 8 heads of 128, 604 MB: 132 us, 4.6 TB/s, two
+// thirds of it writes. Sequence s's groups are the units from floor(start / 8) + s on.
+// ONCE: the results are written past the caches.
+template <typename T, int DP, bool ONCE>
 __global__ __launch_bounds__(THREADS) void k_cache_read(ReadArgs a) {
   constexpr int CH = DP / 16, HPL = 64 / (8 * CH);   // pieces per head, heads per load
   const int lane = threadIdx.x & 63;
@@ -224,32 +239,53 @@ __global__ __launch_bounds__(THREADS) void k_cache_read(ReadArgs a) {
           o[e / 2][e % 2 * 2 + k] = pack2<T>(y, z);
         }
       u32x4* const to = reinterpret_cast<u32x4*>(out + ((int64_t)(first + j0 + t) * g.Hkv + h) * g.D + col);
-      to[0] = o[0];
-      to[1] = o[1];
+      if constexpr (ONCE) {
+        __builtin_nontemporal_store(o[0], to);
+        __builtin_nontemporal_store(o[1], to + 1);
+      } else {
+        to[0] = o[0];
+        to[1] = o[1];
+      }
     }
   }
 }
 
 // --------------------------------------------------------------------------------------------------------- host side
 
-template <typename T, int DP>
-int launch_write(const WriteArgs& a, hipStream_t st) {
+// So many bytes of new rows are read, and of results written, past the caches (loads and stores of the non-temporal kind):
+// with their lines and those of what was there before, the last cache (256 MiB) would not keep them for the next kernel.
+// 65536 tokens written and 98304 read back, 8 heads of 128: 227 us without, 214 with the results past them, 217 with the
+// rows, 201 with both; 20011 and 120014, 2 heads of 96: 53 and 42 (the results).
+constexpr int64_t LARGE_BYTES = int64_t(1) << 26;
+
+template <typename T, int DP, bool ONCE>
+void start_write(const WriteArgs& a, hipStream_t st) {
   constexpr int RPI = 512 / DP;
   // one new token per sequence needs one load, whatever the block
   const int rows = a.cu == nullptr ? 1 : a.block, nl = (rows + RPI - 1) / RPI;
-  const dim3 grid((unsigned)((a.waves + WAVES - 1) / WAVES)), threads(THREADS);
-  if (nl <= 1) hipLaunchKernelGGL((k_cache_write<T, DP, 1>), grid, threads, 0, st, a);
-  else if (nl <= 2) hipLaunchKernelGGL((k_cache_write<T, DP, 2>), grid, threads, 0, st, a);
-  else if (nl <= 4) hipLaunchKernelGGL((k_cache_write<T, DP, 4>), grid, threads, 0, st, a);
-  else if (nl <= 8) hipLaunchKernelGGL((k_cache_write<T, DP, 8>), grid, threads, 0, st, a);
-  else if (nl <= 16) hipLaunchKernelGGL((k_cache_write<T, DP, 16>), grid, threads, 0, st, a);
-  else if constexpr (DP == 128) hipLaunchKernelGGL((k_cache_write<T, 128, 32>), grid, threads, 0, st, a);
+  const dim3 grid((unsigned)((a.waves + WAVES - 1) / WAVES)), threads(THREADS), each((unsigned)a.waves);
+  if (nl <= 1) hipLaunchKernelGGL((k_cache_write<T, DP, 1, false, ONCE>), grid, threads, 0, st, a);
+  else if (nl <= 2) hipLaunchKernelGGL((k_cache_write<T, DP, 2, false, ONCE>), grid, threads, 0, st, a);
+  else if (nl <= 4) hipLaunchKernelGGL((k_cache_write<T, DP, 4, false, ONCE>), grid, threads, 0, st, a);
+  else if (nl <= 8) hipLaunchKernelGGL((k_cache_write<T, DP, 8, false, ONCE>), grid, threads, 0, st, a);
+  else if (nl <= 16) hipLaunchKernelGGL((k_cache_write<T, DP, 4, true, ONCE>), each, threads, 0, st, a);
+  else if constexpr (DP == 128) hipLaunchKernelGGL((k_cache_write<T, 128, 8, true, ONCE>), each, threads, 0, st, a);
+}
+
+template <typename T, int DP>
+int launch_write(const WriteArgs& a, hipStream_t st) {
+  if ((int64_t)4 * a.N * a.g.Hkv * a.g.D >= LARGE_BYTES) start_write<T, DP, true>(a, st);
+  else start_write<T, DP, false>(a, st);
   return finish();
 }
 
 template <typename T, int DP>
 int launch_read(const ReadArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((k_cache_read<T, DP>), dim3((unsigned)((a.waves + WAVES - 1) / WAVES)), dim3(THREADS), 0, st, a);
+  const dim3 grid((unsigned)((a.waves + WAVES - 1) / WAVES)), threads(THREADS);
+  if ((int64_t)4 * a.rows * a.g.Hkv * a.g.D >= LARGE_BYTES)
+    hipLaunchKernelGGL((k_cache_read<T, DP, true>), grid, threads, 0, st, a);
+  else
+    hipLaunchKernelGGL((k_cache_read<T, DP, false>), grid, threads, 0, st, a);
   return finish();
 }
 
@@ -268,7 +304,7 @@ int mce_cache_write(const void* k, int64_t k_st, int64_t k_sh, const void* v, in
   if (rc) return rc;
   if (N < 0 || N > (int64_t(1) << 27) || (cu == nullptr && N != B) || !good_dtype(dtype)) return MCE_ATTN_EINVAL;
   const int64_t units = cu == nullptr ? B : N / block + 2 * B, waves = units * 2 * Hkv;
-  if (waves > MAX_GROUPS * WAVES) return MCE_ATTN_EINVAL;
+  if (waves > MAX_GROUPS) return MCE_ATTN_EINVAL;
   if (B == 0 || N == 0 || pages == 0 || max_pages == 0) return MCE_ATTN_OK;
   if (lengths == nullptr || block_table == nullptr) return MCE_ATTN_EINVAL;
   if ((rc = check_strided(k, 0, k_st, k_sh, D)) || (rc = check_strided(v, 0, v_st, v_sh, D)) ||

@@ -170,6 +170,33 @@ def test_pages_that_are_not_the_caches():
         assert torch.equal(got[i].double().cpu(), orc.read(orc.values(*want[i]), c.table, back, 130).to(BF).double())
 
 
+@pytest.mark.parametrize("d,page,block", [(128, 64, 16), (64, 128, 128)])
+def test_large_batches(d, page, block):
+    """64 MiB of rows and more are read, and of results written, past the caches: the same codes, scales and values as in
+    pieces that are not."""
+    from memarch_amd.kv_cache import cache_read, cache_write
+    n, hkv = 2 ** 17, 256 // d                       # 128 MiB of keys and values
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(n, hkv, d, generator=g, device="cuda").to(BF) for _ in range(2))
+    table = torch.randperm(n // page, generator=torch.Generator().manual_seed(1)).int().cuda()[None]
+    new = lambda: [torch.zeros(n // page, page, hkv, d, dtype=torch.uint8, device="cuda").view(F8) for _ in range(2)] + \
+        [torch.zeros(n // page, page // block, hkv, device="cuda") for _ in range(2)]
+    once, parts = new(), new()
+    cu = lambda m: torch.tensor([0, m], device="cuda")
+    cache_write(k, v, *once, table, torch.tensor([n]).cuda(), cu(n))
+    for i in range(0, n, n // 8):
+        cache_write(k[i:i + n // 8], v[i:i + n // 8], *parts, table, torch.tensor([i + n // 8]).cuda(), cu(n // 8))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(once[:2], parts[:2]))
+    assert all(torch.equal(a, b) and a.min() > 0 for a, b in zip(once[2:], parts[2:]))
+    got = cache_read(*once, table, cu(n), n)
+    for x, c, s, src in zip(got, once[:2], once[2:], (k, v)):
+        want = (c.float() * s.repeat_interleave(block, 1)[..., None])[table[0].long()].flatten(0, 1).to(BF)
+        assert torch.equal(x, want)
+        assert ((x.float() - src.float()).abs() <= src.float().abs() * 2.0 ** -4 + 2.0 ** -10 * s.max()).all()
+    few = cache_read(*once, table, cu(n // 8), n // 8)
+    assert torch.equal(few[0], got[0][:n // 8]) and torch.equal(few[1], got[1][:n // 8])
+
+
 def test_nothing_to_write():
     from memarch_amd.kv_cache import cache_attention, cache_read, cache_write
     c = Cache(2, 1, 2, 64, 16, 16)
