@@ -34,7 +34,7 @@ MCE_SERVE_API const char* mce_serve_error_string(int code);
 MCE_SERVE_API int mce_serve_last_hip_error(void);
 
 /* out, and for a backward (both may be NULL) res and lse, as in mce_attn_fwd. The plan, scratch memory of the forward, is the
- * order in which blocks of rows are taken, the longest first (0 bytes where all run at once); a backward takes the plan of
+ * order in which blocks of rows are taken, the longest first (0 bytes where their own order is as good); a backward takes the plan of
  * its forward, unchanged, which res asks for. */
 MCE_SERVE_API size_t mce_pack_plan_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
                                          int64_t window, int64_t sinks);

@@ -12,10 +12,10 @@ namespace {
 using namespace attn;
 
 // The units of packed sequences in the order in which they are taken, so that no long one is left over at the end (few queries
-// behind many keys, 8 pieces of 8192 rows over 139264 keys, 16 heads: 1370 us in their own order, with half of the workgroups
-// waiting for the longest from 60% of the time on). Without a window: the sequences with the most keys first, each one's
+// behind many keys, 8 pieces of 8192 rows over 139264 keys, 16 heads: 1206 us in their own order, half of the workgroups gone
+// from 60% of the time on; 1147 in this). Without a window: the sequences with the most keys first, each one's
 // blocks together, from the longest on, as they share keys (taken by their own lengths from everywhere, 16 prompts of up to
-// 7491 tokens read all keys from HBM: 1531 us instead of 1463 in their own order). With a window: the longest blocks first,
+// 7491 tokens read all keys from HBM: 1531 us, 1466 so). With a window: the longest blocks first,
 // few of which are shorter than the others and fill the end. Counting sorts by length in steps of 1/16, one workgroup for
 // the units of q and one for those of k; which of two alike comes first is open, and no result hangs on it.
 constexpr int PLAN_THREADS = 1024;
@@ -171,10 +171,12 @@ Args make_args(Strided q, Strided k, Strided v, const int32_t* cu, const int32_t
   return a;
 }
 
-// Bytes of the plan: none where all workgroups of the forward run at once.
-int64_t plan_bytes_of(const Plan& p, int64_t Hq) {
-  const int64_t seqs = p.uq;   // (nseq + 2 of them at most)
-  return p.uq * Hq <= 512 ? 0 : (p.uq + p.uk) * (int64_t)sizeof(Unit) + 8 * seqs;
+// Bytes of the plan: none where all workgroups of the forward run at once, or sequences are so short that none is left over
+// for long (24 sequences of 1365 tokens on average, 16 heads, a training step: 1393 us in their own order, 1377 with the plan,
+// 7 of which are its kernel; 13 of 3846 with a window 1307 and 1251).
+int64_t plan_bytes_of(const Plan& p, int64_t nseq, int64_t M, int64_t Hq) {
+  const int64_t seqs = nseq + 2;
+  return p.uq * Hq <= 512 || M < 1024 * nseq ? 0 : (p.uq + p.uk) * (int64_t)sizeof(Unit) + 8 * seqs;
 }
 
 template <typename T, int DP>
@@ -238,7 +240,7 @@ int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   if (M > 0 && ((rc = check_strided(k, 0, k_st, k_sh, D)) || (rc = check_strided(v, 0, v_st, v_sh, D)))) return rc;
   if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(res)) & 15) return MCE_ATTN_EALIGN;
   const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
-  const int64_t need = plan_bytes_of(p, Hq);
+  const int64_t need = plan_bytes_of(p, nseq, M, Hq);
   if (need > 0 && (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 255) || plan_bytes < (size_t)need))
     return MCE_ATTN_EWORKSPACE;
   Args a = make_args({static_cast<const uint16_t*>(q), 0, q_st, q_sh}, {static_cast<const uint16_t*>(k), 0, k_st, k_sh},
@@ -256,7 +258,7 @@ int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
 size_t mce_pack_plan_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                            int64_t sinks) {
   if (check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks) || N == 0) return 0;
-  return (size_t)plan_bytes_of(make_plan(nseq, N, M, Hkv, D, window, sinks), Hq);
+  return (size_t)plan_bytes_of(make_plan(nseq, N, M, Hkv, D, window, sinks), nseq, M, Hq);
 }
 
 size_t mce_pack_bwd_ws_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
@@ -289,7 +291,7 @@ int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   for (const void* p : {out, res, (const void*)dq, (const void*)dk, (const void*)dv})
     if (reinterpret_cast<uintptr_t>(p) & 15) return MCE_ATTN_EALIGN;
   const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
-  const bool planned = N > 0 && plan_bytes_of(p, Hq) > 0;
+  const bool planned = N > 0 && plan_bytes_of(p, nseq, M, Hq) > 0;
   if (planned && (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 255))) return MCE_ATTN_EWORKSPACE;
   const int64_t stat = align256(N * Hq * 8), part_s = align256(p.part_s * 4), part_r = align256(p.part_r * 4);
   if (stat + part_s + part_r > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) ||

@@ -138,6 +138,65 @@ def test_shared_key_blocks(lens, keys, hq, hkv, d, window, sinks):
     assert all(torch.equal(a, b) for a, b in zip(got, again))   # no sum depends on an order
 
 
+@pytest.mark.parametrize("lens,keys,hq,hkv,d,window,sinks,first", [
+    ([3100, 0, 4200, 1, 3700], None, 8, 4, 64, 0, 0, 0), ([2100, 5000, 40, 3000], None, 8, 2, 128, 300, 4, 77),
+    ([5000, 300, 2600], [5000, 3000, 2600], 8, 8, 64, 0, 0, 5), ([6000], None, 16, 1, 64, 1000, 0, 0),
+    ([129, 4000, 0], [2500, 4001, 2300], 16, 4, 128, 700, 140, 0)])
+def test_planned_order(lens, keys, hq, hkv, d, window, sinks, first):
+    """Long sequences of many heads are taken in an order of their own. No result hangs on it: two heads alone, which are not,
+    have the same bits, but for the sums of dk and dv, whose parts are others. Those are off by half a step (2^-8) of the sum
+    and of each pair's part, and by the fp32 sums' own errors (2^-16 of the largest)."""
+    from memarch_amd import _lib
+    print(f"packed plan {lens} {keys} {hq} {hkv} {d} {window} {sinks}", flush=True)
+    n, m = first + sum(lens) + 100, first + sum(keys or lens) + 100
+    size = _lib.load_serve().mce_pack_plan_bytes
+    assert size(len(lens), n, m, hq, hkv, d, window, sinks) > 0 and size(len(lens), n, m, 2, 1, d, window, sinks) == 0
+    q, k, v, go = (t.cuda() for t in _inputs(n, m, hq, hkv, d, BF, seed=n))
+    cu, cu_k = _cu(lens, first).cuda(), _cu(keys or lens, first).cuda()
+    got = _step(q, k, v, go, cu, cu_k, window, sinks)
+    again = _step(q, k, v, go, cu, cu_k, window, sinks)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    g = hq // hkv
+    for h in (0, hkv - 1):
+        heads = range(h * g, (h + 1) * g, 2) if g > 1 else [h]
+        parts = []
+        for i in heads:
+            use = slice(i, i + min(g, 2))
+            one = _step(q[:, use], k[:, h:h + 1], v[:, h:h + 1], go[:, use], cu, cu_k, window, sinks)
+            assert torch.equal(one[0], got[0][:, use]) and torch.equal(one[1], got[1][:, use])
+            parts.append(one[2:])
+        for i in (0, 1):
+            a, b = got[2 + i][:, h:h + 1].float(), [x[i].float() for x in parts]
+            tol = 1.01 * 2.0 ** -8 * (a.abs() + sum(x.abs() for x in b)) + 2.0 ** -16 * sum(x.abs().max() for x in b)
+            assert ((a - sum(b)).abs() <= tol).all(), (h, i)
+
+
+def test_planned_graph_and_falling_starts():
+    """A planned step captured, replayed with other lengths; and starts that fall, which the plan must not follow outside."""
+    from memarch_amd.attention import packed_attention
+    q, k, v, go = (t.cuda() for t in _inputs(6000, 6000, 16, 2, 64, BF, seed=4))
+    cu = torch.tensor([0, 3000, 6000], dtype=torch.int32, device="cuda")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    _step(q, k, v, go, cu, None, 500, 2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = packed_attention(*leaves, cu, window=500, sinks=2)
+        got = (out, *torch.autograd.grad(out, leaves, go))
+    for mid, end in ((3000, 6000), (1, 5999), (4500, 4500), (0, 6000), (3000, 6000)):
+        cu.copy_(torch.tensor([0, mid, end]))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = _step(q, k, v, go, cu, None, 500, 2)
+        assert all(torch.equal(a, b) for a, b in zip(got, ref)), (mid, end)
+    keep = [t.detach().clone() for t in (q, k, v, go)]
+    for falling in ([0, 5000, 100], [6000, 0, 6000], [7, -3, 2]):
+        for window in (0, 500):
+            _step(q, k, v, go, torch.tensor(falling, dtype=torch.int32, device="cuda"), None, window, 2 if window else 0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(keep, (q, k, v, go)))
+
+
 def test_many_sequences():
     """More sequences than one look at the starts takes (64), and than two do (4096)."""
     for nseq, dt in ((200, BF), (5000, HF)):
@@ -146,6 +205,9 @@ def test_many_sequences():
         lens[nseq // 2] = 150
         n = sum(lens)
         _check(*_inputs(n, n, 1, 1, 8, dt, seed=2), _cu(lens), None)
+    lens = torch.randint(950, 1250, (70,), generator=g).tolist()   # in planned order
+    n = sum(lens)
+    _check(*_inputs(n, n, 1, 1, 8, BF, seed=3), _cu(lens), None)
 
 
 def test_is_window_attention_of_each_sequence():
