@@ -28,7 +28,9 @@ elements; backward reads gu and go and writes d gu, 5 rows x H elements).
 `--op qk_norm_rope`, `--op window_attention` and `--op paged_attention` measure the attention operators of the same
 model (32 texts of 1024 tokens, 16 heads of 128, bf16; `--window`, `--sinks`): one line each with the pass (forward and
 backward; the paged cache: one new token for each of 64 sequences of up to 8192) and its share of the peak that bounds
-it, from the bytes or operations that it cannot do without.
+it, from the bytes or operations that it cannot do without. `--op packed_attention` is the same for 32768 tokens in 24 texts
+of up to 2600, packed, `--op cache_store` for 32 texts of 1024 tokens written into the 8-bit cache and read back (4 heads),
+`--op cache_attention` for the 64 sequences' next token, written and attended there.
 """
 import argparse
 import ctypes
@@ -76,6 +78,7 @@ def kernel_names(d, folded, dbias):
 # the siblings of the north-star op (--op): the same contractions on the same configuration inputs
 SIBLING_OPS = ("linear_ce", "linear_ce_sparse", "chunk_ce")
 ATTENTION_OPS = ("qk_norm_rope", "window_attention", "paged_attention")
+SERVING_OPS = ("packed_attention", "cache_store", "cache_attention")
 
 
 def fold_nr(d):
@@ -95,7 +98,7 @@ def _args():
     ap.add_argument("--stage-reps", type=int, default=0,
                     help="extra isolated timed repetitions of each C-ABI stage after the timed steps (0: none)")
     ap.add_argument("--calibrate-copy", action="store_true", help="time a 1 GiB device copy and exit")
-    ap.add_argument("--op", choices=("fused_ce",) + SIBLING_OPS + ("induct", "swiglu") + ATTENTION_OPS,
+    ap.add_argument("--op", choices=("fused_ce",) + SIBLING_OPS + ("induct", "swiglu") + ATTENTION_OPS + SERVING_OPS,
                     default="fused_ce",
                     help="fused_ce: the north-star operator (default); linear_ce, linear_ce_sparse, chunk_ce: its "
                          "siblings (fused_ops.py:39-101, full2.py:753-836) on the same inputs; induct: the "
@@ -672,7 +675,7 @@ def bench_swiglu(args):
 
 def bench_attention(args):
     """One attention operator (--op) through its public entry point, timed with torch events on the current stream."""
-    from memarch_amd import attention, rotary
+    from memarch_amd import attention, kv_cache, rotary
     dev = torch.device("cuda", 0)
     gen = torch.Generator(device=dev).manual_seed(2024)
     texts, t, h, d = 32, 1024, 16, 128
@@ -688,6 +691,41 @@ def bench_attention(args):
         step = lambda: attention.paged_attention(q, kc, vc, table, lens, window=window, sinks=sinks)
         nbytes, flops = int(seen.sum()) * 4 * hkv * d + 4 * b * h * d, int(seen.sum()) * 4 * h * d
         config = {"sequences": b, "tokens": most, "page": page, "heads": h, "kv_heads": hkv, "head_dim": d}
+    elif args.op in ("cache_store", "cache_attention"):
+        b, most, page, block, hkv = (texts, t, 64, 32, 4) if args.op == "cache_store" else (64, 8192, 64, 32, 4)
+        pages = b * most // page
+        cache = [torch.randn(pages, page, hkv, d, generator=gen, device=dev).to(torch.float8_e4m3fn) for _ in range(2)]
+        cache += [torch.ones(pages, page // block, hkv, device=dev) for _ in range(2)]
+        cache.append(torch.randperm(pages, generator=gen, device=dev).view(b, -1).int())
+        config = {"sequences": b, "tokens": most, "page": page, "block": block, "kv_heads": hkv, "head_dim": d}
+        if args.op == "cache_store":
+            k, v = mk(b * t, hkv, d), mk(b * t, hkv, d)
+            lens, cu = torch.full((b,), t, device=dev).int(), (torch.arange(b + 1, device=dev) * t).int()
+
+            def step():
+                kv_cache.cache_write(k, v, *cache, lens, cu)
+                kv_cache.cache_read(*cache, cu, b * t)
+            nbytes, flops = 2 * 6 * k.numel(), 0
+        else:
+            q, k, v = mk(b, h, d), mk(b, hkv, d), mk(b, hkv, d)
+            lens = torch.randint(most // 3, most + 1, (b,), generator=gen, device=dev).int()
+            seen = lens.clamp(max=args.window + sinks) if window else lens
+
+            def step():
+                kv_cache.cache_write(k, v, *cache, lens)
+                kv_cache.cache_attention(q, *cache, lens, window=window, sinks=sinks)
+            nbytes, flops = int(seen.sum()) * 2 * hkv * (d + 4 // block) + 4 * b * h * d, int(seen.sum()) * 4 * h * d
+            config["heads"] = h
+    elif args.op == "packed_attention":
+        lens = [(400 + 1013 * i) % 2600 for i in range(23)]
+        lens.append(texts * t - sum(lens))
+        cu = torch.tensor([0] + lens, device=dev).cumsum(0).int()
+        q, k, v, g = (mk(texts * t, h, d).requires_grad_() for _ in range(4))
+        step = lambda: torch.autograd.grad(attention.packed_attention(q, k, v, cu, window=window, sinks=sinks), (q, k, v), g)
+        far = lambda n: n * (n + 1) // 2 if not window or n <= window else \
+            window * (window + 1) // 2 + (n - window) * window + sum(max(0, n - window - j) for j in range(sinks))
+        nbytes, flops = 8 * q.numel() * 2, sum(far(n) for n in lens) * h * d * 14
+        config = {"texts": len(lens), "tokens": texts * t, "longest": max(lens), "heads": h, "kv_heads": h, "head_dim": d}
     else:
         q, k, v, g = (mk(texts, t, h, d).requires_grad_() for _ in range(4))
         config = {"texts": texts, "tokens": t, "heads": h, "kv_heads": h, "head_dim": d}
@@ -703,7 +741,7 @@ def bench_attention(args):
             j = torch.arange(t)[None]
             see = (j <= i) if window is None else (j <= i) & ((i - j < window) | (j < sinks))
             nbytes, flops = 8 * q.numel() * 2, int(see.sum()) * texts * h * d * 14
-    if args.op != "qk_norm_rope":
+    if args.op not in ("qk_norm_rope", "cache_store"):
         config.update(window=args.window, sinks=sinks)
     for _ in range(args.warmup):
         step()
@@ -718,7 +756,8 @@ def bench_attention(args):
     by_flops = flops / PEAK_BF16 > nbytes / PEAK_HBM
     value, unit, peak = (flops / dt / 1e12, "TFLOP/s", PEAK_BF16 / 1e12) if by_flops else \
         (nbytes / dt / 1e9, "GB/s", PEAK_HBM / 1e9)
-    what = "one new token" if args.op == "paged_attention" else "fwd+bwd"
+    what = {"paged_attention": "one new token", "cache_attention": "one new token, with its write",
+            "cache_store": "write and read back"}.get(args.op, "fwd+bwd")
     print(json.dumps({
         "metric": f"{unit} {args.op} {what}", "value": round(value, 1), "unit": unit, "n_gpus": 1, "steps": args.steps,
         "warmup": args.warmup, "ms_per_step": round(dt * 1e3, 4), "higher_is_better": True, "scaling": "weak",
@@ -747,7 +786,7 @@ def main():
     if args.op == "induct":
         bench_induct(args)
         return
-    if args.op in ATTENTION_OPS:
+    if args.op in ATTENTION_OPS + SERVING_OPS:
         bench_attention(args)
         return
     from memarch_amd import fused_ops
