@@ -476,12 +476,23 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
 }
 
 // out = the parts of one query head joined: one wave per head, 2 columns per lane, 64 parts at a time. Their states are
-// read by all lanes at once and their factors shared through LDS, so that the sums' loads depend on nothing.
+// read by all lanes at once and their factors shared through LDS, so that the sums' loads depend on nothing. A wave looks at
+// a sequence, or, where workgroups are fewer, at the place where one of them ends, and takes the sequence that goes on there
+// for the first time (4096 sequences, 32 heads: 433 us by sequences, 57 by ends).
 template <typename T>
 __global__ __launch_bounds__(64) void k_cache_join(Args a) {
   __shared__ float f[64];
-  const int h = blockIdx.x % a.Hq, b = blockIdx.x / a.Hq, lane = threadIdx.x, d = lane * 2;
-  const int64_t run = Cut(a).run, first = Cut::sum_of(a, b), w0 = first / run;
+  const int h = blockIdx.x % a.Hq, at = blockIdx.x / a.Hq, lane = threadIdx.x, d = lane * 2;
+  const int64_t run = Cut(a).run;
+  int b = at;
+  int64_t first;
+  if (a.B <= a.W) {
+    first = Cut::sum_of(a, b);
+  } else {
+    b = Cut::seq_of(a, (at + 1) * run, &first);
+    if (b >= a.B || first / run != at) return;
+  }
+  const int64_t w0 = first / run;
   const int n = (int)((first + Cut::tiles_of(a, b) - 1) / run - w0) + 1;
   if (n == 1) return;
   // part s: place 2 (w0 + s), the first one behind if it does not begin its workgroup's run
@@ -554,7 +565,8 @@ int launch(const Args& a, int64_t B, hipStream_t st) {
   const int pg = a.page % 32 == 0 ? 1 : (a.page % 16 == 0 ? 2 : 4);
   if (a.grp <= HC) run(pg == 1 ? k_cache_attn<T, DP, 1, 1> : (pg == 2 ? k_cache_attn<T, DP, 1, 2> : k_cache_attn<T, DP, 1, 4>));
   else run(pg == 1 ? k_cache_attn<T, DP, 2, 1> : (pg == 2 ? k_cache_attn<T, DP, 2, 2> : k_cache_attn<T, DP, 2, 4>));
-  if (a.W > 0) hipLaunchKernelGGL((k_cache_join<T>), dim3((unsigned)(B * a.Hq)), dim3(64), 0, st, a);
+  const int64_t joins = B <= a.W ? B : (a.W > 0 ? a.W - 1 : 0);
+  if (joins > 0) hipLaunchKernelGGL((k_cache_join<T>), dim3((unsigned)(joins * a.Hq)), dim3(64), 0, st, a);
   return finish();
 }
 

@@ -320,6 +320,19 @@ def test_many_parts(hq, hkv, d, page, block, most, lens, window, sinks):
     assert torch.equal(first, _attend(c, _q(b, hq, d, BF), torch.tensor(lens), window, sinks))
 
 
+@pytest.mark.parametrize("hq,hkv,d,most,lens,w", [
+    (64, 64, 16, 104, [0, 1, 1664, 0, 700, 33, 32, 31, 64, 2, 0, 0, 1664, 1500, 3, 256, 5, 90, 0, 1024], 16),
+    (128, 64, 16, 104, [1664] * 3 + [0] * 16 + [40], 16), (1024, 1024, 16, 62, [992, 500], 1)])
+def test_more_sequences_than_workgroups(hq, hkv, d, most, lens, w):
+    """A workgroup takes several sequences, and those that go on past its end are found from the ends."""
+    from memarch_amd import _lib
+    b = len(lens)
+    assert _lib.load_serve().mce_cache_attn_ws_bytes(b, hq, hkv, d, 16, most, 0, 0) == 2 * w * hq * (d * 4 + 8) and b > w
+    c = _filled(b, most, hkv, d, 16, 16, seed=3)
+    first = _attend(c, _q(b, hq, d, BF), torch.tensor(lens))
+    assert torch.equal(first, _attend(c, _q(b, hq, d, BF), torch.tensor(lens)))
+
+
 def test_scales_far_apart():
     """Blocks whose scales differ by up to 2^40 in the keys and the values: nothing overflows, and in fp16 what the bound
     allows for."""
