@@ -200,9 +200,10 @@ def _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, train):
 def _mark_leaves(out, dev):
     """Leaves the current stream's number on the gradient accumulators of the call's leaves, which live as long as a graph
     that uses them."""
+    here = _stream(dev)
     for node, _ in out.grad_fn.next_functions:
         if node is not None and type(node).__name__ == "AccumulateGrad":
-            node.metadata.setdefault("memarch_stream", torch.cuda.current_stream(dev).cuda_stream)
+            node.metadata.setdefault("memarch_stream", here)
 
 
 def _check_capture(ctx, dev):
@@ -210,7 +211,7 @@ def _check_capture(ctx, dev):
     the stream where that graph was made, which draws the stream into the capture and ends the process."""
     if not torch.cuda.is_current_stream_capturing():
         return
-    here = torch.cuda.current_stream(dev).cuda_stream
+    here = _stream(dev)
     for node, _ in ctx.next_functions:
         if node is not None and type(node).__name__ == "AccumulateGrad" and \
                 node.metadata.get("memarch_stream", here) != here:
@@ -284,7 +285,8 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, window=None, sinks=
     whose earlier keys are at hand): row i of n is position i + m - n of m. Rows that see nothing (m < n, or outside every
     sequence) and the gradients of rows that nothing sees are 0. The numbers stay on the device: they are not checked, a
     call does not wait for them, and a captured call may be replayed with others. Capturing a backward raises while an
-    earlier graph of the same leaves, made by this function on another stream, is alive."""
+    earlier graph of leaves that are q, k or v themselves, made by this function on another stream, is alive (as for any
+    operator, one of leaves farther up must not be)."""
     if torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         q, k, v = (t.to(dt) if t.dtype is torch.float32 else t for t in (q, k, v))
