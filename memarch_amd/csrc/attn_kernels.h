@@ -24,6 +24,8 @@ constexpr int BR = 32;              // query rows per tile there
 constexpr int NS = 4;               // tiles of k_attn_dkv's ring
 
 constexpr int64_t MIN_ITERS = 64;   // row tiles below which a workgroup of k_attn_dkv is not divided
+constexpr int64_t MIN_PACK = 32;    // the same of packed sequences (4 of 4096 tokens, 4 heads on one, window 512: 60 us; 78
+                                    // with 64)
 
 constexpr float LAZY = 8.f;         // k_attn_fwd: growth of a maximum (log2) up to which its old value is kept
 
@@ -592,7 +594,7 @@ struct Keys {
   // workgroups that share the block
   __device__ __forceinline__ int parts(const Args& a, int S) const {
     if constexpr (!PK) return S;
-    const int n = (int)(((int64_t)nt * a.grp + MIN_ITERS - 1) / MIN_ITERS);
+    const int n = (int)(((int64_t)nt * a.grp + MIN_PACK - 1) / MIN_PACK);
     return n < 1 ? 1 : (n < S ? n : S);
   }
 };
@@ -601,7 +603,7 @@ struct Keys {
 // registers, 32 per wave, and row tiles pass through a ring of NS. Scores and go v are formed a second time (seven
 // products in the backward for the formula's five), which needs neither atomics nor ds in memory.
 // Packed sequences: the host does not know how long the blocks are, so S is what the workspace has room for, and a block
-// is shared by no more workgroups than get MIN_ITERS row tiles each; one that is not shared is written at once.
+// is shared by no more workgroups than get MIN_PACK row tiles each; one that is not shared is written at once.
 // Measured (bf16, D = 128): 4 x 16384 tokens of 16 heads over 4, window 1024: 1.24 ms, 0.86 PFLOP/s of visible pairs (8 D
 // each), matrix core busy 45% of the time; the join of the first tokens' blocks 7 us.
 template <typename T, int DP, bool PK>
@@ -617,7 +619,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   const uint32_t w = sink ? blockIdx.x : blockIdx.x - sink_wgs;
   const int S = sink ? a.S_s : a.S_r, nb = sink ? nsink : nr;
   const Place pl(a, w, nb * S, 1, PK && a.plan != nullptr && !sink);
-  const int sp = pl.blk % S, blk = pl.blk / S, b = pl.b, hk = pl.hk, bh = b * a.Hkv + hk;
+  // Packed: the parts that are not used come last. Between the others they left those on few CUs (52 sequences of 339
+  // tokens, 12 heads, window 44 and a first token: 223 us, 127 so).
+  const int sp = PK ? pl.blk / nb : pl.blk % S, blk = PK ? pl.blk % nb : pl.blk / S, b = pl.b, hk = pl.hk, bh = b * a.Hkv + hk;
   const Keys<PK> at(a, b, sink, blk);
   const int len = at.len, kb0 = at.kb0, j0 = kb0 + wave * 32;
   const int parts = at.parts(a, S);
@@ -776,7 +780,6 @@ template <typename T, bool PK>
 __global__ __launch_bounds__(256) void k_attn_dkv_join(Args a, int pieces) {
   const int nsink = PK ? a.nseq * a.n_sb : a.n_sb, nr = PK ? a.uk : (a.T + BKV - 1) / BKV - a.n_sb;
   const uint32_t heads = (uint32_t)a.B * a.Hkv, sink_blocks = a.S_s > 1 ? heads * nsink : 0;
-  const int i = blockIdx.x % pieces * 256 + threadIdx.x;
   uint32_t w = blockIdx.x / pieces;
   const bool sink = w < sink_blocks;
   if (!sink) w -= sink_blocks;
@@ -795,17 +798,24 @@ __global__ __launch_bounds__(256) void k_attn_dkv_join(Args a, int pieces) {
     kb0 = (sink ? blk : a.n_sb + blk) * BKV;
   }
   const int cols = a.D / 4;
-  const int which = i / (BKV * cols), r = i / cols % BKV, d = i % cols * 4, key = kb0 + r;
-  if (which > 1 || key >= rows) return;
-  const float* const p = (sink ? a.part_s : a.part_r) + ((((int64_t)bh * nb + blk) * S * 2 + which) * BKV + r) * a.D + d;
-  f32x4 x = {};
+  for (int i = blockIdx.x % pieces * 256 + threadIdx.x;; i += pieces * 256) {
+    const int which = i / (BKV * cols), r = i / cols % BKV, d = i % cols * 4, key = kb0 + r;
+    if (which > 1) return;
+    if (key >= rows) {
+      if (PK) continue;
+      return;                                             // (pieces for all)
+    }
+    const float* const p = (sink ? a.part_s : a.part_r) + ((((int64_t)bh * nb + blk) * S * 2 + which) * BKV + r) * a.D + d;
+    f32x4 x = {};
 #pragma unroll 4
-  for (int sp = 0; sp < parts; ++sp) x += *reinterpret_cast<const f32x4*>(p + (int64_t)sp * 2 * BKV * a.D);
-  if (which == 0) x *= a.scale;
-  u32x2 v;
-  v[0] = pack2<T>(x[0], x[1]);
-  v[1] = pack2<T>(x[2], x[3]);
-  *reinterpret_cast<u32x2*>((which ? a.dv : a.dk) + (((int64_t)b * a.T + krow + key) * a.Hkv + hk) * a.D + d) = v;
+    for (int sp = 0; sp < parts; ++sp) x += *reinterpret_cast<const f32x4*>(p + (int64_t)sp * 2 * BKV * a.D);
+    if (which == 0) x *= a.scale;
+    u32x2 v;
+    v[0] = pack2<T>(x[0], x[1]);
+    v[1] = pack2<T>(x[2], x[3]);
+    *reinterpret_cast<u32x2*>((which ? a.dv : a.dk) + (((int64_t)b * a.T + krow + key) * a.Hkv + hk) * a.D + d) = v;
+    if (!PK) return;
+  }
 }
 
 }  // namespace

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "../../include/mce_pack.h"
 #include "attn_host.h"
 #include "attn_kernels.h"
@@ -116,17 +118,21 @@ struct Plan {
 // How many workgroups may share a key block's rows (the kernels use fewer where its rows are few). Lengths are not known
 // here: key blocks are shared where there are too few of them to fill the GPU, blocks with first tokens of windowed
 // sequences, which every later row sees, until there are 2048 workgroups for them.
-Plan make_plan(int64_t nseq, int64_t N, int64_t M, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
+Plan make_plan(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
   Plan p = {N / BQ + nseq + 2, M / BKV + nseq + 2, 0, 1, 1, 0, 0};
-  if (window > 0 && window < M && sinks > 0) {
+  // parts that a block can have when it sees n rows
+  auto most_parts = [&](int64_t n) { return ((n + BR - 1) / BR * (Hq / Hkv) + MIN_PACK - 1) / MIN_PACK; };
+  const bool windowed = window > 0 && window < M;
+  if (windowed && sinks > 0) {
     const int64_t most = M / BKV + 1, n = (sinks + BKV - 1) / BKV;
     p.n_sb = (int)(n < most ? n : most);
     const int64_t units = nseq * p.n_sb * Hkv;
-    int64_t s = units > 0 ? (2048 + units - 1) / units : 1;
-    p.S_s = (int)(s > 64 ? 64 : s);
+    const int64_t s = units > 0 ? (2048 + units - 1) / units : 1;
+    p.S_s = (int)std::clamp(std::min(s, most_parts(N)), int64_t(1), int64_t(64));
   }
-  const int64_t s = (1024 + p.uk * Hkv - 1) / (p.uk * Hkv);
-  p.S_r = (int)(s > 16 ? 16 : s);
+  const int64_t s = (768 + p.uk * Hkv - 1) / (p.uk * Hkv);
+  const int64_t rows = windowed && window + BKV + BR < N ? window + BKV + BR : N;
+  p.S_r = (int)std::clamp(std::min(s, most_parts(rows)), int64_t(1), int64_t(16));
   p.part_s = p.S_s > 1 ? nseq * p.n_sb * Hkv * p.S_s * 2 * BKV * D : 0;
   p.part_r = p.S_r > 1 ? p.uk * Hkv * p.S_r * 2 * BKV * D : 0;
   return p;
@@ -136,7 +142,7 @@ int check_sizes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int
   if (nseq < 0 || N < 0 || M < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || D > 128 || D % 8 || window < 0 || sinks < 0)
     return MCE_ATTN_EINVAL;
   if (N > MAX_ROWS || M > MAX_ROWS || nseq > MAX_GROUPS || Hq * D > MAX_ST) return MCE_ATTN_EINVAL;
-  const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  const Plan p = make_plan(nseq, N, M, Hq, Hkv, D, window, sinks);
   // the sums are below 2^63: sinks' blocks are at most M / BKV + 1 per sequence
   if (p.uq > MAX_GROUPS / Hq || p.uk * p.S_r > MAX_GROUPS / Hkv ||
       nseq * p.n_sb * p.S_s > MAX_GROUPS / Hkv - p.uk * p.S_r)
@@ -202,7 +208,9 @@ int launch_bwd(const Args& a, hipStream_t st) {
   hipLaunchKernelGGL((k_attn_dkv<T, DP, true>), dim3((unsigned)(a.Hkv * (nsink * a.S_s + (int64_t)a.uk * a.S_r))),
                      dim3(THREADS), 0, st, a);
   const int64_t join = a.Hkv * ((a.S_s > 1 ? nsink : 0) + (a.S_r > 1 ? (int64_t)a.uk : 0));
-  const int pieces = (2 * BKV * (a.D / 4) + 255) / 256;
+  // few blocks need many threads each; of many most are not shared, and a workgroup that only finds that out costs 1 ns
+  const int64_t all = (2 * BKV * (a.D / 4) + 255) / 256;
+  const int pieces = (int)std::clamp(4096 / std::max(join, int64_t(1)), int64_t(1), all);
   if (join > 0)
     hipLaunchKernelGGL((k_attn_dkv_join<T, true>), dim3((unsigned)(join * pieces)), dim3(256), 0, st, a, pieces);
   return finish();
@@ -239,7 +247,7 @@ int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   if (cu == nullptr || out == nullptr || (rc = check_strided(q, 0, q_st, q_sh, D))) return rc ? rc : MCE_ATTN_EINVAL;
   if (M > 0 && ((rc = check_strided(k, 0, k_st, k_sh, D)) || (rc = check_strided(v, 0, v_st, v_sh, D)))) return rc;
   if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(res)) & 15) return MCE_ATTN_EALIGN;
-  const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  const Plan p = make_plan(nseq, N, M, Hq, Hkv, D, window, sinks);
   const int64_t need = plan_bytes_of(p, nseq, M, Hq);
   if (need > 0 && (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 255) || plan_bytes < (size_t)need))
     return MCE_ATTN_EWORKSPACE;
@@ -258,13 +266,13 @@ int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
 size_t mce_pack_plan_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                            int64_t sinks) {
   if (check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks) || N == 0) return 0;
-  return (size_t)plan_bytes_of(make_plan(nseq, N, M, Hkv, D, window, sinks), nseq, M, Hq);
+  return (size_t)plan_bytes_of(make_plan(nseq, N, M, Hq, Hkv, D, window, sinks), nseq, M, Hq);
 }
 
 size_t mce_pack_bwd_ws_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                              int64_t sinks) {
   if (check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks)) return 0;
-  const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  const Plan p = make_plan(nseq, N, M, Hq, Hkv, D, window, sinks);
   return (size_t)(align256(N * Hq * 8) + align256(p.part_s * 4) + align256(p.part_r * 4));
 }
 
@@ -290,7 +298,7 @@ int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   }
   for (const void* p : {out, res, (const void*)dq, (const void*)dk, (const void*)dv})
     if (reinterpret_cast<uintptr_t>(p) & 15) return MCE_ATTN_EALIGN;
-  const Plan p = make_plan(nseq, N, M, Hkv, D, window, sinks);
+  const Plan p = make_plan(nseq, N, M, Hq, Hkv, D, window, sinks);
   const bool planned = N > 0 && plan_bytes_of(p, nseq, M, Hq) > 0;
   if (planned && (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 255))) return MCE_ATTN_EWORKSPACE;
   const int64_t stat = align256(N * Hq * 8), part_s = align256(p.part_s * 4), part_r = align256(p.part_r * 4);
