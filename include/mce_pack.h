@@ -35,17 +35,20 @@ MCE_SERVE_API int mce_serve_last_hip_error(void);
 
 /* out, and for a backward (both may be NULL) res and lse, as in mce_attn_fwd. The plan, scratch memory of the forward, is the
  * order in which blocks of rows are taken, the longest first (0 bytes where their own order is as good); a backward takes the plan of
- * its forward, unchanged, which res asks for. */
+ * its forward, unchanged, which res asks for. The workspace holds parts of the sums of rows whose keys are shared by several
+ * workgroups, as is done where there are few rows and many keys (else 0 bytes). */
 MCE_SERVE_API size_t mce_pack_plan_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
                                          int64_t window, int64_t sinks);
+MCE_SERVE_API size_t mce_pack_fwd_ws_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
+                                           int64_t window, int64_t sinks);
 MCE_SERVE_API int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                                const void* v, int64_t v_st, int64_t v_sh, const int32_t* cu, const int32_t* cu_k,
                                int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                                int64_t sinks, float scale, int dtype, void* out, void* res, float* lse, void* plan,
-                               size_t plan_bytes, void* stream);
+                               size_t plan_bytes, void* ws, size_t ws_bytes, void* stream);
 
 /* dq, dk and dv from the forward's inputs, out, res, lse and plan. The workspace holds -lse and -d (fp32 [Hq, 2, N]) and, where
- * the sums of dk and dv may be shared by several workgroups, their fp32 parts. */
+ * sums may be shared by several workgroups, their fp32 parts. */
 MCE_SERVE_API size_t mce_pack_bwd_ws_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
                                            int64_t window, int64_t sinks);
 MCE_SERVE_API int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,

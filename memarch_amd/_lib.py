@@ -96,7 +96,8 @@ SERVE_SIGNATURES = {
     "mce_serve_error_string": (ctypes.c_char_p, [_INT]),
     "mce_serve_last_hip_error": (_INT, []),
     "mce_pack_plan_bytes": (_S, 8 * [_I]),
-    "mce_pack_fwd": (_INT, 3 * _ROWS + [_P, _P] + 8 * [_I] + [_F, _INT, _P, _P, _P, _P, _S, _P]),
+    "mce_pack_fwd_ws_bytes": (_S, 8 * [_I]),
+    "mce_pack_fwd": (_INT, 3 * _ROWS + [_P, _P] + 8 * [_I] + [_F, _INT, _P, _P, _P, _P, _S, _P, _S, _P]),
     "mce_pack_bwd_ws_bytes": (_S, 8 * [_I]),
     "mce_pack_bwd": (_INT, 4 * _ROWS + [_P, _P] + 8 * [_I] + [_F, _INT, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
     # include/mce_cache.h

@@ -188,12 +188,13 @@ def _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, train):
     out = torch.empty(N, Hq, D, dtype=q.dtype, device=q.device)
     res = torch.empty_like(out) if train else None
     lse = torch.empty(Hq, N, dtype=torch.float32, device=q.device) if train else None
-    n = _lib.load_serve().mce_pack_plan_bytes(cu.shape[0] - 1, N, k.shape[0], Hq, k.shape[1], D, window, sinks)
+    lib, sizes = _lib.load_serve(), (cu.shape[0] - 1, N, k.shape[0], Hq, k.shape[1], D, window, sinks)
+    n, w = lib.mce_pack_plan_bytes(*sizes), lib.mce_pack_fwd_ws_bytes(*sizes)
     plan = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    ws = torch.empty(w, dtype=torch.uint8, device=q.device) if w else None
     with _On(q.device):
-        _lib.call("mce_pack_fwd", *qs, *ks, *vs, cu.data_ptr(), _ptr(cu_k), cu.shape[0] - 1, N, k.shape[0], Hq, k.shape[1],
-                  D, window, sinks, scale, _DTYPES[q.dtype], out.data_ptr(), _ptr(res), _ptr(lse), _ptr(plan), n,
-                  _stream(q.device))
+        _lib.call("mce_pack_fwd", *qs, *ks, *vs, cu.data_ptr(), _ptr(cu_k), *sizes, scale, _DTYPES[q.dtype], out.data_ptr(),
+                  _ptr(res), _ptr(lse), _ptr(plan), n, _ptr(ws), w, _stream(q.device))
     return q, k, v, out, res, lse, plan
 
 

@@ -43,7 +43,7 @@ Args make_args(Strided q, Strided k, Strided v, const int32_t* lengths, int64_t 
 template <typename T, int DP>
 int launch_fwd(const Args& a, hipStream_t st) {
   const unsigned n = (unsigned)((int64_t)a.B * a.Hq * ((a.T + BQ - 1) / BQ));
-  hipLaunchKernelGGL((k_attn_fwd<T, DP, false>), dim3(n), dim3(THREADS), 0, st, a);
+  hipLaunchKernelGGL((k_attn_fwd<T, DP, false, false>), dim3(n), dim3(THREADS), 0, st, a);
   return finish();
 }
 
@@ -96,7 +96,7 @@ Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t
 template <typename T, int DP>
 int launch_bwd(const Args& a, hipStream_t st) {
   const unsigned n = (unsigned)((int64_t)a.B * a.Hq * ((a.T + BQ - 1) / BQ));
-  hipLaunchKernelGGL((k_attn_dq<T, DP, false>), dim3(n), dim3(THREADS), 0, st, a);
+  hipLaunchKernelGGL((k_attn_dq<T, DP, false, false>), dim3(n), dim3(THREADS), 0, st, a);
   const int64_t heads = (int64_t)a.B * a.Hkv, nr = (a.T + BKV - 1) / BKV - a.n_sb;
   hipLaunchKernelGGL((k_attn_dkv<T, DP, false>), dim3((unsigned)(heads * (a.n_sb * a.S_s + nr * a.S_r))), dim3(THREADS), 0, st,
                      a);

@@ -53,6 +53,10 @@ struct Args {
   int nseq, M;               // M: rows of k
   int uq, uk;                // units of BQ rows of q and of BKV rows of k
   struct Unit* plan;         // those of q and then those of k, the longest first; null: in their own order
+  // workgroups that share the key tiles of a unit of q (1: SPLIT is false); query heads of each (1, 2 or 4) then, and
+  // whether sequences have no more rows on average than one workgroup takes of a head
+  int S_q, fold, thin;
+  float *part_q, *ml;        // their sums [S_q, N, Hq, D], and maxima and denominators (sums of ds and d) [S_q, N, Hq, 2]
 };
 
 // Packed sequences: rows of different sequences lie behind each other, sequence s in rows cu[s] .. cu[s + 1] - 1 of q and
@@ -228,6 +232,63 @@ __device__ __forceinline__ void mask_keys(f32x16& s, int row, int k0h, int windo
   }
 }
 
+// Few rows behind many keys: the key tiles of a block of rows are shared by up to S_q workgroups (SPLIT), none of which
+// gets fewer than MIN_KEYS tiles, and a launch of its own joins their fp32 sums. A workgroup's waves take up to 4 (`fold`)
+// query heads of a group with fewer rows each, so that the group's keys are loaded once, and its other heads follow on the
+// same XCD (1 row behind 131072 keys, 16 heads over 4, in us: 2282 by one workgroup per head; in parts 227, with a group on one
+// XCD 149, folded and in better order 66, which is 4.0 TB/s; 16 heads over 16 are as fast as HBM). The host does not know how many
+// rows and parts a block has: those that are left over come behind the others, as between them they left those on few CUs
+// (64 rows: 88 us, 46 so).
+constexpr int MIN_KEYS = 8;
+struct SplitPlace {
+  int hk, g, r, blk, sp;   // g: the wave's query head of its group; r: its first row in the block
+  bool none;
+  __device__ __forceinline__ SplitPlace(const Args& a, uint32_t bid, int wave) {
+    const uint32_t slot = bid / 8, rows = BQ / a.fold, in = rows / 32;   // rows of each head, waves for them
+    // i: which `fold` heads of the group; q: which quarter (half) of the block's rows
+    uint32_t i = slot % a.grp, q = i % a.fold, at = slot / a.grp;
+    i /= a.fold;
+    if (a.thin) {                                       // few sequences have rows for more than the first
+      const uint32_t heads = a.grp / a.fold, all = ((uint32_t)a.Hkv * a.uq * a.S_q + 7) / 8 * heads;
+      q = slot / all;
+      i = slot % all % heads;
+      at = slot % all / heads;
+    }
+    const uint32_t set = at * 8 + bid % 8, w = set / a.Hkv;
+    g = i * a.fold + wave / in;
+    r = q * rows + wave % in * 32;
+    hk = set % a.Hkv;
+    blk = w / a.S_q;
+    sp = w % a.S_q;
+    none = blk >= a.uq;
+  }
+};
+__device__ __forceinline__ int key_parts(const Args& a, int tiles) {
+  const int n = tiles / MIN_KEYS;
+  return n < 1 ? 1 : (n < a.S_q ? n : a.S_q);
+}
+// The sums of a block's rows that a joining workgroup puts together: 4 columns of a row at a time.
+struct Joint {
+  Rows<true> at;
+  int hq, parts;
+  __device__ __forceinline__ Joint(const Args& a, uint32_t w) : at(a, 0, (int)(w / a.Hq)), hq(w % a.Hq), parts(1) {
+    if (at.any()) parts = key_parts(a, KeyTiles(a, at.first(), at.last()).n);
+  }
+  // f(row, its number among all rows, column); pieces workgroups share the block
+  template <typename F>
+  __device__ __forceinline__ void each(const Args& a, int pieces, F f) const {
+    const int cols = a.D / 4;
+    for (int i = blockIdx.x % pieces * 256 + threadIdx.x; i < BQ * cols; i += pieces * 256) {
+      const int row = at.q0 + i / cols;
+      if (!at.in(row)) return;
+      f(row, at.qrow + row - at.off, i % cols * 4);
+    }
+  }
+};
+__device__ __forceinline__ int64_t part_at(const Args& a, int sp, int64_t line, int hq) {
+  return (((int64_t)sp * a.T + line) * a.Hq + hq);
+}
+
 // ---------------------------------------------------------------------------------------------------------- forward
 // out_i = sum_j exp(c s_ij - c m_i) v_j / sum_j exp(c s_ij - c m_i) in one pass over the keys, m_i a maximum of the scores so far.
 // 32 rows per wave hold their scores as [keys][rows], so that a row's statistics lie in two lanes and the scores become an
@@ -239,22 +300,40 @@ __device__ __forceinline__ void mask_keys(f32x16& s, int row, int k0h, int windo
 // With D <= 64 vector work is busy half the time and the matrix core a quarter, so waves are what fills the gaps: four per
 // SIMD, in 128 registers with the tile's offsets made again for each tile, take 96 us where three take 102 (8 texts of up to
 // 2999 tokens, 12 heads, fp16). At D = 128 the registers leave room for two.
-template <typename T, int DP, bool PK>
+template <typename T, int DP, bool PK, bool SPLIT>
 __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) {
   constexpr int IMG = BK * DP * 2;                     // bytes of a tile
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];   // K and V, two tiles each
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int nq = PK ? a.uq : (a.T + BQ - 1) / BQ;
-  const Place pl(a, blockIdx.x, nq, a.grp, PK && a.plan != nullptr);
-  const int b = pl.b, hk = pl.hk, hq = hk * a.grp + pl.g, bh = b * a.Hq + hq;
-  const Rows<PK> at(a, b, PK && a.plan ? pl.blk : nq - 1 - pl.blk);
-  const int len = at.len, q0 = at.q0, r0 = q0 + wave * 32, row = r0 + (lane & 31);
+  int b = 0, hk, g, blk, sp = 0, parts = 1, r = wave * 32;
+  if constexpr (SPLIT) {
+    const SplitPlace pl(a, blockIdx.x, wave);
+    if (pl.none) return;
+    hk = pl.hk;
+    g = pl.g;
+    blk = pl.blk;
+    sp = pl.sp;
+    r = pl.r;
+  } else {
+    const Place pl(a, blockIdx.x, nq, a.grp, PK && a.plan != nullptr);
+    b = pl.b;
+    hk = pl.hk;
+    g = pl.g;
+    blk = PK && a.plan ? pl.blk : nq - 1 - pl.blk;
+  }
+  const int hq = hk * a.grp + g, bh = b * a.Hq + hq;
+  const Rows<PK> at(a, b, blk);
+  const int len = at.len, q0 = at.q0, r0 = q0 + r, row = r0 + (lane & 31);
   f32x16 acc[DP / 32] = {};
   float m = -INFINITY, l = 0.f;
   bool large = false;   // some row's m is beyond LARGE
   const float c = a.scale * LOG2E;
   if (at.any()) {
     const KeyTiles kt(a, at.first(), at.last());
+    if constexpr (SPLIT) parts = key_parts(a, kt.n);
+    if (SPLIT && (sp >= parts || !at.in(q0 + r / (BQ / a.fold) * (BQ / a.fold)))) return;
+    const int t0 = SPLIT ? kt.n * sp / parts : 0, t1 = SPLIT ? kt.n * (sp + 1) / parts : kt.n;
     FragAddr<DP> ad;
     ad.init(lane);
     TileLoad<DP, BK, NW> tk, tv;
@@ -267,7 +346,7 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) 
       tk.issue(tile_rsrc<BK>(kp, a.k.st, k0, end, a.D), lds, buf * 2 * IMG, wave);
       tv.issue(tile_rsrc<BK>(vp, a.v.st, k0, end, a.D), lds, buf * 2 * IMG + IMG, wave);
     };
-    issue(0, 0);
+    issue(t0, 0);
     // the wave's query rows as fragments: row l%32, columns 16 ks + 8 h + 0..7
     u32x4 qf[DP / 16];
     const i32x4 qr = tile_rsrc<32>(a.q.p + (PK ? at.qrow * a.q.st : b * a.q.sb) + hq * a.q.sh, a.q.st, r0 - at.off, at.read(), a.D);
@@ -278,9 +357,9 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) 
     }
     wait_vmcnt<0>();
     __syncthreads();
-    for (int it = 0; it < kt.n; ++it) {
-      const int img = (it & 1) * 2 * IMG;
-      if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
+    for (int it = t0; it < t1; ++it) {
+      const int img = (it - t0 & 1) * 2 * IMG;
+      if (it + 1 < t1) issue(it + 1, it + 1 - t0 & 1);
       const int k0 = kt.key0(it);
       if constexpr (DP == 64) ad.refresh();            // 128 registers: four waves per SIMD
       // whether the wave's rows see a key of the tile
@@ -351,14 +430,58 @@ __global__ __launch_bounds__(THREADS, DP == 64 ? 4 : 2) void k_attn_fwd(Args a) 
       __syncthreads();
     }
   }
+  if (SPLIT && sp >= parts) return;                       // (a block that sees nothing)
   l = sum_halves(l);
   const int64_t line = at.qrow + row - at.off;
   const int64_t ofs = ((int64_t)b * a.T + line) * a.Hq * a.D + (int64_t)hq * a.D;
   const bool in = at.in(row), see = at.live(row);
+  if (SPLIT && parts > 1) {
+    const int64_t to = part_at(a, sp, line, hq);
+    store_f32<DP>(acc, a.part_q + to * a.D, a.D, in, see, h);
+    if (in && h == 0) {
+      a.ml[to * 2] = m;
+      a.ml[to * 2 + 1] = l;
+    }
+    return;
+  }
   const float inv = 1.f / l;
   store_acc<T, DP>(acc, inv, a.o + ofs, a.D, in, see, h);
   if (a.r != nullptr) store_acc<T, DP, true>(acc, inv, a.r + ofs, a.D, in, see, h);
   if (a.lse != nullptr && in && h == 0) a.lse[(int64_t)bh * a.T + line] = see ? m + __builtin_amdgcn_logf(l) / c : INFINITY;
+}
+
+// out, res and lse of the rows whose keys were shared.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_fwd_join(Args a, int pieces) {
+  const Joint jt(a, blockIdx.x / pieces);
+  if (jt.parts == 1) return;
+  const float c = a.scale * LOG2E;
+  jt.each(a, pieces, [&](int row, int64_t line, int d) {
+    const bool live = jt.at.live(row);
+    float mm = -INFINITY, l = 0.f;
+#pragma unroll 16
+    for (int sp = 0; sp < jt.parts; ++sp) mm = fmaxf(mm, a.ml[part_at(a, sp, line, jt.hq) * 2]);
+    f32x4 x = {};
+#pragma unroll 16
+    for (int sp = 0; sp < jt.parts; ++sp) {
+      const int64_t p = part_at(a, sp, line, jt.hq);
+      const float f = __builtin_amdgcn_exp2f((a.ml[p * 2] - mm) * c);
+      l = __builtin_fmaf(a.ml[p * 2 + 1], f, l);
+      x += *reinterpret_cast<const f32x4*>(a.part_q + p * a.D + d) * f;
+    }
+    x *= 1.f / l;
+    const int64_t to = (line * a.Hq + jt.hq) * a.D + d;
+    u32x2 o, e;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      o[i] = live ? pack2<T>(x[2 * i], x[2 * i + 1]) : 0;
+      e[i] = live ? pack2<T>(x[2 * i] - lo_f32<T>(o[i]), x[2 * i + 1] - hi_f32<T>(o[i])) : 0;
+    }
+    *reinterpret_cast<u32x2*>(a.o + to) = o;
+    if (a.r != nullptr) *reinterpret_cast<u32x2*>(a.r + to) = e;
+    if (a.lse != nullptr && d == 0)
+      a.lse[(int64_t)jt.hq * a.T + line] = live ? mm + __builtin_amdgcn_logf(l) / c : INFINITY;
+  });
 }
 
 // --------------------------------------------------------------------------------------------------------------- dq
@@ -387,21 +510,39 @@ __device__ __forceinline__ u32x4 four(const uint32_t (&w)[8], int s) {
 // pass, as in the forward, so that dq is summed by one wave in one order. It also forms d and leaves -lse and -d for
 // k_attn_dkv. Measured (bf16, D = 128): 4 x 16384 tokens of 16 heads, window 1024: 1.10 ms, 0.73 PFLOP/s of visible pairs
 // (6 D each), matrix core busy 46% of the time.
-template <typename T, int DP, bool PK>
+template <typename T, int DP, bool PK, bool SPLIT>
 __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
   constexpr int IMG = BK * DP * 2;
   __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nq = PK ? a.uq : (a.T + BQ - 1) / BQ;
-  const Place pl(a, blockIdx.x, nq, a.grp, PK && a.plan != nullptr);
-  const int b = pl.b, hk = pl.hk, hq = hk * a.grp + pl.g, bh = b * a.Hq + hq;
-  const Rows<PK> at(a, b, PK && a.plan ? pl.blk : nq - 1 - pl.blk);
-  const int len = at.len, q0 = at.q0, r0 = q0 + wave * 32;
+  int b = 0, hk, g, blk, sp = 0, parts = 1, r = wave * 32;
+  if constexpr (SPLIT) {
+    const SplitPlace pl(a, blockIdx.x, wave);
+    if (pl.none) return;
+    hk = pl.hk;
+    g = pl.g;
+    blk = pl.blk;
+    sp = pl.sp;
+    r = pl.r;
+  } else {
+    const Place pl(a, blockIdx.x, nq, a.grp, PK && a.plan != nullptr);
+    b = pl.b;
+    hk = pl.hk;
+    g = pl.g;
+    blk = PK && a.plan ? pl.blk : nq - 1 - pl.blk;
+  }
+  const int hq = hk * a.grp + g, bh = b * a.Hq + hq;
+  const Rows<PK> at(a, b, blk);
+  const int len = at.len, q0 = at.q0, r0 = q0 + r;
   f32x16 acc[DP / 32] = {};
   float delta = 0.f, nl = -INFINITY, sum = 0.f;
   const float c = a.scale * LOG2E;
   if (at.any()) {
     const KeyTiles kt(a, at.first(), at.last());
+    if constexpr (SPLIT) parts = key_parts(a, kt.n);
+    if (SPLIT && (sp >= parts || !at.in(q0 + r / (BQ / a.fold) * (BQ / a.fold)))) return;
+    const int t0 = SPLIT ? kt.n * sp / parts : 0, t1 = SPLIT ? kt.n * (sp + 1) / parts : kt.n;
     const int lane = lane_now();
     FragAddr<DP> ad;
     ad.init(lane);
@@ -415,7 +556,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       tk.issue(tile_rsrc<BK>(kp, a.k.st, k0, end, a.D), lds, buf * 2 * IMG, wave);
       tv.issue(tile_rsrc<BK>(vp, a.v.st, k0, end, a.D), lds, buf * 2 * IMG + IMG, wave);
     };
-    issue(0, 0);
+    issue(t0, 0);
     u32x4 qf[DP / 16], gf[DP / 16];
     const i32x4 qr = tile_rsrc<32>(a.q.p + (PK ? at.qrow * a.q.st : b * a.q.sb) + hq * a.q.sh, a.q.st, r0 - at.off, at.read(), a.D);
     const i32x4 gr = tile_rsrc<32>(a.go.p + (PK ? at.qrow * a.go.st : b * a.go.sb) + hq * a.go.sh, a.go.st, r0 - at.off, at.read(), a.D);
@@ -440,9 +581,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
     if (PK ? at.in(row) : row < len) nl = -a.lse[(int64_t)bh * a.T + at.qrow + row - at.off];
     wait_vmcnt<0>();
     __syncthreads();
-    for (int it = 0; it < kt.n; ++it) {
-      const int img = (it & 1) * 2 * IMG;
-      if (it + 1 < kt.n) issue(it + 1, (it + 1) & 1);
+    for (int it = t0; it < t1; ++it) {
+      const int img = (it - t0 & 1) * 2 * IMG;
+      if (it + 1 < t1) issue(it + 1, it + 1 - t0 & 1);
       const int k0 = kt.key0(it);
       ad.refresh();
       // the halves of the tile (32 keys) that the wave's rows see a key of: first .. last - 1
@@ -526,11 +667,21 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
       __syncthreads();
     }
   }
+  if (SPLIT && sp >= parts) return;
   sum = sum_halves(sum);
   const int ln = lane_now(), h = ln >> 5, row = r0 + (ln & 31);
   const int64_t line = at.qrow + row - at.off;
   const int64_t ofs = ((int64_t)b * a.T + line) * a.Hq * a.D + (int64_t)hq * a.D;
   const bool in = at.in(row), live = at.live(row);
+  if (SPLIT && parts > 1) {
+    const int64_t to = part_at(a, sp, line, hq);
+    store_f32<DP>(acc, a.part_q + to * a.D, a.D, in, live, h);
+    if (in && h == 0) {
+      a.ml[to * 2] = sum;
+      a.ml[to * 2 + 1] = delta;
+    }
+    return;
+  }
   store_acc<T, DP>(acc, a.scale, a.dq + ofs, a.D, in, live, h);
   if (in && h == 0) {
     // The output's probabilities were rounded, so delta is off by some of its rounding, and the sum of the row's ds, which
@@ -540,6 +691,29 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dq(Args a) {
     p[0] = PK && !live ? -INFINITY : nl;
     p[a.T] = live ? -(delta + sum) : 0.f;
   }
+}
+
+// dq of the rows whose keys were shared, and what k_attn_dkv gets of them.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dq_join(Args a, int pieces) {
+  const Joint jt(a, blockIdx.x / pieces);
+  if (jt.parts == 1) return;
+  jt.each(a, pieces, [&](int row, int64_t line, int d) {
+    const bool live = jt.at.live(row);
+    f32x4 x = {};
+#pragma unroll 16
+    for (int sp = 0; sp < jt.parts; ++sp) x += *reinterpret_cast<const f32x4*>(a.part_q + part_at(a, sp, line, jt.hq) * a.D + d);
+    u32x2 v;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v[i] = live ? pack2<T>(x[2 * i] * a.scale, x[2 * i + 1] * a.scale) : 0;
+    *reinterpret_cast<u32x2*>(a.dq + (line * a.Hq + jt.hq) * a.D + d) = v;
+    if (d > 0) return;
+    float sum = a.ml[part_at(a, 0, line, jt.hq) * 2 + 1];
+    for (int sp = 0; sp < jt.parts; ++sp) sum += a.ml[part_at(a, sp, line, jt.hq) * 2];
+    float* const p = a.stat + (int64_t)jt.hq * 2 * a.T + line;
+    p[0] = live ? -a.lse[(int64_t)jt.hq * a.T + line] : -INFINITY;
+    p[a.T] = live ? -sum : 0.f;
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------------- dk, dv

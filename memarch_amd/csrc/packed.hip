@@ -113,13 +113,15 @@ struct Plan {
   int64_t uq, uk;           // units of rows of q and of keys
   int n_sb, S_s, S_r;
   int64_t part_s, part_r;   // floats of the parts
+  int fold, S_q;
+  int64_t part_q;           // rows of the parts of the rows' sums
 };
 
 // How many workgroups may share a key block's rows (the kernels use fewer where its rows are few). Lengths are not known
 // here: key blocks are shared where there are too few of them to fill the GPU, blocks with first tokens of windowed
 // sequences, which every later row sees, until there are 2048 workgroups for them.
 Plan make_plan(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
-  Plan p = {N / BQ + nseq + 2, M / BKV + nseq + 2, 0, 1, 1, 0, 0};
+  Plan p = {N / BQ + nseq + 2, M / BKV + nseq + 2, 0, 1, 1, 0, 0, 1, 1, 0};
   // parts that a block can have when it sees n rows
   auto most_parts = [&](int64_t n) { return ((n + BR - 1) / BR * (Hq / Hkv) + MIN_PACK - 1) / MIN_PACK; };
   const bool windowed = window > 0 && window < M;
@@ -135,6 +137,21 @@ Plan make_plan(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int6
   p.S_r = (int)std::clamp(std::min(s, most_parts(rows)), int64_t(1), int64_t(16));
   p.part_s = p.S_s > 1 ? nseq * p.n_sb * Hkv * p.S_s * 2 * BKV * D : 0;
   p.part_r = p.S_r > 1 ? p.uk * Hkv * p.S_r * 2 * BKV * D : 0;
+  // Few rows: the keys of a block are shared where the workgroups are not half of the 512 that run at once, and a block of
+  // the mean saves 16 tiles, as the parts and their launch take the time of about 8 (one sequence of 2048 tokens, 8 heads:
+  // 43 us alone and 45 shared; 4096 tokens, 4 heads: 61 and 42; 4 x 16 rows behind 16384 keys: 293 and 46). Long blocks are cut
+  // finer, into parts of 32 tiles (1500 rows behind 131072 keys: 1920 us in two parts, 1710 so); more than 64 take longer to
+  // join than they save (1 row behind 131072 keys, 16 heads over 4: 95 us with 32, 66 with 64, 97 with 128).
+  p.fold = Hq / Hkv % 4 == 0 ? 4 : (Hq / Hkv % 2 == 0 ? 2 : 1);
+  const int64_t keys = windowed && window + sinks + BQ < M ? window + sinks + BQ : M, tiles = keys / BK;
+  const int64_t blocks = (N * p.fold / BQ + nseq) * (Hq / p.fold);
+  if (N > 0 && nseq > 0 && blocks <= 256) {
+    const int64_t mean = std::min(keys, M / nseq - N / nseq / 2);
+    const int64_t fill = std::min(512 / blocks, tiles / MIN_KEYS), fine = std::min(1024 / blocks, mean / (32 * BK));
+    const int64_t S = std::min(std::max(fill, fine), int64_t(64));
+    if (mean * (S - 1) >= 16 * BK * S) p.S_q = (int)S;
+  }
+  p.part_q = p.S_q > 1 ? p.S_q * N * Hq : 0;
   return p;
 }
 
@@ -173,6 +190,9 @@ Args make_args(Strided q, Strided k, Strided v, const int32_t* cu, const int32_t
   a.n_sb = p.n_sb;
   a.S_s = p.S_s;
   a.S_r = p.S_r;
+  a.S_q = p.S_q;
+  a.fold = p.fold;
+  a.thin = N <= nseq * (BQ / p.fold);
   a.scale = scale;
   return a;
 }
@@ -182,24 +202,42 @@ Args make_args(Strided q, Strided k, Strided v, const int32_t* cu, const int32_t
 // 7 of which are its kernel; 13 of 3846 with a window 1307 and 1251).
 int64_t plan_bytes_of(const Plan& p, int64_t nseq, int64_t M, int64_t Hq) {
   const int64_t seqs = nseq + 2;
-  return p.uq * Hq <= 512 || M < 1024 * nseq ? 0 : (p.uq + p.uk) * (int64_t)sizeof(Unit) + 8 * seqs;
+  return p.uq * Hq <= 512 || p.S_q > 1 || M < 1024 * nseq ? 0 : (p.uq + p.uk) * (int64_t)sizeof(Unit) + 8 * seqs;
 }
+
+// Bytes of the parts of the rows' sums, and of the two numbers of each.
+int64_t sums_bytes(const Plan& p, int64_t D) { return align256(p.part_q * D * 4); }
+int64_t split_bytes(const Plan& p, int64_t D) { return sums_bytes(p, D) + align256(p.part_q * 8); }
+unsigned split_grid(const Args& a) { return ((unsigned)(a.Hkv * a.uq * a.S_q) + 7) / 8 * 8 * a.grp; }
+constexpr int JOIN_PIECES = 4;   // workgroups per block of rows that join parts
 
 template <typename T, int DP>
 int launch_fwd(const Args& a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.Hq * a.uq)), joins((unsigned)(a.Hq * a.uq * JOIN_PIECES));
+  if (a.S_q > 1) {
+    hipLaunchKernelGGL((k_attn_fwd<T, DP, true, true>), dim3(split_grid(a)), dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((k_attn_fwd_join<T>), joins, dim3(256), 0, st, a, JOIN_PIECES);
+    return finish();
+  }
   if (a.plan != nullptr) {
     hipLaunchKernelGGL(k_attn_plan, dim3(a.r != nullptr ? 2 : 1), dim3(PLAN_THREADS), 0, st, a);
     const int rc = finish();
     if (rc) return rc;
   }
-  hipLaunchKernelGGL((k_attn_fwd<T, DP, true>), dim3((unsigned)(a.Hq * a.uq)), dim3(THREADS), 0, st, a);
+  hipLaunchKernelGGL((k_attn_fwd<T, DP, true, false>), grid, dim3(THREADS), 0, st, a);
   return finish();
 }
 
 template <typename T, int DP>
 int launch_bwd(const Args& a, hipStream_t st) {
   if (a.T > 0) {
-    hipLaunchKernelGGL((k_attn_dq<T, DP, true>), dim3((unsigned)(a.Hq * a.uq)), dim3(THREADS), 0, st, a);
+    const dim3 grid((unsigned)(a.Hq * a.uq)), joins((unsigned)(a.Hq * a.uq * JOIN_PIECES));
+    if (a.S_q > 1) {
+      hipLaunchKernelGGL((k_attn_dq<T, DP, true, true>), dim3(split_grid(a)), dim3(THREADS), 0, st, a);
+      hipLaunchKernelGGL((k_attn_dq_join<T>), joins, dim3(256), 0, st, a, JOIN_PIECES);
+    } else {
+      hipLaunchKernelGGL((k_attn_dq<T, DP, true, false>), grid, dim3(THREADS), 0, st, a);
+    }
     const int rc = finish();
     if (rc) return rc;
   }
@@ -238,7 +276,7 @@ int mce_serve_last_hip_error(void) { return mce_attn_hip_error; }
 int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                  int64_t v_st, int64_t v_sh, const int32_t* cu, const int32_t* cu_k, int64_t nseq, int64_t N, int64_t M,
                  int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks, float scale, int dtype, void* out,
-                 void* res, float* lse, void* plan, size_t plan_bytes, void* stream) {
+                 void* res, float* lse, void* plan, size_t plan_bytes, void* ws, size_t ws_bytes, void* stream) {
   int rc = check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks);
   if (rc) return rc;
   if (!good_scale(scale) || (dtype != MCE_ATTN_BF16 && dtype != MCE_ATTN_F16) || (cu_k == nullptr && N != M))
@@ -251,6 +289,9 @@ int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   const int64_t need = plan_bytes_of(p, nseq, M, Hq);
   if (need > 0 && (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 255) || plan_bytes < (size_t)need))
     return MCE_ATTN_EWORKSPACE;
+  const int64_t split = split_bytes(p, D);
+  if (split > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < (size_t)split))
+    return MCE_ATTN_EWORKSPACE;
   Args a = make_args({static_cast<const uint16_t*>(q), 0, q_st, q_sh}, {static_cast<const uint16_t*>(k), 0, k_st, k_sh},
                      {static_cast<const uint16_t*>(v), 0, v_st, v_sh}, cu, cu_k, nseq, N, M, Hq, Hkv, D, window, sinks,
                      scale, p);
@@ -258,6 +299,8 @@ int mce_pack_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   a.o = static_cast<uint16_t*>(out);
   a.r = static_cast<uint16_t*>(res);
   a.lse = lse;
+  a.part_q = static_cast<float*>(ws);
+  a.ml = split > 0 ? a.part_q + sums_bytes(p, D) / 4 : nullptr;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dtype == MCE_ATTN_BF16) return D <= 64 ? launch_fwd<__bf16, 64>(a, st) : launch_fwd<__bf16, 128>(a, st);
   return D <= 64 ? launch_fwd<_Float16, 64>(a, st) : launch_fwd<_Float16, 128>(a, st);
@@ -269,11 +312,17 @@ size_t mce_pack_plan_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64
   return (size_t)plan_bytes_of(make_plan(nseq, N, M, Hq, Hkv, D, window, sinks), nseq, M, Hq);
 }
 
+size_t mce_pack_fwd_ws_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                             int64_t sinks) {
+  if (check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks)) return 0;
+  return (size_t)split_bytes(make_plan(nseq, N, M, Hq, Hkv, D, window, sinks), D);
+}
+
 size_t mce_pack_bwd_ws_bytes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                              int64_t sinks) {
   if (check_sizes(nseq, N, M, Hq, Hkv, D, window, sinks)) return 0;
   const Plan p = make_plan(nseq, N, M, Hq, Hkv, D, window, sinks);
-  return (size_t)(align256(N * Hq * 8) + align256(p.part_s * 4) + align256(p.part_r * 4));
+  return (size_t)(align256(N * Hq * 8) + align256(p.part_s * 4) + align256(p.part_r * 4) + split_bytes(p, D));
 }
 
 int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
@@ -302,8 +351,9 @@ int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   const bool planned = N > 0 && plan_bytes_of(p, nseq, M, Hq) > 0;
   if (planned && (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 255))) return MCE_ATTN_EWORKSPACE;
   const int64_t stat = align256(N * Hq * 8), part_s = align256(p.part_s * 4), part_r = align256(p.part_r * 4);
-  if (stat + part_s + part_r > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) ||
-                                     ws_bytes < (size_t)(stat + part_s + part_r)))
+  const int64_t all = stat + part_s + part_r + split_bytes(p, D);
+  if (all > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) ||
+                  ws_bytes < (size_t)all))
     return MCE_ATTN_EWORKSPACE;
   Args a = make_args({static_cast<const uint16_t*>(q), 0, q_st, q_sh}, {static_cast<const uint16_t*>(k), 0, k_st, k_sh},
                      {static_cast<const uint16_t*>(v), 0, v_st, v_sh}, cu, cu_k, nseq, N, M, Hq, Hkv, D, window, sinks,
@@ -316,6 +366,8 @@ int mce_pack_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64
   a.stat = static_cast<float*>(ws);
   a.part_s = a.stat + stat / 4;
   a.part_r = a.part_s + part_s / 4;
+  a.part_q = a.part_r + part_r / 4;
+  a.ml = a.part_q + sums_bytes(p, D) / 4;
   a.dq = static_cast<uint16_t*>(dq);
   a.dk = static_cast<uint16_t*>(dk);
   a.dv = static_cast<uint16_t*>(dv);

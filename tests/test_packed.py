@@ -176,9 +176,9 @@ def test_pack_c_abi_checks_need_no_gpu(lib):
     p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 256
 
     def fwd(q=p, st=64, sh=64, k=p, cu=p, cu_k=p, nseq=2, N=8, M=9, Hq=2, Hkv=1, D=64, window=0, sinks=0, scale=0.1, dtype=1,
-            out=p, res=None, plan=None, nb=0):
+            out=p, res=None, plan=None, nb=0, ws=None, wb=0):
         return lib.mce_pack_fwd(q, st, sh, k, 64, 64, p, 64, 64, cu, cu_k, nseq, N, M, Hq, Hkv, D, window, sinks, scale,
-                                dtype, out, res, None, plan, nb, None)
+                                dtype, out, res, None, plan, nb, ws, wb, None)
 
     for kw in (dict(N=-1), dict(M=-1), dict(nseq=-1), dict(Hq=3, Hkv=2), dict(Hkv=0), dict(D=60), dict(D=136), dict(D=0),
                dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(dtype=0), dict(q=None),
@@ -193,6 +193,13 @@ def test_pack_c_abi_checks_need_no_gpu(lib):
     assert plan > 0 and lib.mce_pack_plan_bytes(2, 8, 9, 2, 1, 64, 0, 0) == 0
     big = dict(N=8000, M=9000, Hq=64)
     assert fwd(**big) == 3 and fwd(**big, plan=p, nb=plan - 1) == 3 and fwd(**big, plan=p + 16, nb=plan) == 3
+
+    few = lib.mce_pack_fwd_ws_bytes(2, 8, 9000, 2, 1, 64, 0, 0)
+    assert few >= 2 * 8 * 2 * 66 * 4 and lib.mce_pack_fwd_ws_bytes(2, 8, 9, 2, 1, 64, 0, 0) == 0
+    assert lib.mce_pack_plan_bytes(2, 8, 9000, 2, 1, 64, 0, 0) == 0
+    assert lib.mce_pack_bwd_ws_bytes(2, 8, 9000, 2, 1, 64, 0, 0) >= few + 2 * 2 * 8 * 4
+    row = dict(N=8, M=9000)
+    assert fwd(**row) == 3 and fwd(**row, ws=p, wb=few - 1) == 3 and fwd(**row, ws=p + 16, wb=few) == 3
 
     need = lib.mce_pack_bwd_ws_bytes(2, 8, 9, 2, 1, 64, 0, 0)
     assert need >= 2 * 2 * 8 * 4 and lib.mce_pack_bwd_ws_bytes(2, 8, 9, 3, 2, 64, 0, 0) == 0
