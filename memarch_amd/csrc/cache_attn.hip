@@ -14,12 +14,12 @@
 // No value crosses lanes. A value's scale goes into its probability's exponent: w_j = exp(s_j) scale_j is what multiplies
 // the codes, and the denominator adds up w_j / scale_j.
 // Codes come through LDS, whole memory lines by neighbouring lanes: loads straight into the registers that the products
-// want them in took one request per 16 bytes, and 240 us where this takes 215 (8 sequences, 131072 tokens each, 4 heads of
-// 128; 5.2 TB/s in the kernel). Each wave has its own two tiles in LDS and walks its own keys without barriers. Where the
+// want them in took one request per 16 bytes, and 240 us where this took 215 (8 sequences, 131072 tokens each, 4 heads of
+// 128; 200 us now, 5.4 TB/s). Each wave has its own two tiles in LDS and walks its own keys without barriers. Where the
 // codes lie is worked out for 16 tiles at once, a group of 8 tokens per lane (as scalar loads of page numbers and scales,
 // whose counter the reads of LDS share, a tile took 1.44 us alone on its CU; 1.03 so).
 // Workgroups share the batch's tiles evenly (struct Cut): 64 sequences of 5000 tokens, 4 heads of 128, with the write of
-// the new token and the join 84 us; one part size for all, 91; a fixed number of parts for each sequence 96.
+// the new token and the join 84 us (81 now); one part size for all, 91; a fixed number of parts for each sequence 96.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
