@@ -1,6 +1,6 @@
 """CPU oracle for the 8-bit key/value cache (memarch_amd.kv_cache).
 
-TEST INFRASTRUCTURE ONLY. Only tests/ may import this module, as the checker; the product path never calls it.
+TEST INFRASTRUCTURE ONLY. Only tests/ may import this module, as the oracle; the product path never calls it.
 
 torch on the CPU in fp64, one block after the other. Codes are kept as the e4m3 values that they stand for:
     nearest8(x)  to nearest, ties to even, 3 bits behind the leading one, steps of 2^-9 at least, up to 448
