@@ -441,3 +441,32 @@ def test_gradients_against_differences():
         want = float((move * grads[i].double().cpu()).sum())
         assert off < 0.15 * abs(want), (i, off, want)   # the comparison says something
         assert abs(out[0] - out[1] - want) <= off, (i, out, want, off)
+
+
+def test_calls_from_several_threads():
+    """Steps of different kinds from several threads, each on a stream of its own, have the bits of those made alone."""
+    import threading
+    cases = [([300], [300], 4, 2, 64, 50), ([3], [4000], 4, 1, 64, 0), ([6000, 4000], [6000, 4000], 8, 2, 64, 0),
+             ([20, 30], [2500, 2700], 2, 2, 128, 0)]
+    made = []
+    for lens, keys, hq, hkv, d, window in cases:
+        x = [t.cuda() for t in _inputs(sum(lens), sum(keys), hq, hkv, d, BF, seed=d)] + [_cu(lens).cuda(), _cu(keys).cuda()]
+        made.append((x, window, _step(*x, window)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        x, window, ref = made[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got = _step(*x, window)
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, ref)):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
