@@ -12,7 +12,9 @@
 //           the other operand where it is; bytes of two keys are put side by side (one permutation per 4 bytes) and
 //           converted in pairs. Product i gives the columns (DP/16) row + i.
 // No value crosses lanes. A value's scale goes into its probability's exponent: w_j = exp(s_j) scale_j is what multiplies
-// the codes, and the denominator adds up w_j / scale_j.
+// the codes. The denominator has an exponential and a maximum of its own: where scales lie far apart (a block of zeros has 2^-100)
+// the w_j next to the largest are lost in fp32, while their exp(s_j) count (8 sequences of 131072 tokens: 203.4 us with the
+// denominator from w_j / scale_j, 204.1 so; 1 of 1000 16.1 and 16.6).
 // Codes come through LDS, whole memory lines by neighbouring lanes: loads straight into the registers that the products
 // want them in took one request per 16 bytes, and 240 us where this took 215 (8 sequences, 131072 tokens each, 4 heads of
 // 128; 200 us now, 5.4 TB/s). Each wave has its own two tiles in LDS and walks its own keys without barriers. Where the
@@ -46,7 +48,7 @@ struct Args {
   Paged g;
   const int32_t* lengths;
   uint16_t* out;
-  float *part, *ml;        // parts of the sums [2 W, Hq, D]; their maxima and denominators [2 W, Hq, 2]
+  float *part, *ml;        // parts of the outputs [2 W, Hq, D]; their maxima and denominators [2 W, Hq, 2]
   int Hq, Hkv, grp, ng, D; // ng: workgroups that share a key/value head's query heads
   int page, max_pages, window, sinks;
   int B, W, G, total;      // W: workgroups per head that share the batch's tiles (0: one per sequence); G: those in a row on
@@ -148,7 +150,7 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
   constexpr int VB = DP / 16, VW = DP / 64;             // value columns per lane, their dwords
   constexpr int IMG = BK * DP;                          // bytes of a tile's keys or values
   __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * IMG];   // two tiles per wave
-  __shared__ float stat[NW][2][CB * HC];
+  __shared__ float stat[NW][3][CB * HC];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, quad = lane >> 4;
   // Workgroups go to the 8 XCDs in turn: those of G neighbouring heads, whose rows share memory lines, follow each other on
@@ -186,11 +188,13 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
         if (col < a.D && hd < heads)
           qf[cb][ks] = *reinterpret_cast<const u32x4*>(a.q + b * a.q_sb + (h0 + hd) * a.q_sh + col);
       }
+    // l = sum_j 2^(s_j - m), acc = sum_j 2^(s_j - m - u) scale_j code_j: m a maximum of the scores s_j (times log2 e), u one of
+    // s_j - m + log2 scale_j
     f32x4 acc[CB][VB] = {};
-    float m[CB], l[CB];
+    float m[CB], l[CB], u[CB];
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
-      m[cb] = -INFINITY;
+      m[cb] = u[cb] = -INFINITY;
       l[cb] = 0.f;
     }
     const float c = a.scale * LOG2E;
@@ -315,41 +319,39 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
         }
       wait_reads();
       load(then.k, then.rows, kst_b, ko, buf);
-      const float kc = ks * c, lv = __builtin_amdgcn_logf(vs), rv = __builtin_amdgcn_rcpf(vs);
+      const float kc = ks * c, lv = __builtin_amdgcn_logf(vs);
       u32x4 pf[CB];
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
-        float x[8], mx = -INFINITY;
-        auto weigh = [&]() {                              // log2 of exp(score) scale, over the maximum kept
-          const float d = lv - (m[cb] == -INFINITY ? 0.f : m[cb]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = __builtin_fmaf(sc[cb][e / 4][e % 4], kc, d);
-            if (edge) x[e] = (see >> e & 1) ? x[e] : -INFINITY;
-          }
-        };
-        weigh();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
-        // the sums are rescaled only when some head's maximum has grown by more than LAZY since the last time
-        if (__builtin_amdgcn_ballot_w64(mx > (m[cb] == -INFINITY ? -INFINITY : LAZY)) != 0) {
-          mx = fmaxf(mx, __shfl_xor(mx, 16));
-          mx = max_halves(mx);
-          const float top = m[cb] == -INFINITY ? mx : m[cb] + fmaxf(mx, 0.f);
-          const float al = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[cb] - top);
-          m[cb] = top;
-          l[cb] *= al;
-#pragma unroll
-          for (int i = 0; i < VB; ++i) acc[cb][i] *= al;
-          weigh();
-        }
-        float sum = 0.f;
+        auto over_heads = [](float y) { return max_halves(fmaxf(y, __shfl_xor(y, 16))); };   // a head's maximum
+        float x[8], mx = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(x[e]);
-          sum += x[e];
+          x[e] = sc[cb][e / 4][e % 4] * kc;
+          if (edge) x[e] = (see >> e & 1) ? x[e] : -INFINITY;
+          mx = fmaxf(mx, x[e]);
         }
-        l[cb] = __builtin_fmaf(sum, rv, l[cb]);
+        const float mu0 = m[cb] == -INFINITY ? 0.f : m[cb];
+        // the sums are rescaled only when some head's maximum has grown by more than LAZY since the last time
+        if (__builtin_amdgcn_ballot_w64((mx - m[cb] > LAZY) | (mx - mu0 + lv - u[cb] > LAZY)) != 0) {
+          const float top = fmaxf(m[cb], over_heads(mx)), by = top == -INFINITY ? 0.f : m[cb] - top;
+          l[cb] *= __builtin_amdgcn_exp2f(by);
+          m[cb] = top;
+          const float y = over_heads(mx - (top == -INFINITY ? 0.f : top) + lv);
+          const float un = fmaxf(u[cb] + by, y);
+          const float al = un == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(u[cb] + by - un);
+          u[cb] = un;
+#pragma unroll
+          for (int i = 0; i < VB; ++i) acc[cb][i] *= al;
+        }
+        const float mu = m[cb] == -INFINITY ? 0.f : m[cb], d = lv - (u[cb] == -INFINITY ? 0.f : u[cb]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] -= mu;
+          sum += __builtin_amdgcn_exp2f(x[e]);
+          x[e] = __builtin_amdgcn_exp2f(x[e] + d);
+        }
+        l[cb] += sum;
 #pragma unroll
         for (int e = 0; e < 4; ++e) pf[cb][e] = pack2<T>(x[2 * e], x[2 * e + 1]);
       }
@@ -426,6 +428,7 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
       if (quad == 0) {
         stat[wave][0][cb * HC + r16] = m[cb];
         stat[wave][1][cb * HC + r16] = l[cb];
+        stat[wave][2][cb * HC + r16] = u[cb];
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -441,23 +444,30 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
     for (int i = threadIdx.x; i < heads * (DP / 4); i += THREADS) {
       const int hd = i / (DP / 4), d = i % (DP / 4) * 4;
       if (d >= a.D) continue;
-      float mm = -INFINITY, ll = 0.f;
+      float mm = -INFINITY, ll = 0.f, t[NW], top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < NW; ++w) mm = fmaxf(mm, stat[w][0][hd]);
       const float mu = mm == -INFINITY ? 0.f : mm;
-      f32x4 o = {};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float f = __builtin_amdgcn_exp2f(stat[w][0][hd] - mu);
-        ll = __builtin_fmaf(stat[w][1][hd], f, ll);
-        o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * 4 * IMG) + hd * DP + d) * f;
+        t[w] = stat[w][0][hd] - mu;
+        ll = __builtin_fmaf(stat[w][1][hd], __builtin_amdgcn_exp2f(t[w]), ll);
+        t[w] += stat[w][2][hd];
+        top = fmaxf(top, t[w]);
       }
+      top = top == -INFINITY ? 0.f : top;
+      f32x4 o = {};
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+        o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * 4 * IMG) + hd * DP + d) *
+             __builtin_amdgcn_exp2f(t[w] - top);
+      // nothing seen: 0; NaN stays
+      o *= (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll)) * __builtin_amdgcn_exp2f(top);
       const int64_t row = (int64_t)b * a.Hq + h0 + hd;
       if (alone) {
-        const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);   // nothing seen: 0; NaN stays
         u32x2 w;
-        w[0] = pack2<T>(o[0] * inv, o[1] * inv);
-        w[1] = pack2<T>(o[2] * inv, o[3] * inv);
+        w[0] = pack2<T>(o[0], o[1]);
+        w[1] = pack2<T>(o[2], o[3]);
         *reinterpret_cast<u32x2*>(a.out + row * a.D + d) = w;
       } else {
         const int64_t to = (int64_t)place0 * a.Hq + h0 + hd;
@@ -475,8 +485,9 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
   }
 }
 
-// out = the parts of one query head joined: one wave per head, 2 columns per lane, 64 parts at a time. Their states are
-// read by all lanes at once and their factors shared through LDS, so that the sums' loads depend on nothing. A wave looks at
+// out = the parts of one query head joined, each by its share of the denominator: one wave per head, 2 columns per lane, 64
+// parts at a time. Their states are read by all lanes at once and their factors shared through LDS, so that the sums' loads
+// depend on nothing. A wave looks at
 // a sequence, or, where workgroups are fewer, at the place where one of them ends, and takes the sequence that goes on there
 // for the first time (4096 sequences, 32 heads: 433 us by sequences, 57 by ends).
 template <typename T>
@@ -502,14 +513,15 @@ __global__ __launch_bounds__(64) void k_cache_join(Args a) {
   for (int s = lane; s < n; s += 64) mm = fmaxf(mm, a.ml[row(s) * 2]);
   for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
   const float mu = mm == -INFINITY ? 0.f : mm;
+  auto own = [&](int s) { return a.ml[row(s) * 2 + 1] * __builtin_amdgcn_exp2f(a.ml[row(s) * 2] - mu); };
   float ll = 0.f, x = 0.f, y = 0.f;
+  for (int s = lane; s < n; s += 64) ll += own(s);
+  for (int o = 32; o > 0; o >>= 1) ll += __shfl_xor(ll, o);
+  const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);   // nothing seen: 0; NaN stays
   for (int s0 = 0; s0 < n; s0 += 64) {
     const int s = s0 + lane, c = n - s0 < 64 ? n - s0 : 64;
     __syncthreads();
-    if (s < n) {
-      f[lane] = __builtin_amdgcn_exp2f(a.ml[row(s) * 2] - mu);
-      ll = __builtin_fmaf(a.ml[row(s) * 2 + 1], f[lane], ll);
-    }
+    if (s < n) f[lane] = own(s) * inv;
     __syncthreads();
     if (d < a.D) {
 #pragma unroll 8
@@ -520,9 +532,7 @@ __global__ __launch_bounds__(64) void k_cache_join(Args a) {
       }
     }
   }
-  for (int o = 32; o > 0; o >>= 1) ll += __shfl_xor(ll, o);
-  const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);   // nothing seen: 0; NaN stays
-  if (d < a.D) *reinterpret_cast<uint32_t*>(a.out + ((int64_t)b * a.Hq + h) * a.D + d) = pack2<T>(x * inv, y * inv);
+  if (d < a.D) *reinterpret_cast<uint32_t*>(a.out + ((int64_t)b * a.Hq + h) * a.D + d) = pack2<T>(x, y);
 }
 
 // --------------------------------------------------------------------------------------------------------- host side
