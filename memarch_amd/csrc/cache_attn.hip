@@ -188,8 +188,8 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
         if (col < a.D && hd < heads)
           qf[cb][ks] = *reinterpret_cast<const u32x4*>(a.q + b * a.q_sb + (h0 + hd) * a.q_sh + col);
       }
-    // l = sum_j 2^(s_j - m), acc = sum_j 2^(s_j - m - u) scale_j code_j: m a maximum of the scores s_j (times log2 e), u one of
-    // s_j - m + log2 scale_j
+    // l = sum_j 2^((s_j - m) c), acc = sum_j 2^((s_j - m) c - u) scale_j code_j: m a maximum of the scores s_j before they are
+    // scaled, u one of (s_j - m) c + log2 scale_j
     f32x4 acc[CB][VB] = {};
     float m[CB], l[CB], u[CB];
 #pragma unroll
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
         }
       wait_reads();
       load(then.k, then.rows, kst_b, ko, buf);
-      const float kc = ks * c, lv = __builtin_amdgcn_logf(vs);
+      const float lv = __builtin_amdgcn_logf(vs);
       u32x4 pf[CB];
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
@@ -327,17 +327,17 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
         float x[8], mx = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = sc[cb][e / 4][e % 4] * kc;
+          x[e] = sc[cb][e / 4][e % 4] * ks;
           if (edge) x[e] = (see >> e & 1) ? x[e] : -INFINITY;
           mx = fmaxf(mx, x[e]);
         }
         const float mu0 = m[cb] == -INFINITY ? 0.f : m[cb];
         // the sums are rescaled only when some head's maximum has grown by more than LAZY since the last time
-        if (__builtin_amdgcn_ballot_w64((mx - m[cb] > LAZY) | (mx - mu0 + lv - u[cb] > LAZY)) != 0) {
-          const float top = fmaxf(m[cb], over_heads(mx)), by = top == -INFINITY ? 0.f : m[cb] - top;
+        if (__builtin_amdgcn_ballot_w64(((mx - m[cb]) * c > LAZY) | ((mx - mu0) * c + lv - u[cb] > LAZY)) != 0) {
+          const float top = fmaxf(m[cb], over_heads(mx)), by = top == -INFINITY ? 0.f : (m[cb] - top) * c;
           l[cb] *= __builtin_amdgcn_exp2f(by);
           m[cb] = top;
-          const float y = over_heads(mx - (top == -INFINITY ? 0.f : top) + lv);
+          const float y = over_heads((mx - (top == -INFINITY ? 0.f : top)) * c + lv);
           const float un = fmaxf(u[cb] + by, y);
           const float al = un == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(u[cb] + by - un);
           u[cb] = un;
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
         const float mu = m[cb] == -INFINITY ? 0.f : m[cb], d = lv - (u[cb] == -INFINITY ? 0.f : u[cb]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] -= mu;
+          x[e] = (x[e] - mu) * c;
           sum += __builtin_amdgcn_exp2f(x[e]);
           x[e] = __builtin_amdgcn_exp2f(x[e] + d);
         }
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(THREADS, waves_per_simd(DP, CB)) void k_cache_attn(
       const float mu = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        t[w] = stat[w][0][hd] - mu;
+        t[w] = (stat[w][0][hd] - mu) * c;
         ll = __builtin_fmaf(stat[w][1][hd], __builtin_amdgcn_exp2f(t[w]), ll);
         t[w] += stat[w][2][hd];
         top = fmaxf(top, t[w]);
@@ -512,8 +512,8 @@ __global__ __launch_bounds__(64) void k_cache_join(Args a) {
   float mm = -INFINITY;
   for (int s = lane; s < n; s += 64) mm = fmaxf(mm, a.ml[row(s) * 2]);
   for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
-  const float mu = mm == -INFINITY ? 0.f : mm;
-  auto own = [&](int s) { return a.ml[row(s) * 2 + 1] * __builtin_amdgcn_exp2f(a.ml[row(s) * 2] - mu); };
+  const float mu = mm == -INFINITY ? 0.f : mm, c = a.scale * LOG2E;
+  auto own = [&](int s) { return a.ml[row(s) * 2 + 1] * __builtin_amdgcn_exp2f((a.ml[row(s) * 2] - mu) * c); };
   float ll = 0.f, x = 0.f, y = 0.f;
   for (int s = lane; s < n; s += 64) ll += own(s);
   for (int o = 32; o > 0; o >>= 1) ll += __shfl_xor(ll, o);

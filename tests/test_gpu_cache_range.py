@@ -1,4 +1,4 @@
-"""cache_attention at the ends of its range: scales as far apart as cache_write makes them."""
+"""cache_attention at the ends of its range: scales as far apart as cache_write makes them, scores of any finite size."""
 import pytest
 import torch
 
@@ -139,3 +139,88 @@ def test_scales_of_keys_far_from_one(dt, move):
     for x, f in ((q, 0), (far, move)):
         out = cache_attention(x.cuda(), *_cached(k * 2.0 ** f, v, s * 2.0 ** f, s), lens).double().cpu()
         assert ((out - ref).abs() <= tol).all(), f
+
+
+def _blocks_of(values, power, g):
+    """Scales [b, n / BLOCK, h] of 2^power over 1, 2 or 4: `values`, multiples of 2^power, have codes of different sizes then."""
+    b, n, h, _ = values.shape
+    return 2.0 ** power / 2.0 ** torch.randint(0, 3, (b, n // BLOCK, h), generator=g).double()
+
+
+def _spread_values(b, n, h, d, g):
+    vscale = torch.exp2(torch.randint(-4, 4, (b, n // BLOCK, h), generator=g).double())
+    return torch.randint(-15, 16, (b, n, h, d), generator=g).double() * vscale.repeat_interleave(BLOCK, 1)[..., None], vscale
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 3)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt,power,scale", [(BF, 0, 2e4), (BF, 10, None), (BF, 0, 1e9), (BF, 4, 1.0), (BF, 14, 1.0), (BF, 58, None),
+                                            (HF, 13, None), (HF, 15, None), (HF, 0, 1e12)])
+def test_scores_of_any_finite_size(dt, power, scale, d, window, sinks):
+    """Scores from 1e4 to 1e36: q and k hold -1, 0 and 1 times a power of two, so that scores are exact and either equal or too
+    far apart to share a softmax: the output is the mean of v over the highest scores, whatever their blocks' scales. Exponentials
+    are powers of two then, so what rounds is the result (u), fp32 sums (2^-24 a key) and the division (2^-20)."""
+    from memarch_amd.kv_cache import cache_attention
+    g = torch.Generator().manual_seed(power + d)
+    for lens in ([200, 183, 1], [20000]):
+        b, n = len(lens), -(-max(lens) // PAGE) * PAGE
+        k = torch.randint(-1, 2, (b, n, 2, d), generator=g).double() * 2.0 ** power
+        v, vscale = _spread_values(b, n, 2, d, g)
+        q = torch.randint(-1, 2, (b, 4, d), generator=g).to(dt) * 2.0 ** power
+        assert torch.isfinite(q).all() and q.dtype == dt
+        out = cache_attention(q.cuda(), *_cached(k, v, _blocks_of(k, power, g), vscale), torch.tensor(lens).cuda(),
+                              window=window or None, sinks=sinks, scale=scale).double().cpu()
+        for i, m in enumerate(lens):
+            j = torch.arange(m)
+            j = j[(m - 1 - j < window) | (j < sinks)] if window else j
+            kk, vv = (x[i, j].repeat_interleave(2, 1).transpose(0, 1) for x in (k, v))
+            s = (q[i].double()[:, None] @ kk.mT)[:, 0]
+            p = (s == s.amax(-1, keepdim=True)).double()
+            p = (p / p.sum(-1, keepdim=True))[:, None]
+            ref, mag = (p @ vv)[:, 0], (p @ vv.abs())[:, 0]
+            tol = (torch.finfo(dt).eps / 2 * ref.abs() + (m * 2.0 ** -24 + 2.0 ** -20) * mag) * 1.01
+            assert ((out[i] - ref).abs() <= tol).all(), (i, float((out[i] - ref).abs().max()))   # (NaN fails it too)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 16, 2.0 ** 20, 2.0 ** 24, 2.0 ** 28, 2.0 ** 31, 2.0 ** 32, 2.0 ** 60])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dt", [BF, HF], ids=["bf16", "fp16"])
+def test_equal_keys_of_large_scores(dt, sign, size):
+    """One key row everywhere, of any score (both signs): the mean of v; and a sequence of one token: its value. The scores are equal
+    to the last bit (codes and scales differ by powers of two), so the bound is that of the test above."""
+    from memarch_amd.kv_cache import cache_attention
+    g = torch.Generator().manual_seed(9)
+    lens, d = [1, 64, 333, 20000], 64
+    n = 20000
+    row = torch.randint(1, 4, (4, 1, 2, d), generator=g).double()
+    k = row.expand(4, n, 2, d).contiguous()
+    v, vscale = _spread_values(4, n, 2, d, g)
+    q = (sign * torch.rand(4, 4, d, generator=g)).to(dt)
+    most = float((q.double().abs() * row[:, 0].repeat_interleave(2, 1)).sum(-1).max())
+    out = cache_attention(q.cuda(), *_cached(k, v, _blocks_of(k, 0, g), vscale), torch.tensor(lens).cuda(),
+                          scale=size / most).double().cpu()
+    for i, m in enumerate(lens):
+        vv = v[i, :m].repeat_interleave(2, 1)
+        ref, mag = vv.mean(0), vv.abs().mean(0)
+        tol = (torch.finfo(dt).eps / 2 * ref.abs() + (m * 2.0 ** -24 + 2.0 ** -20) * mag) * 1.01
+        assert ((out[i] - ref).abs() <= tol).all(), (m, float((out[i] - ref).abs().max()))
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_next_to_the_largest_number(sign):
+    """Scores of 3.2e38, which fp32 holds and their product with log2 e does not: the mean of v, as above."""
+    from memarch_amd.kv_cache import cache_attention
+    g = torch.Generator().manual_seed(10)
+    lens, d, n = [1, 64, 333, 20000], 64, 20000
+    row = torch.randint(1, 4, (4, 1, 2, d), generator=g).double() * 2.0 ** 60
+    v, vscale = _spread_values(4, n, 2, d, g)
+    q = (sign * 2.0 ** 60 * torch.rand(4, 4, d, generator=g)).to(BF)
+    most = float((q.double().abs() * row[:, 0].repeat_interleave(2, 1)).sum(-1).max())
+    k = row.expand(4, n, 2, d).contiguous()
+    out = cache_attention(q.cuda(), *_cached(k, v, _blocks_of(k, 60, g), vscale), torch.tensor(lens).cuda(),
+                          scale=3.2e38 / most).double().cpu()
+    for i, m in enumerate(lens):
+        vv = v[i, :m].repeat_interleave(2, 1)
+        ref, mag = vv.mean(0), vv.abs().mean(0)
+        tol = (torch.finfo(BF).eps / 2 * ref.abs() + (m * 2.0 ** -24 + 2.0 ** -20) * mag) * 1.01
+        assert ((out[i] - ref).abs() <= tol).all(), (m, float((out[i] - ref).abs().max()))
