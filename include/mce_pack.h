@@ -13,7 +13,8 @@
  *
  * Buffers: q and go [N, Hq, D], k and v [M, Hkv, D] with element strides (token, head), the last dimension contiguous,
  * 16-byte aligned, strides multiples of 8, the token stride at least D; D a multiple of 8 up to 128; out, res, dq [N, Hq, D]
- * and dk, dv [M, Hkv, D] contiguous; lse [Hq, N] fp32. N and M are at most 2^27, Hq (N / 128 + nseq + 2) is below 2^24.
+ * and dk, dv [M, Hkv, D] contiguous; lse [Hq, N] fp32. N and M are at most 2^27, Hq (N / 128 + nseq + 2) is below 2^24 and
+ * Hkv (M / 128 + nseq + 2) below 2^23 - 2^11; with a window nseq sinks / 128 is below 2^31.
  * Roundings, ranges and the conventions of the calls are those of mce_attn.h: asynchronous on `stream`, no allocation,
  * arguments checked before anything is launched, MCE_ATTN_E* codes. The split of work depends on the sizes alone, so a
  * captured call may be replayed with other lengths.

@@ -48,10 +48,11 @@ struct Args {
   int n_sb, S_s, S_r;
   float *part_s, *part_r;    // their fp32 parts [B Hkv, block, S, 2, BKV, D] where S > 1
   // Packed sequences (below): B = 1, T = rows of q. [B, T, ...] above are [N, ...] or [head, ..., N], and the parts are
-  // [unit Hkv, S, 2, BKV, D] (part_s: [sequence n_sb Hkv, S, 2, BKV, D]).
+  // [unit Hkv, S, 2, BKV, D].
   const int32_t *cu, *cu_k;  // starts of the nseq sequences in the rows of q and of k, and their ends
   int nseq, M;               // M: rows of k
   int uq, uk;                // units of BQ rows of q and of BKV rows of k
+  int us, by_key;            // units of key blocks with first tokens: n_sb of every sequence, or (by_key) those of k
   struct Unit* plan;         // those of q and then those of k, the longest first; null: in their own order
   // workgroups that share the key tiles of a unit of q (1: SPLIT is false); query heads of each (1, 2 or 4) then, and
   // whether sequences have no more rows on average than one workgroup takes of a head
@@ -722,12 +723,16 @@ __global__ __launch_bounds__(256) void k_attn_dq_join(Args a, int pieces) {
 template <bool PK>
 struct Keys {
   int kb0, len, off, own, t0, nt;
-  bool skip;            // packed: no block of this unit, or one of those with first tokens among the others
+  bool skip;            // packed: no block of this unit, or one of those with first tokens among the others (or the reverse)
   int64_t qrow, krow;
   // blk: the block among those with first tokens, or among the others
   __device__ __forceinline__ Keys(const Args& a, int b, bool sink, int blk) {
     if constexpr (PK) {
-      if (sink) {
+      if (sink && a.by_key) {
+        const Unit x = unit_at<true>(a, blk);
+        set(a, x, true);
+        skip |= x.blk >= a.n_sb || x.outside;
+      } else if (sink) {
         Unit x = unit_of<true>(a, 1 + blk / a.n_sb, 0);
         x.blk = blk % a.n_sb;
         set(a, x, true);
@@ -786,7 +791,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
   __shared__ __attribute__((aligned(1024))) char lds[NS * 2 * IMG];   // Q and go of the ring's tiles
   __shared__ __attribute__((aligned(256))) float stats[NS][2][BR];    // -lse and -delta of their rows
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nsink = PK ? a.nseq * a.n_sb : a.n_sb, nr = PK ? a.uk : (a.T + BKV - 1) / BKV - a.n_sb;
+  const int nsink = PK ? a.us : a.n_sb, nr = PK ? a.uk : (a.T + BKV - 1) / BKV - a.n_sb;
   // workgroups of the blocks with first tokens (the longest) first, then the others, those with the most rows first
   const uint32_t heads = (uint32_t)a.B * a.Hkv, sink_wgs = heads * nsink * a.S_s;
   const bool sink = blockIdx.x < sink_wgs;
@@ -952,7 +957,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_dkv(Args a) {
 // threads).
 template <typename T, bool PK>
 __global__ __launch_bounds__(256) void k_attn_dkv_join(Args a, int pieces) {
-  const int nsink = PK ? a.nseq * a.n_sb : a.n_sb, nr = PK ? a.uk : (a.T + BKV - 1) / BKV - a.n_sb;
+  const int nsink = PK ? a.us : a.n_sb, nr = PK ? a.uk : (a.T + BKV - 1) / BKV - a.n_sb;
   const uint32_t heads = (uint32_t)a.B * a.Hkv, sink_blocks = a.S_s > 1 ? heads * nsink : 0;
   uint32_t w = blockIdx.x / pieces;
   const bool sink = w < sink_blocks;

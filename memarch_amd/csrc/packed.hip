@@ -111,6 +111,7 @@ constexpr int64_t MAX_ROWS = int64_t(1) << 27;
 
 struct Plan {
   int64_t uq, uk;           // units of rows of q and of keys
+  int64_t us;               // units of key blocks with first tokens
   int n_sb, S_s, S_r;
   int64_t part_s, part_r;   // floats of the parts
   int fold, S_q;
@@ -119,23 +120,25 @@ struct Plan {
 
 // How many workgroups may share a key block's rows (the kernels use fewer where its rows are few). Lengths are not known
 // here: key blocks are shared where there are too few of them to fill the GPU, blocks with first tokens of windowed
-// sequences, which every later row sees, until there are 2048 workgroups for them.
+// sequences, which every later row sees, until there are 2048 workgroups for them. Those are taken as the first n_sb of each
+// sequence, or, where that is more than all units of keys (many sequences that cannot all be so long), found among the units.
 Plan make_plan(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t sinks) {
-  Plan p = {N / BQ + nseq + 2, M / BKV + nseq + 2, 0, 1, 1, 0, 0, 1, 1, 0};
+  Plan p = {N / BQ + nseq + 2, M / BKV + nseq + 2, 0, 0, 1, 1, 0, 0, 1, 1, 0};
   // parts that a block can have when it sees n rows
   auto most_parts = [&](int64_t n) { return ((n + BR - 1) / BR * (Hq / Hkv) + MIN_PACK - 1) / MIN_PACK; };
   const bool windowed = window > 0 && window < M;
   if (windowed && sinks > 0) {
     const int64_t most = M / BKV + 1, n = (sinks + BKV - 1) / BKV;
     p.n_sb = (int)(n < most ? n : most);
-    const int64_t units = nseq * p.n_sb * Hkv;
+    p.us = std::min(nseq * p.n_sb, p.uk);
+    const int64_t units = p.us * Hkv;
     const int64_t s = units > 0 ? (2048 + units - 1) / units : 1;
     p.S_s = (int)std::clamp(std::min(s, most_parts(N)), int64_t(1), int64_t(64));
   }
   const int64_t s = (768 + p.uk * Hkv - 1) / (p.uk * Hkv);
   const int64_t rows = windowed && window + BKV + BR < N ? window + BKV + BR : N;
   p.S_r = (int)std::clamp(std::min(s, most_parts(rows)), int64_t(1), int64_t(16));
-  p.part_s = p.S_s > 1 ? nseq * p.n_sb * Hkv * p.S_s * 2 * BKV * D : 0;
+  p.part_s = p.S_s > 1 ? p.us * Hkv * p.S_s * 2 * BKV * D : 0;
   p.part_r = p.S_r > 1 ? p.uk * Hkv * p.S_r * 2 * BKV * D : 0;
   // Few rows: the keys of a block are shared where the workgroups are not half of the 512 that run at once, and a block of
   // the mean saves 16 tiles, as the parts and their launch take the time of about 8 (one sequence of 2048 tokens, 8 heads:
@@ -160,9 +163,9 @@ int check_sizes(int64_t nseq, int64_t N, int64_t M, int64_t Hq, int64_t Hkv, int
     return MCE_ATTN_EINVAL;
   if (N > MAX_ROWS || M > MAX_ROWS || nseq > MAX_GROUPS || Hq * D > MAX_ST) return MCE_ATTN_EINVAL;
   const Plan p = make_plan(nseq, N, M, Hq, Hkv, D, window, sinks);
-  // the sums are below 2^63: sinks' blocks are at most M / BKV + 1 per sequence
-  if (p.uq > MAX_GROUPS / Hq || p.uk * p.S_r > MAX_GROUPS / Hkv ||
-      nseq * p.n_sb * p.S_s > MAX_GROUPS / Hkv - p.uk * p.S_r)
+  // the products are below 2^63: sinks' blocks are at most M / BKV + 1 per sequence
+  if (p.uq > MAX_GROUPS / Hq || p.uk * p.S_r > MAX_GROUPS / Hkv || nseq * p.n_sb > INT32_MAX ||
+      p.us * p.S_s > MAX_GROUPS / Hkv - p.uk * p.S_r)
     return MCE_ATTN_EINVAL;
   return MCE_ATTN_OK;
 }
@@ -181,6 +184,8 @@ Args make_args(Strided q, Strided k, Strided v, const int32_t* cu, const int32_t
   a.M = (int)M;
   a.uq = (int)p.uq;
   a.uk = (int)p.uk;
+  a.us = (int)p.us;
+  a.by_key = p.us < nseq * p.n_sb;
   a.Hq = (int)Hq;
   a.Hkv = (int)Hkv;
   a.grp = (int)(Hq / Hkv);
@@ -242,10 +247,9 @@ int launch_bwd(const Args& a, hipStream_t st) {
     if (rc) return rc;
   }
   if (a.M == 0) return MCE_ATTN_OK;
-  const int64_t nsink = (int64_t)a.nseq * a.n_sb;
-  hipLaunchKernelGGL((k_attn_dkv<T, DP, true>), dim3((unsigned)(a.Hkv * (nsink * a.S_s + (int64_t)a.uk * a.S_r))),
+  hipLaunchKernelGGL((k_attn_dkv<T, DP, true>), dim3((unsigned)(a.Hkv * ((int64_t)a.us * a.S_s + (int64_t)a.uk * a.S_r))),
                      dim3(THREADS), 0, st, a);
-  const int64_t join = a.Hkv * ((a.S_s > 1 ? nsink : 0) + (a.S_r > 1 ? (int64_t)a.uk : 0));
+  const int64_t join = a.Hkv * ((a.S_s > 1 ? (int64_t)a.us : 0) + (a.S_r > 1 ? (int64_t)a.uk : 0));
   // few blocks need many threads each; of many most are not shared, and a workgroup that only finds that out costs 1 ns
   const int64_t all = (2 * BKV * (a.D / 4) + 255) / 256;
   const int pieces = (int)std::clamp(4096 / std::max(join, int64_t(1)), int64_t(1), all);
