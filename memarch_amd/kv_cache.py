@@ -47,6 +47,20 @@ def _codes(cache, scale, shape, name):
     return at, sp, st, sh, scale.data_ptr()
 
 
+def _check_written(k_cache, v_cache, k_scale, v_scale):
+    """Refuses a cache two of whose elements share memory (expanded heads, one buffer for both): several waves would write it."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        span = 1   # of the dimensions with smaller strides
+        for stride, n in () if t.is_contiguous() else sorted(zip(t.stride(), t.shape)):
+            if n > 1:
+                if stride < span:
+                    raise ValueError(f"{name}, which is written, has elements that share memory: {tuple(t.shape)}, strides "
+                                     f"{t.stride()}")
+                span += stride * (n - 1)
+    if k_cache.data_ptr() == v_cache.data_ptr() != 0 or k_scale.data_ptr() == v_scale.data_ptr() != 0:
+        raise ValueError("the keys and values, or their scales, are written to the same memory")
+
+
 def _check_cache(k_cache, v_cache, k_scale, v_scale, block_table):
     """The cache's shape [pages, page, Hkv, D], its block and the table's max_pages."""
     shape = k_cache.shape
@@ -92,12 +106,14 @@ def cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lengths, 
     has lengths[b] with them (int32 or int64 [B], the argument that cache_attention takes afterwards); without it row b is
     sequence b's one new token. A block of slots that gets tokens keeps those in front of them; its scale grows with what is
     written, never shrinks while it holds older tokens, and starts anew with its first slot. Tokens whose page is outside
-    the cache (entries of -1, say) are left out. A page that gets tokens must belong to one sequence."""
+    the cache (entries of -1, say) are left out. A page that gets tokens must belong to one sequence. A cache whose elements
+    share memory raises."""
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, Hkv, D]")
     if k.dtype not in _DTYPES or v.dtype != k.dtype:
         raise ValueError(f"k and v must both be bfloat16 or both float16, got {k.dtype} and {v.dtype}")
     shape, block, most = _check_cache(k_cache, v_cache, k_scale, v_scale, block_table)
+    _check_written(k_cache, v_cache, k_scale, v_scale)
     pages, page, h, d = shape
     if k.shape[1:] != (h, d):
         raise ValueError(f"k {tuple(k.shape)} does not fit a cache of {h} heads of {d}")
