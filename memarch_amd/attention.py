@@ -126,6 +126,28 @@ def _forward(q, k, v, lengths, window, sinks, scale, train):
     return q, k, v, out, res, lse
 
 
+def _mark_leaves(out, dev):
+    """Leaves the current stream's number on the gradient accumulators of the call's leaves, which live as long as a graph
+    that uses them."""
+    here = _stream(dev)
+    for node, _ in out.grad_fn.next_functions:
+        if node is not None and type(node).__name__ == "AccumulateGrad":
+            node.metadata.setdefault("memarch_stream", here)
+
+
+def _check_capture(ctx, dev):
+    """Refuses to capture a backward whose leaves an earlier graph still holds: autograd makes their accumulators wait on
+    the stream where that graph was made, which draws the stream into the capture and ends the process."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    here = _stream(dev)
+    for node, _ in ctx.next_functions:
+        if node is not None and type(node).__name__ == "AccumulateGrad" and \
+                node.metadata.get("memarch_stream", here) != here:
+            raise RuntimeError("a backward cannot be captured while a graph of the same leaves that was made on another "
+                               "stream is alive: delete its outputs first, or capture with detached leaves")
+
+
 class _WindowAttention(torch.autograd.Function):
     """forward(ctx, q, k, v, lengths, window, sinks, scale) -> out; backward -> dq, dk, dv."""
 
@@ -140,6 +162,7 @@ class _WindowAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, go):
         q, k, v, out, res, lse, lengths = ctx.saved_tensors
+        _check_capture(ctx, q.device)
         window, sinks, scale = ctx.mask
         B, T, Hq, D = q.shape
         Hkv = k.shape[2]
@@ -164,7 +187,9 @@ def window_attention(q, k, v, window=None, sinks=0, lengths=None, scale=None):
     by none, their output and gradients are 0 and what lies in their rows is not read (inside a length, a NaN or an
     infinity may reach rows near it that do not see it, as 0 * NaN does in a dense form). scale defaults to D^-0.5.
     Under torch.autocast fp32 tensors are cast to its type, as for scaled_dot_product_attention. Differentiable once
-    in q, k and v, in reverse mode: a tensor with a forward-mode tangent raises."""
+    in q, k and v, in reverse mode: a tensor with a forward-mode tangent raises. Capturing a backward raises while an earlier
+    graph of leaves that are q, k or v themselves, made here or by packed_attention on another stream, is alive (as for any
+    operator, one of leaves farther up must not be)."""
     if torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         q, k, v = (t.to(dt) if t.dtype is torch.float32 else t for t in (q, k, v))
@@ -178,7 +203,9 @@ def window_attention(q, k, v, window=None, sinks=0, lengths=None, scale=None):
     _check_same(q, ("k", k), ("v", v), ("lengths", lengths))
     _check_tangents(q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
+        out = _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
+        _mark_leaves(out, q.device)
+        return out
     return _forward(q, k, v, lengths, window, sinks, scale, False)[3]
 
 
@@ -196,28 +223,6 @@ def _packed_forward(q, k, v, cu, cu_k, window, sinks, scale, train):
         _lib.call("mce_pack_fwd", *qs, *ks, *vs, cu.data_ptr(), _ptr(cu_k), *sizes, scale, _DTYPES[q.dtype], out.data_ptr(),
                   _ptr(res), _ptr(lse), _ptr(plan), n, _ptr(ws), w, _stream(q.device))
     return q, k, v, out, res, lse, plan
-
-
-def _mark_leaves(out, dev):
-    """Leaves the current stream's number on the gradient accumulators of the call's leaves, which live as long as a graph
-    that uses them."""
-    here = _stream(dev)
-    for node, _ in out.grad_fn.next_functions:
-        if node is not None and type(node).__name__ == "AccumulateGrad":
-            node.metadata.setdefault("memarch_stream", here)
-
-
-def _check_capture(ctx, dev):
-    """Refuses to capture a backward whose leaves an earlier graph still holds: autograd makes their accumulators wait on
-    the stream where that graph was made, which draws the stream into the capture and ends the process."""
-    if not torch.cuda.is_current_stream_capturing():
-        return
-    here = _stream(dev)
-    for node, _ in ctx.next_functions:
-        if node is not None and type(node).__name__ == "AccumulateGrad" and \
-                node.metadata.get("memarch_stream", here) != here:
-            raise RuntimeError("a backward cannot be captured while a graph of the same leaves that was made on another "
-                               "stream is alive: delete its outputs first, or capture with detached leaves")
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -285,9 +290,8 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, window=None, sinks=
     rows of their own for each sequence, and a sequence's queries are the last of its positions (the next piece of a text
     whose earlier keys are at hand): row i of n is position i + m - n of m. Rows that see nothing (m < n, or outside every
     sequence) and the gradients of rows that nothing sees are 0. The numbers stay on the device: they are not checked, a
-    call does not wait for them, and a captured call may be replayed with others. Capturing a backward raises while an
-    earlier graph of leaves that are q, k or v themselves, made by this function on another stream, is alive (as for any
-    operator, one of leaves farther up must not be)."""
+    call does not wait for them, and a captured call may be replayed with others. Capturing a backward raises where that of
+    window_attention does."""
     if torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         q, k, v = (t.to(dt) if t.dtype is torch.float32 else t for t in (q, k, v))
