@@ -673,6 +673,13 @@ def bench_swiglu(args):
     print(json.dumps(res), flush=True)
 
 
+def cache_bytes(written, seen, hkv, d, block):
+    """Bytes of the 8-bit cache's traffic, keys and values: `written` tokens of 2 bytes an element stored as codes of 1, `seen` tokens'
+    codes read; a scale of 4 bytes per `block` tokens and head on either side."""
+    scale = 4 / block
+    return round(2 * hkv * (written * (3 * d + scale) + seen * (d + scale)))
+
+
 def bench_attention(args):
     """One attention operator (--op) through its public entry point, timed with torch events on the current stream."""
     from memarch_amd import attention, kv_cache, rotary
@@ -705,7 +712,7 @@ def bench_attention(args):
             def step():
                 kv_cache.cache_write(k, v, *cache, lens, cu)
                 kv_cache.cache_read(*cache, cu, b * t)
-            nbytes, flops = 2 * 6 * k.numel(), 0
+            nbytes, flops = cache_bytes(b * t, b * t, hkv, d, block) + 2 * 2 * k.numel(), 0   # and what comes back, 2 bytes each
         else:
             q, k, v = mk(b, h, d), mk(b, hkv, d), mk(b, hkv, d)
             lens = torch.randint(most // 3, most + 1, (b,), generator=gen, device=dev).int()
@@ -714,7 +721,7 @@ def bench_attention(args):
             def step():
                 kv_cache.cache_write(k, v, *cache, lens)
                 kv_cache.cache_attention(q, *cache, lens, window=window, sinks=sinks)
-            nbytes, flops = int(seen.sum()) * 2 * hkv * (d + 4 // block) + 4 * b * h * d, int(seen.sum()) * 4 * h * d
+            nbytes, flops = cache_bytes(b, int(seen.sum()), hkv, d, block) + 4 * b * h * d, int(seen.sum()) * 4 * h * d
             config["heads"] = h
     elif args.op == "packed_attention":
         lens = [(400 + 1013 * i) % 2600 for i in range(23)]
