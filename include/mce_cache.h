@@ -27,15 +27,22 @@
  *   out_bh = sum_j p_j v_j,  p = softmax over the seen j of scale q_bh . k_j     (nothing seen: out = 0)
  * Codes are exact in the element type, so the first product's operands are exact; sums are fp32; exp(score) times the
  * value's scale is rounded to the element type as operand of the second product, and the result is rounded once. Scales
- * are positive, finite and between 2^-100 and 2^120; those of blocks without a seen token are not used.
+ * are positive, finite and between 2^-100 and 2^120; those of blocks without a seen token are not used. The denominator is
+ * fp32 however far scales are apart, and scores may be of any finite size; what operands of the second product lose is what lies
+ * below the type's range next to the largest exp(score) times scale (2^-25 of it in fp16).
  *
  * Buffers: k, v [N, Hkv, D] and q [B, Hq, D] in 16 bits with element strides (token, head; batch, head for q), 16-byte
  * aligned, strides multiples of 8; caches with strides (page, slot, head) in bytes, 16-byte aligned, strides multiples of
  * 16, slots at least D apart; the last dimension contiguous everywhere; results contiguous. D is a multiple of 16 up to
- * 128, page a multiple of 8 up to 65536, block a multiple of 8 up to 128 that divides page. cu as in mce_pack.h: numbers
- * outside 0 .. N count as the nearest of the two; where they fall, what is written is not defined, but lies inside the
- * buffers. Calls are asynchronous on `stream`, allocate nothing and return 0 or an MCE_ATTN_E* code; arguments are checked
- * before anything is launched, and the split of work depends on sizes alone.
+ * 128, page a multiple of 8 up to 65536, block a multiple of 8 up to 128 that divides page. Two elements of a cache that is
+ * written must not share memory. cu as in mce_pack.h: numbers outside 0 .. N count as the nearest of the two; where they fall,
+ * what is written is not defined, but lies inside the buffers. Launches hold fewer than 2^24 workgroups: a write takes
+ * 2 Hkv (N / block + 2 B) below that (cu NULL: 2 Hkv B), a read (rows / 8 + B + 2) / 2, an attention B Hq below 2^24 - 2^20.
+ * Calls are asynchronous on `stream`, allocate nothing and return 0 or an MCE_ATTN_E* code; arguments are checked before anything
+ * is launched. Grids depend on sizes alone, so a captured call may be replayed with other lengths. Where the attention shares the
+ * batch's tiles among workgroups evenly (small batches, and large ones of long caches), the places at which a sequence's sums are
+ * cut depend on the lengths of all sequences: its last bits may change when a neighbour grows, and are the same for the same
+ * lengths.
  */
 #ifndef MCE_CACHE_H
 #define MCE_CACHE_H

@@ -60,7 +60,7 @@ __device__ __forceinline__ int codes2(float x, float y, float f, int w) {
 // are shared by a workgroup's waves (SPLIT): as one wave each they left the GPU short of waves (20011 tokens, 2 heads of
 // 96, blocks of 128: 12.1 us, 10.1 so). Earlier codes are read only when the scale grows. Sequence b's blocks are the units
 // from floor(cu[b] / block) + 2 b on: n tokens touch at most floor(n / block) + 2 blocks.
-// Bound by HBM: 65536 tokens, 8 heads of 128, blocks of 32, 403 MB: 74 us, 5.5 TB/s.
+// Bound by HBM: 65536 tokens, 8 heads of 128, blocks of 32, 403 MB: 67 us, 6.0 TB/s.
 // ONCE: the new rows are read past the caches.
 template <typename T, int DP, int NL, bool SPLIT, bool ONCE>
 __global__ __launch_bounds__(THREADS, 4) void k_cache_write(WriteArgs a) {
@@ -179,7 +179,7 @@ constexpr int HEADS = 4;   // loads of 16 bytes per lane under way at once
 
 // A wave takes 8 neighbouring tokens (which lie in one page) of the keys or the values, and some of the heads: 16 codes per
 // lane and load, whole 128-byte lines on both sides. Rows before the first sequence and behind the last are taken as
-// sequences without pages, so every row is written. Bound by HBM: 98304 tokens, 8 heads of 128, 604 MB: 132 us, 4.6 TB/s, two
+// sequences without pages, so every row is written. Bound by HBM: 98304 tokens, 8 heads of 128, 604 MB: 135 us, 4.5 TB/s, two
 // thirds of it writes. Sequence s's groups are the units from floor(start / 8) + s on.
 // ONCE: the results are written past the caches.
 template <typename T, int DP, bool ONCE>
@@ -252,10 +252,10 @@ __global__ __launch_bounds__(THREADS) void k_cache_read(ReadArgs a) {
 
 // --------------------------------------------------------------------------------------------------------- host side
 
-// So many bytes of new rows are read, and of results written, past the caches (loads and stores of the non-temporal kind):
-// with their lines and those of what was there before, the last cache (256 MiB) would not keep them for the next kernel.
+// So many bytes of new rows are read, and of results written, past the caches (loads and stores of the non-temporal kind).
 // 65536 tokens written and 98304 read back, 8 heads of 128: 227 us without, 214 with the results past them, 217 with the
-// rows, 201 with both; 20011 and 120014, 2 heads of 96: 53 and 42 (the results).
+// rows, 201 with both; 20011 and 120014, 2 heads of 96: 53 and 42 (the results). Both are passes with nobody who reads the results
+// behind them: what such a kernel loses where the last cache (256 MiB) would have held them is not measured.
 constexpr int64_t LARGE_BYTES = int64_t(1) << 26;
 
 template <typename T, int DP, bool ONCE>

@@ -202,9 +202,12 @@ Args make_args(Strided q, Strided k, Strided v, const int32_t* cu, const int32_t
   return a;
 }
 
-// Bytes of the plan: none where all workgroups of the forward run at once, or sequences are so short that none is left over
-// for long (24 sequences of 1365 tokens on average, 16 heads, a training step: 1393 us in their own order, 1377 with the plan,
-// 7 of which are its kernel; 13 of 3846 with a window 1307 and 1251).
+// Bytes of the plan: none where all workgroups of the forward run at once, and with sequences below 1024 tokens on average.
+// Steps in their own order and with the plan, whose kernel takes 7 us of it, in us: 49999 tokens, 16 heads over 4, D = 64, window
+// 1024, mean 4096: 1289 and 1214, 1365: 1071 and 974; 32768 tokens, 16 heads, D = 128, no window, mean 1365: 1406 and 1412. Below
+// the line it pays too where workgroups are many (65536 tokens, 16 heads over 4, D = 128, no window, mean 256: 1201 and 1143; 64:
+// 1184 and 1078), and not where they are few or short (the forward alone of 65536 tokens, 8 heads over 2, D = 64, window 128, mean
+// 512: 61 and 66; of 8192, 16 over 4, window 64, mean 256: 22 and 26).
 int64_t plan_bytes_of(const Plan& p, int64_t nseq, int64_t M, int64_t Hq) {
   const int64_t seqs = nseq + 2;
   return p.uq * Hq <= 512 || p.S_q > 1 || M < 1024 * nseq ? 0 : (p.uq + p.uk) * (int64_t)sizeof(Unit) + 8 * seqs;

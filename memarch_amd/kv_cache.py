@@ -173,7 +173,8 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths,
     """paged_attention over the 8-bit cache: attention of one new token per sequence, q [B, Hq, D] (bf16 or fp16, Hq a
     multiple of Hkv) -> [B, Hq, D]. lengths [B] (int32 or int64) counts a sequence's tokens with the new one, which
     cache_write has put there. The mask is that of window_attention's last row. A sequence of length 0 gives 0; tokens in
-    pages outside the cache (entries of -1, say) and past max_pages are not seen."""
+    pages outside the cache (entries of -1, say) and past max_pages are not seen. The same call gives the same bits; the last
+    bits of a sequence may differ between batches whose other lengths differ, as those decide where its sums are cut."""
     shape, block, most = _check_cache(k_cache, v_cache, k_scale, v_scale, block_table)
     pages, page, h, d = shape
     if q.dim() != 3 or q.shape[2] != d or q.shape[1] < 1 or q.shape[1] % h:
